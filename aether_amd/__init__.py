@@ -90,6 +90,15 @@ _SIGS = {
     "aeth_attn_decode": (_INT, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P]),
     "aeth_attn_decode_noalloc": (_INT, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P]),
     "aeth_attn_prefill": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P, _P]),
+    "aeth_qk_norm_rope": (_INT, [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, ctypes.c_float, _I64, _P, _P, _P, _I64, _P,
+                                 _I64, _P]),
+    "aeth_kv8_layer_bytes": (_I64, [_I64, _I64, _I64]),
+    "aeth_kv8_append": (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
+    "aeth_kv8_append_batch": (_INT, [_P, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
+    "aeth_kv8_read": (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
+    "aeth_attn_kv8_ws_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "aeth_attn_kv8": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
+    "aeth_attn_kv8_batch": (_INT, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
     "aeth_silu_mul": (_INT, [_P, _P, _I64, _P]),
     "aeth_add": (_INT, [_P, _P, _I64, _P]),
     "aeth_argmax": (_INT, [_P, _I64, _P, _P]),

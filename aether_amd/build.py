@@ -27,6 +27,8 @@ SOURCES = [
     "aeth_decode_ops.hip",
     "aeth_prefill.hip",
     "aeth_backend.hip",
+    "aeth_kv8.hip",
+    "aeth_attn_kv8.hip",
     "aeth_host.cpp",
     "aeth_blas.cpp",
     "aeth_runner.cpp",
@@ -52,6 +54,7 @@ EXTRA = {
     "aeth_gemm_q80.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "aeth_gemm_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "aeth_gemm_gq.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "aeth_attn_kv8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 COMMON = [

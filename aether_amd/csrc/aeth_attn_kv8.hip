@@ -1,0 +1,471 @@
+// Attention over the 8-bit cache (aeth_kv8.hpp): GQA, causal, with a sliding window.
+//
+// Query i of n stands at position p = len - n + i of a sequence of len tokens and sees the keys
+// max(0, p - window + 1) .. p. A column is one (query, head): column x = i·G + head of the G query
+// heads that share a KV head; 16 columns fill the int8 matrix product
+//   Sᵀ[64 tokens][16] = K[64][hd] · Qᵀ,   Oᵀ[hd][16] += Vᵀ[hd][64] · Pᵀ
+// on v_mfma_i32_16x16x64_i8. The codes are one operand as they stand. q and the probabilities enter
+// as integers of 24 bits, three balanced base-256 digits d2·65536 + d1·256 + d0 with d in [-128, 127]:
+// three int8 products whose i32 sums are exact. So
+//  * a score carries q rounded to 2^-23 of its row's largest component (|q·2^e| in [2^22, 2^23)), as
+//    keys are held to 2^-8 of theirs, and nothing else but the f32 roundings of its final products;
+//  * p·sv (the probability times the token's V scale) is rounded to 2^-23 of the largest of its column
+//    in a tile of 64 tokens, whatever the running maximum: neither a flat row nor a tile far below
+//    the maximum loses bits. Tiles are summed in f32.
+// Running maximum and sum in f32, in log2 units; the partials are rescaled only when some column's
+// maximum grows by more than 2^8 (the result does not depend on which maximum is used).
+// A masked key's score, probability and V scale are replaced by selects, so infinities and NaN there
+// reach nothing; a visible token whose scale is NaN makes the columns that see it NaN.
+#include <math.h>
+
+#include <algorithm>
+
+#include "aeth_common.hpp"
+#include "aeth_internal.hpp"
+#include "aeth_kv8.hpp"
+#include "aeth_ops_internal.hpp"
+
+typedef int a8_i4 __attribute__((ext_vector_type(4)));
+typedef float a8_f4 __attribute__((ext_vector_type(4)));
+
+namespace {
+
+struct A8 {
+    const float* q;         // [seqs][n] rows of q_stride floats
+    int64_t q_stride;
+    const uint8_t* cache;
+    int64_t seq_bytes;
+    const int* lens;        // [seqs]: len = lens[seq] + len_add, clamped to [0, max_len]; nullptr: max_len
+    int len_add, max_len;
+    int n, nq, nkv, G, cols;  // queries, query heads, KV heads, query heads a KV head, n·G
+    int tiles;              // tiles a head's slice holds
+    int window;             // 0: none
+    int ncb, chunks, tpc;   // column blocks, chunks of tpc tiles
+    float* out;             // [seqs][n][nq·hd]
+    float* ws;              // partials when chunks > 1
+    int qvec, ovec;         // q rows / out 16-byte aligned
+};
+
+__device__ __forceinline__ float a8_max_rows(float v) { return aeth_max_rows(v); }
+
+// 2^j of the largest j with |x|·2^j <= 0x7F7F00 for |x| <= mx (three balanced digits), as its exponent;
+// 0 for mx = 0, infinite or NaN
+__device__ __forceinline__ int a8_exponent(float mx) {
+    if (!(mx > 0.0f && mx < INFINITY)) return 0;
+    int e;
+    (void)frexpf(mx, &e);
+    int j = min(23 - e, 126);
+    if (ldexpf(mx, j) > 8355584.0f) j--;
+    return max(j, -126);
+}
+__device__ __forceinline__ float a8_pow2(int j) { return __int_as_float((127 + j) << 23); }
+
+// four integers of 24 bits (in the low bits of f32 words 2^23 + X or of plain words) → their digits'
+// words; each byte is digit + 128 before the exclusive or
+__device__ __forceinline__ void a8_digits(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t& d0, uint32_t& d1, uint32_t& d2) {
+    a += 0x808080u;
+    b += 0x808080u;
+    c += 0x808080u;
+    d += 0x808080u;
+    const uint32_t p = __builtin_amdgcn_perm(b, a, 0x05010400u), q = __builtin_amdgcn_perm(d, c, 0x05010400u);
+    const uint32_t s = __builtin_amdgcn_perm(b, a, 0x0C0C0602u), t = __builtin_amdgcn_perm(d, c, 0x0C0C0602u);
+    d0 = __builtin_amdgcn_perm(q, p, 0x05040100u) ^ 0x80808080u;
+    d1 = __builtin_amdgcn_perm(q, p, 0x07060302u) ^ 0x80808080u;
+    d2 = __builtin_amdgcn_perm(t, s, 0x05040100u) ^ 0x80808080u;
+}
+
+__device__ __forceinline__ int a8_len(const A8& A, int seq) {
+    if (!A.lens) return A.max_len;
+    const int64_t l = (int64_t)A.lens[seq] + A.len_add;
+    return (int)min(max(l, (int64_t)0), (int64_t)A.max_len);
+}
+
+// The tiles some column of columns [c0, c0 + count) sees: [beg, end)
+__device__ __forceinline__ void a8_tiles(const A8& A, int len, int c0, int count, int& beg, int& end) {
+    const int i0 = c0 / A.G, i1 = min(c0 + count, A.cols) - 1;
+    const int hi = len - A.n + i1 / A.G + 1;                                      // keys < hi
+    const int lo = A.window > 0 ? max(0, len - A.n + i0 + 1 - A.window) : 0;
+    beg = lo >> 6;
+    end = hi > 0 ? (hi + 63) >> 6 : 0;
+    if (end < beg) end = beg;
+}
+
+// Workgroup (KV head, column block of 16·NC, chunk, sequence): its four waves take the chunk's tiles round
+// robin, each with its own running softmax, and merge through LDS.
+template <int HD, int NC>
+__global__ void __launch_bounds__(256) k_attn8(A8 A) {
+    constexpr int KS = HD / 64, DT = HD / 16, PLD = HD + 4;
+    constexpr float TH = 8.0f;
+    __shared__ __attribute__((aligned(16))) float po[4][16 * NC][PLD];
+    __shared__ float pm[4][16 * NC], pl[4][16 * NC];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, g = lane >> 4;
+    int id = blockIdx.x;
+    const int h = id % A.nkv;
+    id /= A.nkv;
+    const int cb = A.ncb - 1 - id % A.ncb;  // late queries, the longest rows, first
+    const int chunk = id / A.ncb, seq = blockIdx.y;
+    const int len = a8_len(A, seq);
+    int beg, end;
+    a8_tiles(A, len, cb * 16 * NC, 16 * NC, beg, end);
+    const int t0 = beg + chunk * A.tpc, t1 = min(t0 + A.tpc, end);
+    if (t0 >= t1 && chunk > 0) return;  // (uniform) the merge leaves it out
+    const uint8_t* head = A.cache + seq * A.seq_bytes + (int64_t)h * A.tiles * aeth_kv8_tile_bytes(HD);
+
+    a8_i4 kf[4][KS], vf[DT];
+    a8_f4 sk[4], sv[4];
+    auto load = [&](int t) {
+        const uint8_t* p = head + (int64_t)t * aeth_kv8_tile_bytes(HD);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int s = 0; s < KS; s++) kf[j][s] = *(const a8_i4*)(p + (16 * j + c) * HD + 64 * s + 16 * g);
+#pragma unroll
+        for (int j = 0; j < 4; j++) sk[j] = *(const a8_f4*)(p + 2 * KV8_TILE * HD + 4 * (16 * j + 4 * g));
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) vf[dt] = *(const a8_i4*)(p + KV8_TILE * HD + (16 * dt + c) * KV8_TILE + 16 * g);
+#pragma unroll
+        for (int j = 0; j < 4; j++) sv[j] = *(const a8_f4*)(p + 2 * KV8_TILE * HD + 4 * (KV8_TILE + 16 * j + 4 * g));
+    };
+    if (t0 + w < t1) load(t0 + w);
+
+    // the columns: q's digits, the keys [lo, hi) they see
+    uint32_t qd[NC][3][KS][4];
+    float qs[NC], m[NC], l[NC];
+    int lo[NC], hi[NC];
+    a8_f4 o[NC][DT];
+#pragma unroll
+    for (int u = 0; u < NC; u++) {
+        const int x = cb * 16 * NC + 16 * u + c, xc = min(x, A.cols - 1), i = xc / A.G;
+        const float* src = A.q + ((int64_t)seq * A.n + i) * A.q_stride + (int64_t)(h * A.G + xc % A.G) * HD + 16 * g;
+        float qv[KS][16], mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                float4 y;
+                if (A.qvec) y = *(const float4*)(src + 64 * s + e);
+                else y = make_float4(src[64 * s + e], src[64 * s + e + 1], src[64 * s + e + 2], src[64 * s + e + 3]);
+                qv[s][e] = y.x;
+                qv[s][e + 1] = y.y;
+                qv[s][e + 2] = y.z;
+                qv[s][e + 3] = y.w;
+            }
+        uint32_t mb = 0;
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                mb = max(mb, __float_as_uint(qv[s][e]) & 0x7FFFFFFFu);
+            }
+        {   // over the four lane groups, as integers: a NaN's bits are above an infinity's
+            const auto a = __builtin_amdgcn_permlane16_swap(mb, mb, false, false);
+            mb = max(a[0], a[1]);
+            const auto b = __builtin_amdgcn_permlane32_swap(mb, mb, false, false);
+            mb = max(b[0], b[1]);
+        }
+        mx = __uint_as_float(mb);
+        const int e2 = a8_exponent(mx);
+        const float f = a8_pow2(e2);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                a8_digits((uint32_t)(int)rintf(qv[s][e] * f), (uint32_t)(int)rintf(qv[s][e + 1] * f),
+                          (uint32_t)(int)rintf(qv[s][e + 2] * f), (uint32_t)(int)rintf(qv[s][e + 3] * f), qd[u][0][s][e / 4],
+                          qd[u][1][s][e / 4], qd[u][2][s][e / 4]);
+        // an infinity or NaN in q: every score NaN
+        qs[u] = mb >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : a8_pow2(-e2) * (1.4426950408889634f / sqrtf((float)HD));
+        m[u] = -INFINITY;
+        l[u] = 0.0f;
+        hi[u] = len - A.n + i + 1;
+        lo[u] = A.window > 0 ? hi[u] - A.window : 0;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) o[u][dt] = (a8_f4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // every column of the block sees the keys [all_lo, all_hi)
+    const int all_hi = len - A.n + (cb * 16 * NC) / A.G + 1;
+    const int all_lo = A.window > 0 ? len - A.n + (min(cb * 16 * NC + 16 * NC, A.cols) - 1) / A.G + 1 - A.window : 0;
+
+    const a8_i4 zero = {0, 0, 0, 0};
+    for (int t = t0 + w; t < t1; t += 4) {
+        const bool edge = 64 * t < all_lo || 64 * t + 64 > all_hi;  // (uniform) some key is masked
+        // V scales that are no numbers (append writes NaN): rare
+        uint32_t vb = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) vb = max(vb, __float_as_uint(sv[j][r]) & 0x7FFFFFFFu);
+        const bool vbad = __any(vb >= 0x7F800000u);
+#pragma unroll
+        for (int u = 0; u < NC; u++) {
+            float s[16];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                a8_i4 d[3];
+#pragma unroll
+                for (int p = 0; p < 3; p++) {
+                    d[p] = zero;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) {
+                        const a8_i4 b = {(int)qd[u][p][ks][0], (int)qd[u][p][ks][1], (int)qd[u][p][ks][2], (int)qd[u][p][ks][3]};
+                        d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[j][ks], b, d[p], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    s[4 * j + r] = fmaf((float)((d[2][r] << 8) + d[1][r]), 256.0f, (float)d[0][r]) * (sk[j][r] * qs[u]);
+            }
+            float wv[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) wv[i] = sv[i >> 2][i & 3];
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int key = 64 * t + 16 * (i >> 2) + 4 * g + (i & 3);
+                    const bool seen = key >= lo[u] && key < hi[u];
+                    s[i] = seen ? s[i] : -INFINITY;
+                    wv[i] = seen ? wv[i] : 0.0f;
+                }
+            }
+            if (vbad) {
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (!(fabsf(wv[i]) < INFINITY)) {
+                        wv[i] = 0.0f;
+                        l[u] = __uint_as_float(0x7FC00000u);
+                    }
+            }
+            float mx = s[0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
+            mx = a8_max_rows(mx);
+            if (__any(mx > m[u] + TH)) {  // (uniform)
+                const float mn = fmaxf(m[u], mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
+                l[u] *= al;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) o[u][dt] *= al;
+                m[u] = mn;
+            }
+            const float mo = m[u] == -INFINITY ? 0.0f : m[u];  // every key masked so far: s - mo is -Inf
+            float wm = 0.0f, ps = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float p = __builtin_amdgcn_exp2f(s[i] - mo);
+                ps += p;
+                wv[i] *= p;
+                wm = fmaxf(wm, wv[i]);
+            }
+            l[u] += ps;
+            wm = a8_max_rows(wm);
+            if (!(wm < INFINITY)) l[u] = __uint_as_float(0x7FC00000u);  // values past 2^119: no number rather than a wrong one
+            const int j2 = a8_exponent(wm);
+            const float f = a8_pow2(j2), fi = a8_pow2(-j2);
+            uint32_t pd[3][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t x[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) x[r] = __float_as_uint(fmaf(wv[4 * j + r], f, 8388608.0f));
+                a8_digits(x[0], x[1], x[2], x[3], pd[0][j], pd[1][j], pd[2][j]);
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                a8_i4 d[3];
+#pragma unroll
+                for (int p = 0; p < 3; p++) {
+                    const a8_i4 b = {(int)pd[p][0], (int)pd[p][1], (int)pd[p][2], (int)pd[p][3]};
+                    d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[dt], b, zero, 0, 0, 0);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    o[u][dt][r] = fmaf(fmaf((float)((d[2][r] << 8) + d[1][r]), 256.0f, (float)d[0][r]), fi, o[u][dt][r]);
+            }
+        }
+        if (t + 4 < t1) load(t + 4);
+    }
+#pragma unroll
+    for (int u = 0; u < NC; u++) {
+        l[u] = aeth_sum_rows(l[u]);
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) *(a8_f4*)&po[w][16 * u + c][16 * dt + 4 * g] = o[u][dt];
+        if (g == 0) {
+            pm[w][16 * u + c] = m[u];
+            pl[w][16 * u + c] = l[u];
+        }
+    }
+    __syncthreads();
+    const int unit = (seq * A.nkv + h) * A.ncb + cb;
+    float* part = A.ws + ((int64_t)unit * A.chunks + chunk) * (16 * NC) * (HD + 2);
+    for (int at = tid; at < 16 * NC * HD / 4; at += 256) {
+        const int cc = at / (HD / 4), d = 4 * (at % (HD / 4)), x = cb * 16 * NC + cc;
+        if (x >= A.cols) continue;
+        float M = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < 4; v++) M = fmaxf(M, pm[v][cc]);
+        float L = 0.0f;
+        a8_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const float wt = pm[v][cc] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[v][cc] - M);
+            L += wt * pl[v][cc];
+            acc += *(const a8_f4*)&po[v][cc][d] * wt;
+        }
+        if (A.chunks > 1) {
+            *(a8_f4*)(part + cc * HD + d) = acc;
+            if (d == 0) {
+                part[16 * NC * HD + 2 * cc] = M;
+                part[16 * NC * HD + 2 * cc + 1] = L;
+            }
+            continue;
+        }
+        acc = L == 0.0f ? (a8_f4){0.0f, 0.0f, 0.0f, 0.0f} : acc * (1.0f / L);  // a row that sees nothing: 0
+        float* dst = A.out + ((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + d;
+        if (A.ovec) *(a8_f4*)dst = acc;
+        else dst[0] = acc[0], dst[1] = acc[1], dst[2] = acc[2], dst[3] = acc[3];
+    }
+}
+
+// Joins the chunks of one column: a workgroup of hd threads, thread = output dimension
+template <int HD, int NC>
+__global__ void __launch_bounds__(HD) k_attn8_merge(A8 A) {
+    const int d = threadIdx.x, h = blockIdx.x % A.nkv, x = blockIdx.x / A.nkv, seq = blockIdx.y;
+    const int cb = x / (16 * NC), cc = x % (16 * NC);
+    const int len = a8_len(A, seq);
+    int beg, end;
+    a8_tiles(A, len, cb * 16 * NC, 16 * NC, beg, end);
+    const int live = max(1, (end - beg + A.tpc - 1) / A.tpc);
+    const float* part = A.ws + (int64_t)((seq * A.nkv + h) * A.ncb + cb) * A.chunks * (16 * NC) * (HD + 2);
+    float M = -INFINITY;
+    for (int k = 0; k < live; k++) M = fmaxf(M, part[(int64_t)k * (16 * NC) * (HD + 2) + 16 * NC * HD + 2 * cc]);
+    float L = 0.0f, acc = 0.0f;
+    for (int k = 0; k < live; k++) {
+        const float* p = part + (int64_t)k * (16 * NC) * (HD + 2);
+        const float m = p[16 * NC * HD + 2 * cc], wt = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+        L += wt * p[16 * NC * HD + 2 * cc + 1];
+        acc += wt * p[cc * HD + d];
+    }
+    A.out[((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + d] = L == 0.0f ? 0.0f : acc * (1.0f / L);
+}
+
+// Chunks a row block's tiles are split into so that `units` of them fill the chip: two workgroups a CU
+int64_t a8_target() { return 2 * (int64_t)aeth_num_cus(); }
+
+template <int HD, int NC>
+int launch(A8 A, int64_t seqs, hipStream_t s) {
+    const dim3 grid((unsigned)((int64_t)A.nkv * A.ncb * A.chunks), (unsigned)seqs);
+    hipLaunchKernelGGL((k_attn8<HD, NC>), grid, dim3(256), 0, s, A);
+    AETH_LAUNCH_CHECK();
+    if (A.chunks > 1) {
+        hipLaunchKernelGGL((k_attn8_merge<HD, NC>), dim3((unsigned)((int64_t)A.nkv * A.cols), (unsigned)seqs), dim3(HD), 0, s, A);
+        AETH_LAUNCH_CHECK();
+    }
+    return AETH_OK;
+}
+
+}  // namespace
+
+int64_t aeth_attn_kv8_ws(int64_t seqs, int64_t n, int64_t nq, int64_t nkv, int64_t hd, int64_t len) {
+    if (len <= 4 * KV8_TILE) return 0;  // never split
+    // `units` row blocks in fewer than target chunks each, or none split: at most target + units partials, and a
+    // smaller call at most twice the target
+    const int64_t units = seqs * nkv * aeth_cdiv(n * (nq / nkv), 16), target = a8_target();
+    return (target + (units < target ? units : target)) * 32 * (hd + 2) * (int64_t)sizeof(float);
+}
+
+int aeth_attn_kv8_launch(const float* q, int64_t q_stride, const void* cache, int64_t seq_bytes, const int* lens, int len_add,
+                         int64_t seqs, int64_t n, int64_t nq, int64_t nkv, int64_t hd, int64_t max_seq, int64_t max_len,
+                         int64_t window, float* out, void* ws, hipStream_t s) {
+    if (n <= 0 || seqs <= 0) return AETH_OK;
+    A8 A;
+    A.q = q;
+    A.q_stride = q_stride;
+    A.cache = (const uint8_t*)cache;
+    A.seq_bytes = seq_bytes;
+    A.lens = lens;
+    A.len_add = len_add;
+    A.max_len = (int)max_len;
+    A.n = (int)n;
+    A.nq = (int)nq;
+    A.nkv = (int)nkv;
+    A.G = (int)(nq / nkv);
+    A.cols = (int)(n * A.G);
+    A.tiles = (int)aeth_cdiv(max_seq, KV8_TILE);
+    A.window = window > 0 && window < max_len ? (int)window : 0;  // one that reaches past key 0 masks nothing
+    A.out = out;
+    A.ws = (float*)ws;
+    A.qvec = ((uintptr_t)q & 15) == 0 && (q_stride & 3) == 0;
+    A.ovec = ((uintptr_t)out & 15) == 0;
+    const int nc = A.cols > 16 && hd <= 128 ? 2 : 1;  // (two column sets of 256 dimensions do not fit the registers)
+    A.ncb = (int)aeth_cdiv(A.cols, 16 * nc);
+    // the most tiles a column block sees, and the chunks that fill the chip
+    const int64_t rows = aeth_cdiv(16 * nc, A.G) + 1;
+    const int64_t span = A.window ? std::min(aeth_cdiv(max_len, KV8_TILE), (A.window + std::min(rows, n) + 62) / KV8_TILE + 1)
+                                  : aeth_cdiv(max_len, KV8_TILE);
+    const int64_t units = seqs * nkv * A.ncb;
+    const int64_t want = std::max<int64_t>(1, std::min(aeth_cdiv(a8_target(), units), aeth_cdiv(span, 4)));
+    A.tpc = (int)(aeth_cdiv(aeth_cdiv(span, want), 4) * 4);
+    if (A.tpc < 4) A.tpc = 4;
+    A.chunks = (int)std::max<int64_t>(1, aeth_cdiv(span, A.tpc));
+    if (hd == 64) return nc == 1 ? launch<64, 1>(A, seqs, s) : launch<64, 2>(A, seqs, s);
+    if (hd == 128) return nc == 1 ? launch<128, 1>(A, seqs, s) : launch<128, 2>(A, seqs, s);
+    return launch<256, 1>(A, seqs, s);
+}
+
+// what the two entry points ask of their arguments in common
+static int check_attn(const char* what, const float* q, int64_t q_stride, const void* cache, int64_t seqs, int64_t n, int64_t nq,
+                      int64_t nkv, int64_t hd, int64_t max_seq, int64_t max_len, int64_t window, const float* out, const void* ws,
+                      int64_t ws_bytes) {
+    if (!q || !cache || !out || ((uintptr_t)cache & 15) || (((uintptr_t)q | (uintptr_t)out) & 3) || ((uintptr_t)ws & 15))
+        return aeth_set_error(AETH_EINVAL, "%s: bad argument (cache and workspace 16-byte aligned, rows 4-byte)", what);
+    if (nkv <= 0 || nq <= 0 || nq % nkv != 0 || max_seq <= 0 || max_seq > KV8_MAX_SEQ || window < 0 || n < 0 || seqs < 0)
+        return aeth_set_error(AETH_EINVAL, "%s: bad shape (heads %lld / %lld, max_seq %lld, window %lld)", what, (long long)nq,
+                              (long long)nkv, (long long)max_seq, (long long)window);
+    if (!aeth_kv8_head_dim(hd) || nq > 4096)
+        return aeth_set_error(AETH_EUNSUPPORTED, "%s: %lld heads of %lld (head_dim 64, 128 or 256)", what, (long long)nq, (long long)hd);
+    if (max_len < n || max_len > max_seq)
+        return aeth_set_error(AETH_EINVAL, "%s: %lld queries, %lld of %lld positions", what, (long long)n, (long long)max_len, (long long)max_seq);
+    int64_t span;
+    if ((n > 1 || seqs > 1) ? (q_stride < nq * hd || !aeth_mul_ok(seqs * n, q_stride, &span) || span > INT64_MAX / 4) : q_stride < 0)
+        return aeth_set_error(AETH_EINVAL, "%s: query stride %lld of rows of %lld", what, (long long)q_stride, (long long)(nq * hd));
+    if (n * nq > (int64_t)1 << 24 || seqs > 65535 || seqs * n * nq > (int64_t)1 << 28)
+        return aeth_set_error(AETH_EUNSUPPORTED, "%s: %lld x %lld queries of %lld heads in one call", what, (long long)seqs, (long long)n, (long long)nq);
+    const int64_t need = aeth_attn_kv8_ws(seqs, n, nq, nkv, hd, max_len);
+    if (need > 0 && (!ws || ws_bytes < need))
+        return aeth_set_error(AETH_EINVAL, "%s: a workspace of %lld bytes (%lld given)", what, (long long)need, (long long)(ws ? ws_bytes : 0));
+    return AETH_OK;
+}
+
+extern "C" AETH_API int64_t aeth_attn_kv8_ws_bytes(int64_t n_seqs, int64_t n, int64_t n_heads, int64_t kv_heads, int64_t head_dim,
+                                                   int64_t max_len) {
+    if (n_seqs < 0 || n < 0 || kv_heads <= 0 || n_heads <= 0 || n_heads % kv_heads != 0 || n_heads > 4096 || !aeth_kv8_head_dim(head_dim) ||
+        max_len < 0 || max_len > KV8_MAX_SEQ || n_seqs > 65535 || n > (int64_t)1 << 24) {
+        aeth_set_error(AETH_EINVAL, "aeth_attn_kv8_ws_bytes: bad shape");
+        return -1;
+    }
+    return aeth_attn_kv8_ws(n_seqs, n, n_heads, kv_heads, head_dim, max_len);
+}
+
+extern "C" AETH_API int aeth_attn_kv8(const float* d_q, int64_t q_stride, const void* d_layer, int64_t n, int64_t n_heads,
+                                      int64_t kv_heads, int64_t head_dim, int64_t max_seq, int64_t seq, int64_t window,
+                                      float* d_out, void* d_ws, int64_t ws_bytes, void* stream) {
+    const int rc = check_attn("aeth_attn_kv8", d_q, q_stride, d_layer, 1, n, n_heads, kv_heads, head_dim, max_seq, seq, window, d_out, d_ws, ws_bytes);
+    if (rc) return rc;
+    return aeth_attn_kv8_launch(d_q, q_stride, d_layer, 0, nullptr, 0, 1, n, n_heads, kv_heads, head_dim, max_seq, seq, window, d_out,
+                                d_ws, (hipStream_t)stream);
+}
+
+extern "C" AETH_API int aeth_attn_kv8_batch(const float* d_q, int64_t q_stride, const void* d_layers, int64_t layer_stride,
+                                            const int32_t* d_lens, int64_t n_seqs, int64_t n_heads, int64_t kv_heads, int64_t head_dim,
+                                            int64_t max_seq, int64_t max_len, int64_t window, float* d_out, void* d_ws,
+                                            int64_t ws_bytes, void* stream) {
+    const char* what = "aeth_attn_kv8_batch";
+    if (!d_lens || ((uintptr_t)d_lens & 3) || max_len < 1) return aeth_set_error(AETH_EINVAL, "%s: bad argument (lengths)", what);
+    const int rc = check_attn(what, d_q, q_stride, d_layers, n_seqs, 1, n_heads, kv_heads, head_dim, max_seq, max_len, window, d_out, d_ws, ws_bytes);
+    if (rc) return rc;
+    int64_t all;
+    if (layer_stride < 0 || (layer_stride & 15) || !aeth_mul_ok(n_seqs, layer_stride, &all) ||
+        (n_seqs > 1 && layer_stride < kv_heads * aeth_cdiv(max_seq, KV8_TILE) * aeth_kv8_tile_bytes((int)head_dim)))
+        return aeth_set_error(AETH_EINVAL, "%s: %lld sequences %lld bytes apart", what, (long long)n_seqs, (long long)layer_stride);
+    return aeth_attn_kv8_launch(d_q, q_stride, d_layers, layer_stride, d_lens, 0, n_seqs, 1, n_heads, kv_heads, head_dim, max_seq, max_len,
+                                window, d_out, d_ws, (hipStream_t)stream);
+}

@@ -38,3 +38,19 @@ int aeth_prefill_rope_kv_launch(float* qkv, int64_t n, int64_t nh, int64_t nkv, 
 int aeth_attn_prefill_launch(const float* q, int64_t q_stride, const float* layer_kv, int64_t n, int64_t nh,
                              int64_t nkv, int64_t hd, int64_t max_seq, int64_t window, float* out, hipStream_t s);
 int aeth_silu_pairs_launch(const float* gu, int64_t total, float* h, hipStream_t s);
+// The 8-bit cache (aeth_kv8.hip, aeth_attn_kv8.hip; arguments already checked). d_slots: one token a sequence at its
+// slot; otherwise n tokens of one sequence from `slot`.
+int aeth_kv8_append_launch(void* cache, int64_t seq_bytes, const int* d_slots, int64_t seqs, const float* k, const float* v,
+                           int64_t token_stride, int64_t head_stride, int64_t n, int64_t nkv, int64_t hd, int64_t max_seq,
+                           int64_t slot, hipStream_t s);
+int aeth_kv8_read_launch(const void* cache, float* k, float* v, int64_t token_stride, int64_t head_stride, int64_t n,
+                         int64_t nkv, int64_t hd, int64_t max_seq, int64_t slot, hipStream_t s);
+// lens: device lengths (+ len_add, clamped to max_len); nullptr: max_len. ws: aeth_attn_kv8_ws(...) bytes.
+int64_t aeth_attn_kv8_ws(int64_t seqs, int64_t n, int64_t nq, int64_t nkv, int64_t hd, int64_t len);
+int aeth_attn_kv8_launch(const float* q, int64_t q_stride, const void* cache, int64_t seq_bytes, const int* lens, int len_add,
+                         int64_t seqs, int64_t n, int64_t nq, int64_t nkv, int64_t hd, int64_t max_seq, int64_t max_len,
+                         int64_t window, float* out, void* ws, hipStream_t s);
+// head norms and rotation of q | k rows (weights nullptr: that part unnormalised); row i at d_pos[i], else pos + i
+int aeth_qk_norm_rope_launch(const float* x, int64_t x_stride, int64_t n, int64_t n_heads, int64_t kv_heads, int64_t hd,
+                             const float* qw, const float* kw, float eps, int64_t pos, const int* d_pos, const float* sin_t,
+                             const float* cos_t, int64_t max_seq, float* out, int64_t out_stride, hipStream_t s);

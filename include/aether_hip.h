@@ -263,6 +263,79 @@ AETH_API int aeth_attn_decode_noalloc(const float* d_q, const float* d_layer_kv,
 AETH_API int aeth_attn_prefill(const float* d_q, int64_t q_stride, const float* d_layer_kv, int64_t n,
                                int64_t n_heads, int64_t kv_heads, int64_t head_dim, int64_t max_seq, float* d_out,
                                void* stream);
+/* Norms of queries and keys for each head with the position rotation in the same
+ * pass (no counterpart in the reference, whose models have no head norms): rows
+ * of a projection output, row i at d_x + i·x_stride, n_heads query heads of
+ * head_dim, then kv_heads key heads (what follows in a row, the value heads of a
+ * fused projection, is not read). Head by head y = x / sqrt(mean(x²) + eps) · w,
+ * w = d_qw or d_kw (head_dim floats; NULL: those heads unnormalised), as
+ * aeth_rmsnorm, then aeth_rope's rotation by the table row
+ * min(position, max_seq - 1), the position of row i being d_pos[i] (device,
+ * n int32, below 0 taken as 0) or pos + i where d_pos is NULL. Row i of the
+ * result, the heads alone, at d_out + i·out_stride; d_out may be d_x with the
+ * same stride (in place), and else overlaps nothing. head_dim even. */
+AETH_API int aeth_qk_norm_rope(const float* d_x, int64_t x_stride, int64_t n, int64_t n_heads, int64_t kv_heads,
+                               int64_t head_dim, const float* d_qw, const float* d_kw, float eps, int64_t pos,
+                               const int32_t* d_pos, const float* d_sin, const float* d_cos, int64_t max_seq,
+                               float* d_out, int64_t out_stride, void* stream);
+
+/* ── the key/value cache in 8 bits (no counterpart in the reference) ──────
+ * A layer slice of one sequence, aeth_kv8_layer_bytes(...) bytes, 16-byte
+ * aligned: [kv_heads][ceil(max_seq/64)] tiles of 64 tokens, a tile being
+ *   K codes  int8 [64][head_dim]
+ *   V codes  int8 [head_dim][64], token t of the tile at byte
+ *            16·((t/4) % 4) + 4·(t/16) + t % 4 of a row
+ *   K scales float [64], V scales float [64]
+ * Token and head hold s = amax/127 (f32) and the codes 127·x/amax rounded to the
+ * nearest integer, ties to even (the exact quotient's); a code stands for
+ * code·s. All zero: scale and codes 0. A row with an infinity or NaN: scale
+ * NaN, codes 0; it reads back as NaN. Every token has its own scale, so an
+ * append changes no other token, and the bytes do not depend on how a prompt
+ * was split into calls. A slice may start out with any content: slots that
+ * nothing was appended to are never used by a call whose lengths leave them out.
+ * head_dim 64, 128 or 256; max_seq up to 2^30. About a quarter of the f32
+ * cache: 2·head_dim + 8 bytes a token and head. */
+AETH_API int64_t aeth_kv8_layer_bytes(int64_t kv_heads, int64_t head_dim, int64_t max_seq);
+/* Appends n tokens' K and V (token i, head h: head_dim floats at
+ * i·token_stride + h·head_stride of d_k / d_v) to slots slot .. slot + n - 1. */
+AETH_API int aeth_kv8_append(void* d_layer, const float* d_k, const float* d_v, int64_t token_stride,
+                             int64_t head_stride, int64_t n, int64_t kv_heads, int64_t head_dim, int64_t max_seq,
+                             int64_t slot, void* stream);
+/* One token for each of n_seqs sequences, whose slices lie layer_stride bytes (a
+ * multiple of 16) apart: row i to slot d_slots[i] (device) of sequence i. A
+ * slot outside [0, max_seq) takes nothing, as a full StaticKVCache does. */
+AETH_API int aeth_kv8_append_batch(void* d_layers, int64_t layer_stride, const int32_t* d_slots, const float* d_k,
+                                   const float* d_v, int64_t token_stride, int64_t head_stride, int64_t n_seqs,
+                                   int64_t kv_heads, int64_t head_dim, int64_t max_seq, void* stream);
+/* The values of slots slot .. slot + n - 1, laid out as aeth_kv8_append takes them. */
+AETH_API int aeth_kv8_read(const void* d_layer, float* d_k, float* d_v, int64_t token_stride, int64_t head_stride,
+                           int64_t n, int64_t kv_heads, int64_t head_dim, int64_t max_seq, int64_t slot, void* stream);
+/* Bytes of workspace that an attention call of at most n_seqs sequences, n queries
+ * each and max_len positions needs (0: none; -1: a bad shape); 16-byte aligned,
+ * its content of no account. The library keeps none of its own for these
+ * calls: two that may run at once (two streams, two captured graphs) take two. */
+AETH_API int64_t aeth_attn_kv8_ws_bytes(int64_t n_seqs, int64_t n, int64_t n_heads, int64_t kv_heads, int64_t head_dim,
+                                        int64_t max_len);
+/* GQA attention of the last n of seq tokens over an 8-bit layer slice: query i
+ * (row i of d_q, head h at column h·head_dim, rotated) stands at position
+ * seq - n + i and sees the slots max(0, p - window + 1) .. p (window 0: 0 .. p):
+ * n = 1 is aeth_attn_decode, n = seq aeth_attn_prefill, and what lies between a
+ * chunk of a prompt or a drafted continuation. d_out is [n][n_heads·head_dim],
+ * not overlapping d_q. q enters a score rounded to 2^-23 of its row's largest
+ * component, a probability rounded to 2^-23 of the largest product of
+ * probability and V scale in 64 tokens; sums in 32 bits or more. A visible
+ * token with an infinity or NaN makes the row NaN, a masked one has no effect. */
+AETH_API int aeth_attn_kv8(const float* d_q, int64_t q_stride, const void* d_layer, int64_t n, int64_t n_heads,
+                           int64_t kv_heads, int64_t head_dim, int64_t max_seq, int64_t seq, int64_t window,
+                           float* d_out, void* d_ws, int64_t ws_bytes, void* stream);
+/* The same for one query of each of n_seqs sequences (row i of d_q the last token
+ * of sequence i), of d_lens[i] tokens each (device, read on the stream: a
+ * captured call follows them), clamped to [0, max_len]; length 0 gives a row of
+ * zeros. max_len <= max_seq also sets how the work is split. */
+AETH_API int aeth_attn_kv8_batch(const float* d_q, int64_t q_stride, const void* d_layers, int64_t layer_stride,
+                                 const int32_t* d_lens, int64_t n_seqs, int64_t n_heads, int64_t kv_heads,
+                                 int64_t head_dim, int64_t max_seq, int64_t max_len, int64_t window, float* d_out,
+                                 void* d_ws, int64_t ws_bytes, void* stream);
 /* SiLU-MLP glue (runner.rs:1617-1625): g = g * sigmoid(g) * up. */
 AETH_API int aeth_silu_mul(float* d_gate, const float* d_up, int64_t n, void* stream);
 /* Residual add (runner.rs:1609-1611): x += y. */

@@ -1,0 +1,119 @@
+"""The 8-bit key/value cache and its attention from their definitions, in 64 bits
+(torch on whatever device the tensors are), and the error bounds that the
+kernels' roundings allow."""
+import math
+
+import torch
+
+TILE = 64
+# an f32 value rounded to an integer of 24 bits in balanced digits: the largest component is over 0x7F7F00 / 2
+# units, so half a unit is at most this share of it
+STEP = 0.5 / 4177792
+U = 2.0 ** -24  # half a step of f32, relative
+
+
+def layer_shape(nkv, hd, max_seq):
+    return nkv, -(-max_seq // TILE), 2 * TILE * hd + 8 * TILE
+
+
+def vbyte(t):
+    return 16 * ((t // 4) % 4) + 4 * (t // 16) + t % 4
+
+
+def codes(x):
+    """[..., hd] f32 → int codes (64 bits: exact quotients, ties to even) and f32 scales."""
+    amax = x.abs().amax(-1)
+    fine = torch.isfinite(amax)
+    a = torch.where(fine & (amax > 0), amax, torch.ones_like(amax)).double()
+    c = torch.round(x.double() * 127.0 / a[..., None])
+    c = torch.where((fine & (amax > 0))[..., None], c, torch.zeros_like(c)).to(torch.int8)
+    s = torch.where(fine, (amax.double() / 127.0).float(), torch.full_like(amax, math.nan))
+    return c, s
+
+
+def unpack(layer, nkv, hd, max_seq):
+    """The bytes of a layer slice → codes [nkv][slots][hd] of K and V (int8), scales [nkv][slots]."""
+    h, tiles, _ = layer_shape(nkv, hd, max_seq)
+    b = layer.reshape(h, tiles, -1)
+    k = b[..., :TILE * hd].reshape(h, tiles * TILE, hd).view(torch.int8)
+    v = b[..., TILE * hd:2 * TILE * hd].reshape(h, tiles, hd, TILE).view(torch.int8)
+    at = torch.tensor([vbyte(t) for t in range(TILE)], device=layer.device)
+    v = v[..., at].transpose(-1, -2).reshape(h, tiles * TILE, hd)
+    s = b[..., 2 * TILE * hd:].contiguous().view(torch.float32)
+    return k, v, s[..., :TILE].reshape(h, -1), s[..., TILE:].reshape(h, -1)
+
+
+def pack(kc, ks, vc, vs):
+    """Codes [nkv][slots][hd] (slots a multiple of 64) and scales → the bytes of a layer slice."""
+    h, slots, hd = kc.shape
+    tiles = slots // TILE
+    out = torch.empty((h, tiles, 2 * TILE * hd + 8 * TILE), dtype=torch.uint8, device=kc.device)
+    out[..., :TILE * hd] = kc.reshape(h, tiles, -1).contiguous().view(torch.uint8)
+    inv = torch.empty(TILE, dtype=torch.long, device=kc.device)
+    for t in range(TILE):
+        inv[vbyte(t)] = t
+    v = vc.reshape(h, tiles, TILE, hd)[:, :, inv].transpose(-1, -2).contiguous()
+    out[..., TILE * hd:2 * TILE * hd] = v.reshape(h, tiles, -1).view(torch.uint8)
+    s = torch.cat([ks.reshape(h, tiles, TILE), vs.reshape(h, tiles, TILE)], -1).contiguous()
+    out[..., 2 * TILE * hd:] = s.view(torch.uint8)
+    return out
+
+
+def attention(q, layer, nkv, hd, max_seq, length, window):
+    """q [n][heads·hd] f32 of the last n of `length` tokens → (result, bound), both [n][heads·hd] f64. The
+    bound is what the roundings of include/aether_hip.h allow, element by element:
+      q:  half a unit of 24 bits of the row's largest component, times Σ|k| of the key;
+      score: 8 f32 roundings of it; exponential: 4, and that of its argument, 2·|s - max|·U;
+      p·sv: half a unit of 24 bits of the tile's largest, times Σ|code| over the tile;
+      sums: one f32 rounding a tile, 16 for what joins waves and chunks, for sum and output each."""
+    n, heads = q.shape[0], q.shape[1] // hd
+    g = heads // nkv
+    kc, vc, ks, vs = unpack(layer, nkv, hd, max_seq)
+    out = torch.zeros((n, heads * hd), dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    if length == 0:
+        return out, tol
+    pos = torch.arange(length - n, length, device=q.device)[:, None]
+    t = torch.arange(length, device=q.device)[None, :]
+    seen = (t <= pos) & ((t > pos - window) if window else (t >= 0))
+    tiles = -(-length // TILE)
+    pad = tiles * TILE - length
+    for h in range(nkv):
+        kd = kc[h, :length].double() * ks[h, :length, None].double()
+        vd = vc[h, :length].double() * vs[h, :length, None].double()
+        some = seen.any(0)
+        kd, vd = torch.where(some[:, None], kd, 0.0), torch.where(some[:, None], vd, 0.0)
+        for j in range(h * g, (h + 1) * g):
+            qd = q[:, j * hd:(j + 1) * hd].double()
+            s = (qd @ kd.t().contiguous()) / math.sqrt(hd)
+            s = torch.where(seen, s, -math.inf)
+            m = s.amax(1, keepdim=True)
+            p = torch.exp(s - m)
+            l = p.sum(1, keepdim=True)
+            cols = slice(j * hd, (j + 1) * hd)
+            pv = torch.where(p == 0, 0.0, p)
+            out[:, cols] = (pv @ vd) / l
+            mass = (pv @ vd.abs()) / l
+            es = qd.abs().amax(1, keepdim=True) * STEP * kd.abs().sum(1)[None] / math.sqrt(hd) + 8 * U * s.abs() + 4 * U + 2 * U * (s - m).abs()
+            es = torch.where(seen, es, 0.0).amax(1, keepdim=True)
+            w = torch.nn.functional.pad(p * torch.where(some, vs[h, :length].double(), 0.0)[None], (0, pad)).reshape(n, tiles, TILE).amax(2)
+            c = torch.nn.functional.pad(torch.where(some[:, None], vc[h, :length].double().abs(), 0.0), (0, 0, 0, pad)).reshape(tiles, TILE, hd).sum(1)
+            tol[:, cols] = 2 * es * mass + STEP * (w @ c) / l + 2 * (tiles + 16) * U * mass
+    return out, tol + 1e-37
+
+
+def qk_norm_rope(x, nq, nk, hd, qw, kw, eps, positions, sin, cos):
+    """[n][>= (nq + nk)·hd] f32 → (result, bound) [n][(nq + nk)·hd] f64: eight f32 roundings of each factor
+    (the sum of squares: hd / 8 in a lane and six joins, halved by the root), three of the rotation."""
+    n = x.shape[0]
+    y = x[:, :(nq + nk) * hd].double().reshape(n, nq + nk, hd)
+    for part, w in ((slice(0, nq), qw), (slice(nq, nq + nk), kw)):
+        if w is not None:
+            z = y[:, part]
+            y[:, part] = z / torch.sqrt((z * z).mean(-1, keepdim=True) + eps) * w.double()
+    p = positions.clamp(0, sin.shape[0] - 1).long()
+    s, c = sin[p].double()[:, None], cos[p].double()[:, None]
+    a, b = y[..., :hd // 2], y[..., hd // 2:]
+    out = torch.cat([a * c - b * s, a * s + b * c], -1)
+    mag = torch.cat([(a * c).abs() + (b * s).abs()] * 2, -1).maximum(torch.cat([(a * s).abs() + (b * c).abs()] * 2, -1))
+    return out.reshape(n, -1), ((hd / 16 + 14) * U * mag).reshape(n, -1) + 1e-37
