@@ -113,31 +113,27 @@ __global__ void __launch_bounds__(256) k_attn8(A8 A) {
 
     a8_i4 kf[4][KS], vf[DT];
     a8_f4 sk[4], sv[4];
+    // codes read once go past the caches (131000 tokens: 47.6 µs against 51.4)
+    auto ld = [](const uint8_t* p) { return NC == 1 && HD <= 128 ? __builtin_nontemporal_load((const a8_i4*)p) : *(const a8_i4*)p; };
     auto load = [&](int t) {
         const uint8_t* p = head + (int64_t)t * aeth_kv8_tile_bytes(HD);
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int s = 0; s < KS; s++) kf[j][s] = *(const a8_i4*)(p + (16 * j + c) * HD + 64 * s + 16 * g);
+            for (int s = 0; s < KS; s++) kf[j][s] = ld(p + (16 * j + c) * HD + 64 * s + 16 * g);
 #pragma unroll
         for (int j = 0; j < 4; j++) sk[j] = *(const a8_f4*)(p + 2 * KV8_TILE * HD + 4 * (16 * j + 4 * g));
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) vf[dt] = *(const a8_i4*)(p + KV8_TILE * HD + (16 * dt + c) * KV8_TILE + 16 * g);
+        for (int dt = 0; dt < DT; dt++) vf[dt] = ld(p + KV8_TILE * HD + (16 * dt + c) * KV8_TILE + 16 * g);
 #pragma unroll
         for (int j = 0; j < 4; j++) sv[j] = *(const a8_f4*)(p + 2 * KV8_TILE * HD + 4 * (KV8_TILE + 16 * j + 4 * g));
     };
-    if (t0 + w < t1) load(t0 + w);
-
-    // the columns: q's digits, the keys [lo, hi) they see
-    uint32_t qd[NC][3][KS][4];
-    float qs[NC], m[NC], l[NC];
-    int lo[NC], hi[NC];
-    a8_f4 o[NC][DT];
+    // the columns: q (its loads go out first), the keys [lo, hi) they see
+    float qv[NC][KS][16];
 #pragma unroll
     for (int u = 0; u < NC; u++) {
-        const int x = cb * 16 * NC + 16 * u + c, xc = min(x, A.cols - 1), i = xc / A.G;
+        const int xc = min(cb * 16 * NC + 16 * u + c, A.cols - 1), i = xc / A.G;
         const float* src = A.q + ((int64_t)seq * A.n + i) * A.q_stride + (int64_t)(h * A.G + xc % A.G) * HD + 16 * g;
-        float qv[KS][16], mx = 0.0f;
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -145,17 +141,29 @@ __global__ void __launch_bounds__(256) k_attn8(A8 A) {
                 float4 y;
                 if (A.qvec) y = *(const float4*)(src + 64 * s + e);
                 else y = make_float4(src[64 * s + e], src[64 * s + e + 1], src[64 * s + e + 2], src[64 * s + e + 3]);
-                qv[s][e] = y.x;
-                qv[s][e + 1] = y.y;
-                qv[s][e + 2] = y.z;
-                qv[s][e + 3] = y.w;
+                qv[u][s][e] = y.x;
+                qv[u][s][e + 1] = y.y;
+                qv[u][s][e + 2] = y.z;
+                qv[u][s][e + 3] = y.w;
             }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (t0 + w < t1) load(t0 + w);
+    __builtin_amdgcn_sched_barrier(0);
+    uint32_t qd[NC][3][KS][4];
+    float qs[NC], m[NC], l[NC];
+    int lo[NC], hi[NC];
+    a8_f4 o[NC][DT];
+#pragma unroll
+    for (int u = 0; u < NC; u++) {
+        const int x = cb * 16 * NC + 16 * u + c, xc = min(x, A.cols - 1), i = xc / A.G;
+        float mx;
         uint32_t mb = 0;
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                mb = max(mb, __float_as_uint(qv[s][e]) & 0x7FFFFFFFu);
+                mb = max(mb, __float_as_uint(qv[u][s][e]) & 0x7FFFFFFFu);
             }
         {   // over the four lane groups, as integers: a NaN's bits are above an infinity's
             const auto a = __builtin_amdgcn_permlane16_swap(mb, mb, false, false);
@@ -170,8 +178,8 @@ __global__ void __launch_bounds__(256) k_attn8(A8 A) {
         for (int s = 0; s < KS; s++)
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-                a8_digits((uint32_t)(int)rintf(qv[s][e] * f), (uint32_t)(int)rintf(qv[s][e + 1] * f),
-                          (uint32_t)(int)rintf(qv[s][e + 2] * f), (uint32_t)(int)rintf(qv[s][e + 3] * f), qd[u][0][s][e / 4],
+                a8_digits((uint32_t)(int)rintf(qv[u][s][e] * f), (uint32_t)(int)rintf(qv[u][s][e + 1] * f),
+                          (uint32_t)(int)rintf(qv[u][s][e + 2] * f), (uint32_t)(int)rintf(qv[u][s][e + 3] * f), qd[u][0][s][e / 4],
                           qd[u][1][s][e / 4], qd[u][2][s][e / 4]);
         // an infinity or NaN in q: every score NaN
         qs[u] = mb >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : a8_pow2(-e2) * (1.4426950408889634f / sqrtf((float)HD));
@@ -325,38 +333,366 @@ __global__ void __launch_bounds__(256) k_attn8(A8 A) {
     }
 }
 
-// Joins the chunks of one column: a workgroup of hd threads, thread = output dimension
-template <int HD, int NC>
-__global__ void __launch_bounds__(HD) k_attn8_merge(A8 A) {
-    const int d = threadIdx.x, h = blockIdx.x % A.nkv, x = blockIdx.x / A.nkv, seq = blockIdx.y;
-    const int cb = x / (16 * NC), cc = x % (16 * NC);
-    const int len = a8_len(A, seq);
-    int beg, end;
-    a8_tiles(A, len, cb * 16 * NC, 16 * NC, beg, end);
-    const int live = max(1, (end - beg + A.tpc - 1) / A.tpc);
-    const float* part = A.ws + (int64_t)((seq * A.nkv + h) * A.ncb + cb) * A.chunks * (16 * NC) * (HD + 2);
-    float M = -INFINITY;
-    for (int k = 0; k < live; k++) M = fmaxf(M, part[(int64_t)k * (16 * NC) * (HD + 2) + 16 * NC * HD + 2 * cc]);
-    float L = 0.0f, acc = 0.0f;
-    for (int k = 0; k < live; k++) {
-        const float* p = part + (int64_t)k * (16 * NC) * (HD + 2);
-        const float m = p[16 * NC * HD + 2 * cc], wt = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-        L += wt * p[16 * NC * HD + 2 * cc + 1];
-        acc += wt * p[cc * HD + d];
-    }
-    A.out[((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + d] = L == 0.0f ? 0.0f : acc * (1.0f / L);
+// ── many columns: a prompt, or a chunk of one ─────────────────────────────
+// The int8 form above spends more on joining digits than on the softmax itself: eight instructions a score
+// and ten a probability and output share. Here the codes become fp16 (exactly), once for a workgroup's
+// 32·NW columns, on their way to LDS, and q and the probabilities are each two fp16 parts, x = hi + lo
+// (22 significant bits), so that both products run on v_mfma_f32_32x32x16_f16 in two passes that share
+// their f32 accumulators: nothing is left to join.
+//  * q: x·2^-e below 2^15, lo's last place 2^-24: to 2^-23 of each component (the small ones to 2^-40 of the row's
+//    largest).
+//  * p·sv enters times a power of two of its column, which follows the largest such product the column has seen
+//    (in [2^9, 2^15)): to 2^-23 of itself, or 2^-34 of that largest one where it is far smaller.
+// Wave = 32 columns; Sᵀ = K·Qᵀ leaves a lane (column l%32, half h = l/32) the keys 8a + 4h + r of 32, which is
+// the order in which V's operand takes its tokens (j = 2T + u, g = 2a + h of aeth_kv8.hpp), so the
+// probabilities stay in their lanes. The next tile's codes are loaded a tile ahead, converted and stored in
+// the other LDS buffer before this tile's products: one barrier a tile.
+typedef _Float16 a8_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 a8_h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 a8_h2 __attribute__((ext_vector_type(2)));
+typedef float a8_f16 __attribute__((ext_vector_type(16)));
+
+// four signed bytes as fp16
+__device__ __forceinline__ a8_h4 a8_half4(uint32_t w) {
+    w ^= 0x80808080u;
+    const a8_h2 k = {(_Float16)-1152.0f, (_Float16)-1152.0f};  // (0x64 | b) is 1024 + b
+    const a8_h2 a = __builtin_bit_cast(a8_h2, __builtin_amdgcn_perm(0x64646464u, w, 0x07010700u)) + k;
+    const a8_h2 b = __builtin_bit_cast(a8_h2, __builtin_amdgcn_perm(0x64646464u, w, 0x07030702u)) + k;
+    return (a8_h4){a[0], a[1], b[0], b[1]};
 }
 
-// Chunks a row block's tiles are split into so that `units` of them fill the chip: two workgroups a CU
-int64_t a8_target() { return 2 * (int64_t)aeth_num_cus(); }
+template <int HD, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
+    constexpr int KS = HD / 16, DT = HD / 32, NT = 64 * NW, CH = 4 * HD / NT;
+    static_assert(CH >= 1 && CH * NT == 4 * HD, "16-byte pieces of a plane a thread");
+    constexpr int KF = 1040;  // bytes from one K fragment to the next: eight threads of a row store to eight bank groups
+    constexpr float TH = 8.0f;
+    __shared__ __attribute__((aligned(16))) char kb[2][2 * KS * KF];
+    __shared__ __attribute__((aligned(16))) char vb[2][DT * 4 * 1024];
+    __shared__ __attribute__((aligned(16))) float sc[2][2 * KV8_TILE];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hf = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int id = blockIdx.x;
+    const int h = id % A.nkv;
+    id /= A.nkv;
+    const int cb = A.ncb - 1 - id % A.ncb, chunk = id / A.ncb, seq = blockIdx.y;
+    const int len = a8_len(A, seq);
+    int beg, end;
+    a8_tiles(A, len, cb * 32 * NW, 32 * NW, beg, end);
+    const int t0 = beg + chunk * A.tpc, t1 = min(t0 + A.tpc, end);
+    if (t0 >= t1 && chunk > 0) return;  // (uniform) the merge leaves it out
+    const uint8_t* head = A.cache + seq * A.seq_bytes + (int64_t)h * A.tiles * aeth_kv8_tile_bytes(HD);
 
-template <int HD, int NC>
-int launch(A8 A, int64_t seqs, hipStream_t s) {
+    uint4 rk[CH], rv[CH];
+    float rsk = 0.0f, rsv = 0.0f;
+    auto fetch_k = [&](int t) {
+        const uint8_t* p = head + (int64_t)t * aeth_kv8_tile_bytes(HD);
+#pragma unroll
+        for (int u = 0; u < CH; u++) rk[u] = *(const uint4*)(p + 16 * (tid + NT * u));
+        if (tid < KV8_TILE) {
+            rsk = *(const float*)(p + 2 * KV8_TILE * HD + 4 * tid);
+            rsv = *(const float*)(p + 2 * KV8_TILE * HD + 4 * (KV8_TILE + tid));
+        }
+    };
+    auto fetch_v = [&](int t) {
+        const uint8_t* p = head + (int64_t)t * aeth_kv8_tile_bytes(HD) + KV8_TILE * HD;
+#pragma unroll
+        for (int u = 0; u < CH; u++) rv[u] = *(const uint4*)(p + 16 * (tid + NT * u));
+    };
+    auto stage_k = [&](int b) {  // token t, dimensions 16·ks .. + 15 → lanes t%32 and 32 + t%32 of fragment (t/32, ks)
+#pragma unroll
+        for (int u = 0; u < CH; u++) {
+            const int at = tid + NT * u, t = at / KS, ks = at % KS;
+            char* dst = kb[b] + ((t >> 5) * KS + ks) * KF + (t & 31) * 16;
+            const a8_h4 x = a8_half4(rk[u].x), y = a8_half4(rk[u].y), z = a8_half4(rk[u].z), q = a8_half4(rk[u].w);
+            *(a8_h8*)dst = (a8_h8){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            *(a8_h8*)(dst + 512) = (a8_h8){z[0], z[1], z[2], z[3], q[0], q[1], q[2], q[3]};
+        }
+        // a V scale that is no number goes to the token's K scale: its scores are NaN where it is seen
+        if (tid < KV8_TILE) {
+            const bool fine = fabsf(rsv) < INFINITY;
+            sc[b][tid] = fine ? rsk : __uint_as_float(0x7FC00000u);
+            sc[b][KV8_TILE + tid] = fine ? rsv : 0.0f;
+        }
+    };
+    auto stage_v = [&](int b) {  // dimension d, token group g = 2a + half → half of a lane's eight tokens of fragments (d/32, j)
+#pragma unroll
+        for (int u = 0; u < CH; u++) {
+            const int at = tid + NT * u, d = at >> 2, g = at & 3;
+            char* dst = vb[b] + (d >> 5) * 4096 + ((d & 31) + 32 * (g & 1)) * 16 + 8 * (g >> 1);
+            *(a8_h4*)dst = a8_half4(rv[u].x);
+            *(a8_h4*)(dst + 1024) = a8_half4(rv[u].y);
+            *(a8_h4*)(dst + 2048) = a8_half4(rv[u].z);
+            *(a8_h4*)(dst + 3072) = a8_half4(rv[u].w);
+        }
+    };
+    if (t0 < t1) {
+        fetch_k(t0);
+        fetch_v(t0);
+    }
+
+    const int x0 = cb * 32 * NW + 32 * w, x = x0 + c, xc = min(x, A.cols - 1), qi = xc / A.G;
+    const int hi = len - A.n + qi + 1, lo = A.window > 0 ? hi - A.window : 0;
+    // of the wave: every column sees [all_lo, all_hi), none outside [any_lo, any_hi)
+    const int i0 = min(x0, A.cols - 1) / A.G, i1 = min(x0 + 31, A.cols - 1) / A.G;
+    const int all_hi = len - A.n + i0 + 1, any_hi = len - A.n + i1 + 1;
+    const int all_lo = A.window > 0 ? any_hi - A.window : 0, any_lo = A.window > 0 ? all_hi - A.window : 0;
+    a8_h8 qh[KS], ql[KS];
+    float qs;
+    {
+        const float* src = A.q + ((int64_t)seq * A.n + qi) * A.q_stride + (int64_t)(h * A.G + xc % A.G) * HD + 8 * hf;
+        float y[KS][8];
+        uint32_t mb = 0;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            if (A.qvec) {
+                const float4 a = *(const float4*)(src + 16 * ks), b = *(const float4*)(src + 16 * ks + 4);
+                y[ks][0] = a.x; y[ks][1] = a.y; y[ks][2] = a.z; y[ks][3] = a.w;
+                y[ks][4] = b.x; y[ks][5] = b.y; y[ks][6] = b.z; y[ks][7] = b.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[ks][e] = src[16 * ks + e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) mb = max(mb, __float_as_uint(y[ks][e]) & 0x7FFFFFFFu);
+        }
+        const auto a = __builtin_amdgcn_permlane32_swap(mb, mb, false, false);
+        mb = max(a[0], a[1]);
+        const int e2 = a8_exponent(__uint_as_float(mb)) - 8;  // the largest below 2^15
+        const float f = a8_pow2(e2);
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = y[ks][e] * f;
+                qh[ks][e] = (_Float16)v;
+                ql[ks][e] = (_Float16)(v - (float)qh[ks][e]);
+            }
+        // an infinity or NaN in q: every score NaN
+        qs = mb >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : a8_pow2(-e2) * (1.4426950408889634f / sqrtf((float)HD));
+    }
+    float m = -INFINITY, l = 0.0f, top = 0.0f, fw = 1.0f;  // the largest p·sv so far; its power of two
+    a8_f16 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) o[dt] = (a8_f16){};
+
+    if (t0 < t1) {
+        stage_k(0);
+        stage_v(0);
+        if (t0 + 1 < t1) {
+            fetch_k(t0 + 1);
+            fetch_v(t0 + 1);
+        }
+    }
+    a8_f16 s;
+    a8_h8 ph[2], pl[2];
+    auto scores = [&](int b, int T) {
+        s = (a8_f16){};
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const a8_h8 kf = *(const a8_h8*)(kb[b] + (T * KS + ks) * KF + lane * 16);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[ks], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[ks], s, 0, 0, 0);
+        }
+    };
+    auto values = [&](int b, int T) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                const a8_h8 vf = *(const a8_h8*)(vb[b] + (dt * 4 + 2 * T + u) * 1024 + lane * 16);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[u], o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[u], o[dt], 0, 0, 0);
+            }
+    };
+    auto softmax = [&](int t, int b, int T) {
+        const int k0 = 64 * t + 32 * T;
+        a8_f4 sk[4], sv[4];
+#pragma unroll
+        for (int a = 0; a < 4; a++) {
+            sk[a] = *(const a8_f4*)&sc[b][32 * T + 8 * a + 4 * hf];
+            sv[a] = *(const a8_f4*)&sc[b][KV8_TILE + 32 * T + 8 * a + 4 * hf];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] *= sk[i >> 2][i & 3];
+        if (k0 < all_lo || k0 + 32 > all_hi) {  // (uniform) some key is masked
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int key = k0 + 8 * (i >> 2) + 4 * hf + (i & 3);
+                s[i] = key >= lo && key < hi ? s[i] : -INFINITY;
+            }
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
+        {
+            const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])) * qs;
+        }
+        if (__any(mx > m + TH)) {  // (uniform)
+            const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= al;
+            top *= al;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) o[dt] *= al;
+            m = mn;
+        }
+        const float mo = m == -INFINITY ? 0.0f : m;
+        float wm = 0.0f, ps = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[i], qs, -mo));
+            ps += p;
+            s[i] = p * sv[i >> 2][i & 3];
+            wm = fmaxf(wm, s[i]);
+        }
+        l += ps;
+        {
+            const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(wm), __float_as_uint(wm), false, false);
+            wm = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+        }
+        top = fmaxf(top, wm);
+        if (__any(top > 0.0f && !(top * fw >= 512.0f && top * fw < 32768.0f))) {  // (uniform) out of its power of two's range
+            if (!(top < INFINITY)) l = __uint_as_float(0x7FC00000u);  // values past 2^119: no number rather than a wrong one
+            const float fn = top > 0.0f ? a8_pow2(a8_exponent(top) - 12) : fw;  // top·fn in [2^10, 2^11)
+            const float fi = 1.0f / fw;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) o[dt] = o[dt] * fi * fn;
+            fw = fn;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float v = s[i] * fw;
+            asm("" : "+v"(v));  // (one product for both parts)
+            const _Float16 y = (_Float16)v;
+            ph[i >> 3][i & 7] = y;
+            pl[i >> 3][i & 7] = (_Float16)(v - (float)y);
+        }
+    };
+    __syncthreads();
+    for (int t = t0; t < t1; t++) {
+        const int b = (t - t0) & 1;
+        if (t + 1 < t1) {
+            stage_k(b ^ 1);
+            stage_v(b ^ 1);
+            if (t + 2 < t1) {
+                fetch_k(t + 2);
+                fetch_v(t + 2);
+            }
+        }
+#pragma unroll
+        for (int T = 0; T < 2; T++) {
+            const int k0 = 64 * t + 32 * T;
+            if (k0 >= any_hi || k0 + 32 <= any_lo) continue;  // (uniform in the wave) no column sees any
+            scores(b, T);
+            softmax(t, b, T);
+            values(b, T);
+        }
+        __syncthreads();
+    }
+    {
+        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    }
+    if (x >= A.cols) return;
+    const float fi = 1.0f / fw;  // exact: a power of two
+    if (A.chunks > 1) {
+        const int cc = 32 * w + c;
+        float* part = A.ws + ((int64_t)((seq * A.nkv + h) * A.ncb + cb) * A.chunks + chunk) * (32 * NW) * (HD + 2);
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int a = 0; a < 4; a++)
+                *(a8_f4*)(part + cc * HD + 32 * dt + 8 * a + 4 * hf) =
+                    (a8_f4){o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]} * fi;
+        if (hf == 0) {
+            part[32 * NW * HD + 2 * cc] = m;
+            part[32 * NW * HD + 2 * cc + 1] = l;
+        }
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : fi / l;
+    float* dst = A.out + ((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + 4 * hf;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int a = 0; a < 4; a++) {
+            const a8_f4 y = (a8_f4){o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]} * inv;
+            float* d = dst + 32 * dt + 8 * a;
+            if (A.ovec) *(a8_f4*)d = y;
+            else d[0] = y[0], d[1] = y[1], d[2] = y[2], d[3] = y[3];
+        }
+}
+
+// Joins the chunks of one column (of blocks of cw): 256 threads, four dimensions each of every 1024/hd-th chunk, so
+// that the partials of a long cache are read at once rather than one after the other
+template <int HD>
+__global__ void __launch_bounds__(256) k_attn8_merge(A8 A, int cw) {
+    constexpr int NG = 1024 / HD;  // chunk groups
+    __shared__ __attribute__((aligned(16))) float sum[NG][HD];
+    const int tid = threadIdx.x, lane = tid & 63, d = 4 * (tid % (HD / 4)), grp = tid / (HD / 4);
+    const int h = blockIdx.x % A.nkv, x = blockIdx.x / A.nkv, seq = blockIdx.y;
+    const int cb = x / cw, cc = x % cw;
+    int beg, end;
+    a8_tiles(A, a8_len(A, seq), cb * cw, cw, beg, end);
+    const int live = max(1, (end - beg + A.tpc - 1) / A.tpc);
+    const int64_t step = (int64_t)cw * (HD + 2);
+    const float* part = A.ws + (int64_t)((seq * A.nkv + h) * A.ncb + cb) * A.chunks * step;
+    const float* st = part + cw * HD + 2 * cc;
+    const float* val = part + cc * HD + d;
+    float M = -INFINITY, L = 0.0f;
+    for (int k = lane; k < live; k += 64) M = fmaxf(M, st[k * step]);
+    M = aeth_wave_max(M);
+    for (int k = lane; k < live; k += 64) {
+        const float2 ml = *(const float2*)(st + k * step);
+        L += (ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M)) * ml.y;
+    }
+    L = aeth_wave_sum(L);
+    a8_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int k = grp; k < live; k += NG) {
+        const float m = st[k * step];
+        acc += *(const a8_f4*)(val + k * step) * (m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M));
+    }
+    *(a8_f4*)&sum[grp][d] = acc;
+    __syncthreads();
+    if (tid >= HD) return;
+    float y = 0.0f;
+#pragma unroll
+    for (int g = 0; g < NG; g++) y += sum[g][tid];
+    A.out[((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + tid] = L == 0.0f ? 0.0f : y * (1.0f / L);
+}
+
+// The form a call takes: the columns of a workgroup, and the workgroups its tiles are split into where there are
+// fewer. Lengths that only the device knows (ragged) get twice as many: the longest sequence's no longer decide
+// (48 sequences of 1 .. 4096 tokens: 51.3 µs against 58.0).
+struct Form {
+    int cw;
+    int64_t target;
+    int tiles_min;  // tiles a chunk has at least
+};
+Form a8_form(int64_t seqs, int64_t cols, int64_t nkv, int64_t hd, bool ragged) {
+    const int64_t cus = aeth_num_cus(), small = (ragged ? 4 : 2) * cus;
+    if (hd > 128 || cols <= 16) return {16, small, 4};
+    if (cols <= 64) return {32, small, 4};
+    if (hd == 128 && seqs * nkv * aeth_cdiv(cols, 256) >= cus) return {256, cus, 8};
+    return {128, 2 * cus, 8};
+}
+
+template <int HD>
+int a8_launch(const A8& A, const Form& f, int64_t seqs, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)A.nkv * A.ncb * A.chunks), (unsigned)seqs);
-    hipLaunchKernelGGL((k_attn8<HD, NC>), grid, dim3(256), 0, s, A);
+    if constexpr (HD == 256) {
+        hipLaunchKernelGGL((k_attn8<HD, 1>), grid, dim3(256), 0, s, A);
+    } else {
+        if (f.cw == 16) hipLaunchKernelGGL((k_attn8<HD, 1>), grid, dim3(256), 0, s, A);
+        else if (f.cw == 32) hipLaunchKernelGGL((k_attn8<HD, 2>), grid, dim3(256), 0, s, A);
+        else if (f.cw == 128) hipLaunchKernelGGL((k_attn8p<HD, 4>), grid, dim3(256), 0, s, A);
+        else if constexpr (HD == 128) hipLaunchKernelGGL((k_attn8p<HD, 8>), grid, dim3(512), 0, s, A);
+    }
     AETH_LAUNCH_CHECK();
     if (A.chunks > 1) {
-        hipLaunchKernelGGL((k_attn8_merge<HD, NC>), dim3((unsigned)((int64_t)A.nkv * A.cols), (unsigned)seqs), dim3(HD), 0, s, A);
+        hipLaunchKernelGGL(k_attn8_merge<HD>, dim3((unsigned)((int64_t)A.nkv * A.cols), (unsigned)seqs), dim3(256), 0, s, A, f.cw);
         AETH_LAUNCH_CHECK();
     }
     return AETH_OK;
@@ -366,10 +702,16 @@ int launch(A8 A, int64_t seqs, hipStream_t s) {
 
 int64_t aeth_attn_kv8_ws(int64_t seqs, int64_t n, int64_t nq, int64_t nkv, int64_t hd, int64_t len) {
     if (len <= 4 * KV8_TILE) return 0;  // never split
-    // `units` row blocks in fewer than target chunks each, or none split: at most target + units partials, and a
-    // smaller call at most twice the target
-    const int64_t units = seqs * nkv * aeth_cdiv(n * (nq / nkv), 16), target = a8_target();
-    return (target + (units < target ? units : target)) * 32 * (hd + 2) * (int64_t)sizeof(float);
+    // `units` column blocks are split into at most target / units + 1 chunks each, or not at all: fewer than
+    // 2·target partials, and target + units. A smaller call (fewer sequences or queries) may take another form.
+    const int64_t cols = n * (nq / nkv), cus = aeth_num_cus();
+    auto need = [&](int64_t cw, int64_t target) {
+        const int64_t units = seqs * nkv * aeth_cdiv(cols, cw);
+        return (target + std::min(units, target)) * cw;
+    };
+    int64_t most = hd > 128 || cols <= 16 ? need(16, 4 * cus) : need(32, 4 * cus);
+    if (hd <= 128 && cols > 64) most = std::max(most, need(128, 2 * cus));
+    return most * (hd + 2) * (int64_t)sizeof(float);
 }
 
 int aeth_attn_kv8_launch(const float* q, int64_t q_stride, const void* cache, int64_t seq_bytes, const int* lens, int len_add,
@@ -395,20 +737,20 @@ int aeth_attn_kv8_launch(const float* q, int64_t q_stride, const void* cache, in
     A.ws = (float*)ws;
     A.qvec = ((uintptr_t)q & 15) == 0 && (q_stride & 3) == 0;
     A.ovec = ((uintptr_t)out & 15) == 0;
-    const int nc = A.cols > 16 && hd <= 128 ? 2 : 1;  // (two column sets of 256 dimensions do not fit the registers)
-    A.ncb = (int)aeth_cdiv(A.cols, 16 * nc);
+    const Form f = a8_form(seqs, A.cols, nkv, hd, lens != nullptr);
+    A.ncb = (int)aeth_cdiv(A.cols, f.cw);
     // the most tiles a column block sees, and the chunks that fill the chip
-    const int64_t rows = aeth_cdiv(16 * nc, A.G) + 1;
+    const int64_t rows = aeth_cdiv(f.cw, A.G) + 1;
     const int64_t span = A.window ? std::min(aeth_cdiv(max_len, KV8_TILE), (A.window + std::min(rows, n) + 62) / KV8_TILE + 1)
                                   : aeth_cdiv(max_len, KV8_TILE);
     const int64_t units = seqs * nkv * A.ncb;
-    const int64_t want = std::max<int64_t>(1, std::min(aeth_cdiv(a8_target(), units), aeth_cdiv(span, 4)));
+    const int64_t want = std::max<int64_t>(1, std::min(aeth_cdiv(f.target, units), aeth_cdiv(span, f.tiles_min)));
     A.tpc = (int)(aeth_cdiv(aeth_cdiv(span, want), 4) * 4);
     if (A.tpc < 4) A.tpc = 4;
     A.chunks = (int)std::max<int64_t>(1, aeth_cdiv(span, A.tpc));
-    if (hd == 64) return nc == 1 ? launch<64, 1>(A, seqs, s) : launch<64, 2>(A, seqs, s);
-    if (hd == 128) return nc == 1 ? launch<128, 1>(A, seqs, s) : launch<128, 2>(A, seqs, s);
-    return launch<256, 1>(A, seqs, s);
+    if (hd == 64) return a8_launch<64>(A, f, seqs, s);
+    if (hd == 128) return a8_launch<128>(A, f, seqs, s);
+    return a8_launch<256>(A, f, seqs, s);
 }
 
 // what the two entry points ask of their arguments in common

@@ -63,9 +63,12 @@ def attention(q, layer, nkv, hd, max_seq, length, window):
     """q [n][heads·hd] f32 of the last n of `length` tokens → (result, bound), both [n][heads·hd] f64. The
     bound is what the roundings of include/aether_hip.h allow, element by element:
       q:  half a unit of 24 bits of the row's largest component, times Σ|k| of the key;
-      score: 8 f32 roundings of it; exponential: 4, and that of its argument, 2·|s - max|·U;
-      p·sv: half a unit of 24 bits of the tile's largest, times Σ|code| over the tile;
-      sums: one f32 rounding a tile, 16 for what joins waves and chunks, for sum and output each."""
+      score: 8 f32 roundings of it, and as the sum of 16 products at a time in two parts (two roundings a
+        step: the products' sum, the running one) hd/4 of Σ|q·k|;
+      exponential: 4, and that of its argument, 2·|s - max|·U;
+      p·sv: half a unit of 24 bits of the tile's largest, times Σ|code| over the tile, or of itself and
+        2^-34 of the row's largest, times the code;
+      sums: as the scores', tokens/4 roundings, 16 for what joins waves and chunks, for sum and output each."""
     n, heads = q.shape[0], q.shape[1] // hd
     g = heads // nkv
     kc, vc, ks, vs = unpack(layer, nkv, hd, max_seq)
@@ -94,11 +97,13 @@ def attention(q, layer, nkv, hd, max_seq, length, window):
             pv = torch.where(p == 0, 0.0, p)
             out[:, cols] = (pv @ vd) / l
             mass = (pv @ vd.abs()) / l
-            es = qd.abs().amax(1, keepdim=True) * STEP * kd.abs().sum(1)[None] / math.sqrt(hd) + 8 * U * s.abs() + 4 * U + 2 * U * (s - m).abs()
+            es = (qd.abs().amax(1, keepdim=True) * STEP * kd.abs().sum(1)[None] + hd / 4 * U * (qd.abs() @ kd.abs().t().contiguous())) / math.sqrt(hd)
+            es = es + 8 * U * s.abs() + 4 * U + 2 * U * (s - m).abs()
             es = torch.where(seen, es, 0.0).amax(1, keepdim=True)
             w = torch.nn.functional.pad(p * torch.where(some, vs[h, :length].double(), 0.0)[None], (0, pad)).reshape(n, tiles, TILE).amax(2)
+            far = w.amax(1, keepdim=True) * 2.0 ** -34 * torch.where(some[:, None], vc[h, :length].double().abs(), 0.0).sum(0)
             c = torch.nn.functional.pad(torch.where(some[:, None], vc[h, :length].double().abs(), 0.0), (0, 0, 0, pad)).reshape(tiles, TILE, hd).sum(1)
-            tol[:, cols] = 2 * es * mass + STEP * (w @ c) / l + 2 * (tiles + 16) * U * mass
+            tol[:, cols] = 2 * es * mass + (STEP * (w @ c) + far) / l + U * mass + 2 * (length / 4 + 16) * U * mass
     return out, tol + 1e-37
 
 
