@@ -37,6 +37,7 @@ class LlamaConfig(ctypes.Structure):
 
 
 CFG_FULL_CONTEXT = 1  # aeth_llama_config.flags: keep max_seq_len past 4096 (up to 8192)
+CFG_KV_INT8 = 2  # aeth_llama_config.flags: the cache in 8 bits
 RUNNER_MAX_SEQ = 4096  # the cache length cap of LlamaRunner::new (runner.rs:225)
 
 

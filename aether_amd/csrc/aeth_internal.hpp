@@ -65,6 +65,7 @@ struct aeth_weight {
 };
 
 int aeth_num_cus();
+int aeth_fill_normal_launch(uint64_t seed, float* d_out, int64_t first, int64_t n, float mean, float stdv, hipStream_t s);
 int64_t aeth_blocks_per_row(int dtype, int64_t k);
 // Bytes of a weight's raw form: planar / rows: n·blocks_per_row·block_bytes;
 // GGUF order: (n·k / block_elems)·block_bytes. < 0 on a bad dtype / shape.

@@ -19,11 +19,22 @@ typedef float kv8_f4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
-__device__ __forceinline__ uint32_t kv8_umax16(uint32_t v) {  // max over the lane's 16-lane row
+template <int L>
+__device__ __forceinline__ uint32_t kv8_umax(uint32_t v) {  // max over aligned groups of L lanes (8, 16 or 32)
     v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));
     v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));
     v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));
-    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));
+    if (L >= 16) v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));
+    if (L >= 32) {
+        const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max(a[0], a[1]);
+    }
+    return v;
+}
+
+__device__ __forceinline__ uint32_t kv8_abs_max(uint32_t m, float4 y) {  // as integers: a NaN's bits are above an infinity's
+    m = max(max(m, __float_as_uint(y.x) & 0x7FFFFFFFu), __float_as_uint(y.y) & 0x7FFFFFFFu);
+    return max(max(m, __float_as_uint(y.z) & 0x7FFFFFFFu), __float_as_uint(y.w) & 0x7FFFFFFFu);
 }
 
 // 127 / amax in f64 to 2^-50 relative (amax > 0), by two Newton steps on the reciprocal instruction
@@ -51,6 +62,11 @@ __device__ __forceinline__ float4 kv8_ld4(const float* p, bool vec) {
         return make_float4(v.x, v.y, v.z, v.w);
     }
     return make_float4(p[0], p[1], p[2], p[3]);
+}
+
+__device__ __forceinline__ uint32_t kv8_code4(float4 y, double inv, bool finite) {
+    const uint32_t w = kv8_code(y.x, inv) | kv8_code(y.y, inv) << 8 | kv8_code(y.z, inv) << 16 | kv8_code(y.w, inv) << 24;
+    return finite ? w : 0;
 }
 
 struct AppendArgs {
@@ -101,20 +117,14 @@ __global__ void __launch_bounds__(256) k_kv8_append(AppendArgs A) {
         for (int p = 0; p < 2; p++) {
             uint32_t m = 0;
 #pragma unroll
-            for (int u = 0; u < V4; u++) {
-                const float4 y = x[r][p][u];
-                m = max(max(m, __float_as_uint(y.x) & 0x7FFFFFFFu), __float_as_uint(y.y) & 0x7FFFFFFFu);
-                m = max(max(m, __float_as_uint(y.z) & 0x7FFFFFFFu), __float_as_uint(y.w) & 0x7FFFFFFFu);
-            }
-            m = kv8_umax16(m);
+            for (int u = 0; u < V4; u++) m = kv8_abs_max(m, x[r][p][u]);
+            m = kv8_umax<16>(m);
             const bool finite = m < 0x7F800000u;
             const float amax = __uint_as_float(m);
             const double inv = finite && m > 0 ? kv8_inverse(amax) : 0.0;
 #pragma unroll
             for (int u = 0; u < V4; u++) {
-                const float4 y = x[r][p][u];
-                uint32_t w = kv8_code(y.x, inv) | kv8_code(y.y, inv) << 8 | kv8_code(y.z, inv) << 16 | kv8_code(y.w, inv) << 24;
-                if (!finite) w = 0;
+                const uint32_t w = kv8_code4(x[r][p][u], inv, finite);
                 if (p == 1) vs[t * LW + 16 * u + l16] = w;
                 else if (is_new) *(uint32_t*)(base + t * HD + 64 * u + 4 * l16) = w;
             }
@@ -412,6 +422,49 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_v(QkArgs A) {
                                          qk_rot1(a.w, b.w, sn.w, cs.w)}, (kv8_f4*)(dst + HALF));
 }
 
+// One token at device position and slot: hd / 8 lanes a head of q | k | v
+template <int HD>
+__global__ void __launch_bounds__(256) k_kv8_step(float* qkv, int nq, int nkv, const int* st, const float* sin_t, const float* cos_t,
+                                                  int64_t max_seq, int tiles, uint8_t* cache) {
+    constexpr int L = HD / 8, HALF = HD / 2;
+    const int unit = (blockIdx.x * 256 + threadIdx.x) / L, h = min(unit, nq + 2 * nkv - 1), e = 4 * (threadIdx.x % L);
+    float* src = qkv + (int64_t)h * HD + e;
+    float4 a = *(const float4*)src, b = *(const float4*)(src + HALF);
+    const int64_t p = min(max((int64_t)st[1], (int64_t)0), max_seq - 1), slot = st[2];
+    const float4 sn = *(const float4*)(sin_t + p * HALF + e), cs = *(const float4*)(cos_t + p * HALF + e);
+    if (h < nq + nkv) {
+        const float4 x = a, y = b;
+        a = make_float4(qk_rot0(x.x, y.x, sn.x, cs.x), qk_rot0(x.y, y.y, sn.y, cs.y), qk_rot0(x.z, y.z, sn.z, cs.z), qk_rot0(x.w, y.w, sn.w, cs.w));
+        b = make_float4(qk_rot1(x.x, y.x, sn.x, cs.x), qk_rot1(x.y, y.y, sn.y, cs.y), qk_rot1(x.z, y.z, sn.z, cs.z), qk_rot1(x.w, y.w, sn.w, cs.w));
+    }
+    const uint32_t m = kv8_umax<L>(kv8_abs_max(kv8_abs_max(0, a), b));
+    if (unit >= nq + 2 * nkv) return;
+    if (h < nq) {
+        *(float4*)src = a;
+        *(float4*)(src + HALF) = b;
+        return;
+    }
+    if (slot < 0 || slot >= max_seq) return;
+    const bool finite = m < 0x7F800000u;
+    const float amax = __uint_as_float(m);
+    const double inv = finite && m > 0 ? kv8_inverse(amax) : 0.0;
+    const uint32_t wa = kv8_code4(a, inv, finite), wb = kv8_code4(b, inv, finite);
+    const int v = h >= nq + nkv, t = (int)(slot & 63);
+    uint8_t* base = cache + ((int64_t)(h - nq - v * nkv) * tiles + (slot >> 6)) * aeth_kv8_tile_bytes(HD);
+    if (v) {
+        uint8_t* dst = base + KV8_TILE * HD + e * KV8_TILE + aeth_kv8_vbyte(t);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            dst[i * KV8_TILE] = (uint8_t)(wa >> (8 * i));
+            dst[(HALF + i) * KV8_TILE] = (uint8_t)(wb >> (8 * i));
+        }
+    } else {
+        *(uint32_t*)(base + t * HD + e) = wa;
+        *(uint32_t*)(base + t * HD + HALF + e) = wb;
+    }
+    if (e == 0) *(float*)(base + 2 * KV8_TILE * HD + 4 * (KV8_TILE * v + t)) = finite ? amax / 127.0f : __uint_as_float(0x7FC00000u);
+}
+
 // any even hd, any alignment: a wave a head, lanes over the pairs (read again for the rotation: the row is in cache)
 __global__ void __launch_bounds__(256) k_qk_norm_rope(QkArgs A) {
     const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -457,6 +510,16 @@ int aeth_qk_norm_rope_launch(const float* x, int64_t x_stride, int64_t n, int64_
     } else {
         hipLaunchKernelGGL(k_qk_norm_rope, dim3((unsigned)aeth_cdiv(n * heads, 4)), dim3(256), 0, s, A);
     }
+    AETH_LAUNCH_CHECK();
+    return AETH_OK;
+}
+
+int aeth_kv8_step_launch(float* qkv, int64_t nq, int64_t nkv, int64_t hd, const int* st, const float* sin_t, const float* cos_t,
+                         int64_t max_seq, void* cache, hipStream_t s) {
+    const dim3 grid((unsigned)aeth_cdiv((nq + 2 * nkv) * (hd / 8), 256)), block(256);
+    const int tiles = (int)aeth_cdiv(max_seq, KV8_TILE);
+    if (hd != 128) return aeth_set_error(AETH_EUNSUPPORTED, "8-bit cache step: head_dim %lld (needs 128)", (long long)hd);
+    hipLaunchKernelGGL(k_kv8_step<128>, grid, block, 0, s, qkv, (int)nq, (int)nkv, st, sin_t, cos_t, max_seq, tiles, (uint8_t*)cache);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }

@@ -40,6 +40,8 @@ struct aeth_runner {
     float* rope_sin = nullptr;    // [max_seq][hd/2]
     float* rope_cos = nullptr;
     float* kv = nullptr;          // [L][2][kvh][max_seq][hd]
+    uint8_t* kv8 = nullptr;       // AETH_CFG_KV_INT8: [L] 8-bit layer slices instead (kv is NULL)
+    void *a8_ws = nullptr, *p_a8_ws = nullptr;  // its attention's workspaces: a decode step's, a prompt's
     // activations
     float *x = nullptr, *normed = nullptr, *qkv = nullptr, *attn = nullptr, *gu = nullptr, *logits = nullptr;
     float* attn_ws = nullptr;
@@ -72,6 +74,10 @@ const int64_t kKvd(const aeth_llama_config& c) { return (int64_t)c.num_kv_heads 
 
 int64_t kv_layer_floats(const aeth_llama_config& c) {
     return 2LL * c.num_kv_heads * (int64_t)c.max_seq_len * c.head_dim;
+}
+
+int64_t kv8_layer_bytes(const aeth_llama_config& c) {
+    return aeth_kv8_layer_bytes(c.num_kv_heads, c.head_dim, c.max_seq_len);
 }
 
 // precompute_rope (runner.rs:1912-1924) with the host libm (f32 powf/sinf/cosf).
@@ -169,7 +175,7 @@ void runner_release(aeth_runner* r) {
     aeth_weight_free(r->lm_head);
     void* bufs[] = {r->norms, r->final_norm, r->emb, r->rope_sin, r->rope_cos, r->kv, r->x, r->normed, r->qkv,
                     r->attn, r->gu, r->logits, r->attn_ws, r->am_ws, r->st, r->tok_out, r->amax, r->xws,
-                    r->p_x, r->p_n, r->p_qkv, r->p_att, r->p_gu, r->p_h, r->p_tok};
+                    r->p_x, r->p_n, r->p_qkv, r->p_att, r->p_gu, r->p_h, r->p_tok, r->kv8, r->a8_ws, r->p_a8_ws};
     for (void* b : bufs)
         if (b) hipFree(b);
     if (r->host_out) hipHostFree(r->host_out);
@@ -202,7 +208,6 @@ int enqueue_layers(aeth_runner* r, int l0, int l1) {
     const int64_t d = c.d_model, hd = c.head_dim, nh = c.num_heads, nkv = c.num_kv_heads;
     int rc;
     for (int l = l0; l < l1; l++) {
-        float* lkv = r->kv + (int64_t)l * kv_layer_floats(c);
         GemvEpi e1 = step_epi(r);
         e1.norm_w = r->norms + (int64_t)l * 2 * d;
         e1.eps = c.rms_norm_eps;
@@ -219,9 +224,18 @@ int enqueue_layers(aeth_runner* r, int l0, int l1) {
                 (rc = aeth_gemv_launch_ex(r->wv[l], r->x, 1, r->qkv + qd + kvd, e1, s)))
                 return rc;
         }
-        if ((rc = aeth_attn_launch(nullptr, r->qkv, lkv, r->rope_sin, r->rope_cos, r->st, 0, nh, nkv, hd,
-                                   c.max_seq_len, c.sliding_window, r->attn_ws, r->attn, s)))
-            return rc;
+        if (r->kv8) {  // RoPE and the quantised append of the token, then the attention over fill + 1 slots
+            uint8_t* lkv = r->kv8 + l * kv8_layer_bytes(c);
+            if ((rc = aeth_kv8_step_launch(r->qkv, nh, nkv, hd, r->st, r->rope_sin, r->rope_cos, c.max_seq_len, lkv, s)) ||
+                (rc = aeth_attn_kv8_launch(r->qkv, nh * hd, lkv, 0, r->st + 2, 1, 1, 1, nh, nkv, hd, c.max_seq_len,
+                                           c.max_seq_len, c.sliding_window, r->attn, r->a8_ws, s)))
+                return rc;
+        } else {
+            float* lkv = r->kv + (int64_t)l * kv_layer_floats(c);
+            if ((rc = aeth_attn_launch(nullptr, r->qkv, lkv, r->rope_sin, r->rope_cos, r->st, 0, nh, nkv, hd,
+                                       c.max_seq_len, c.sliding_window, r->attn_ws, r->attn, s)))
+                return rc;
+        }
         GemvEpi e2 = step_epi(r);
         e2.flags = AETH_MM_ACCUMULATE;
         if ((rc = aeth_gemv_launch_ex(r->wo[l], r->attn, 1, r->x, e2, s))) return rc;
@@ -286,6 +300,8 @@ int ensure_prefill_buffers(aeth_runner* r, int64_t n) {
     }
     if (r->p_tok) AETH_HIP_CHECK(hipFree(r->p_tok));
     r->p_tok = nullptr;
+    if (r->p_a8_ws) AETH_HIP_CHECK(hipFree(r->p_a8_ws));
+    r->p_a8_ws = nullptr;
     r->p_cap = 0;
     for (int i = 0; i < 6; i++) {
         int rc = dmalloc(bufs[i], sizes[i]);
@@ -293,6 +309,7 @@ int ensure_prefill_buffers(aeth_runner* r, int64_t n) {
     }
     int rc = dmalloc(&r->p_tok, n);
     if (rc) return rc;
+    if (r->kv8 && (rc = dmalloc((uint8_t**)&r->p_a8_ws, aeth_attn_kv8_ws(1, n, c.num_heads, c.num_kv_heads, c.head_dim, n)))) return rc;
     r->p_cap = n;
     return AETH_OK;
 }
@@ -313,7 +330,6 @@ int runner_prefill_locked(aeth_runner* r, const int32_t* tokens, int32_t n, floa
     AETH_HIP_CHECK(hipMemcpyAsync(r->p_tok, tokens, sizeof(int32_t) * n, hipMemcpyHostToDevice, s));
     if ((rc = aeth_embed_rows_launch(r->emb, r->p_tok, n, d, r->p_x, s))) return rc;
     for (int l = 0; l < c.num_layers; l++) {
-        float* lkv = r->kv + (int64_t)l * kv_layer_floats(c);
         const float* attn_norm = r->norms + (int64_t)l * 2 * d;
         const float* ffn_norm = attn_norm + d;
         // the Q4_K, Q6_K and Q8_0 GEMMs take the RMSNorm inside their activation prep (the SwiGLU: below)
@@ -351,12 +367,22 @@ int runner_prefill_locked(aeth_runner* r, const int32_t* tokens, int32_t n, floa
                 return rc;
             }
         }
-        if ((rc = aeth_prefill_rope_kv_launch(r->p_qkv, n, nh, nkv, hd, r->rope_sin, r->rope_cos, c.max_seq_len,
-                                              lkv, s)))
-            return rc;
-        if ((rc = aeth_attn_prefill_launch(r->p_qkv, (nh + 2 * nkv) * hd, lkv, n, nh, nkv, hd, c.max_seq_len,
-                                           c.sliding_window, r->p_att, s)))
-            return rc;
+        const int64_t row = (nh + 2 * nkv) * hd;
+        if (r->kv8) {
+            uint8_t* lkv = r->kv8 + l * kv8_layer_bytes(c);
+            if ((rc = aeth_qk_norm_rope_launch(r->p_qkv, row, n, nh, nkv, hd, nullptr, nullptr, 0.0f, 0, nullptr, r->rope_sin,
+                                               r->rope_cos, c.max_seq_len, r->p_qkv, row, s)) ||
+                (rc = aeth_kv8_append_launch(lkv, 0, nullptr, 1, r->p_qkv + nh * hd, r->p_qkv + (nh + nkv) * hd, row, hd, n, nkv,
+                                             hd, c.max_seq_len, 0, s)) ||
+                (rc = aeth_attn_kv8_launch(r->p_qkv, row, lkv, 0, nullptr, 0, 1, n, nh, nkv, hd, c.max_seq_len, n,
+                                           c.sliding_window, r->p_att, r->p_a8_ws, s)))
+                return rc;
+        } else {
+            float* lkv = r->kv + (int64_t)l * kv_layer_floats(c);
+            if ((rc = aeth_prefill_rope_kv_launch(r->p_qkv, n, nh, nkv, hd, r->rope_sin, r->rope_cos, c.max_seq_len, lkv, s)) ||
+                (rc = aeth_attn_prefill_launch(r->p_qkv, row, lkv, n, nh, nkv, hd, c.max_seq_len, c.sliding_window, r->p_att, s)))
+                return rc;
+        }
         if ((rc = aeth_qmatmul(r->wo[l], r->p_att, n, r->p_x, AETH_MM_ACCUMULATE, s))) return rc;
         const float* h = r->p_h;
         GemmIn din;  // the down GEMM's producer
@@ -465,15 +491,17 @@ int runner_create_impl(const aeth_llama_config* cfg, const void* const* layer_we
     if (c.head_dim != 128 || c.num_heads / c.num_kv_heads > 8)
         return aeth_set_error(AETH_EUNSUPPORTED, "aeth_runner_create: the attention kernel needs head_dim 128 and "
                                                  "at most 8 query heads per KV head");
-    if (c.sliding_window < 0 || (c.flags & ~AETH_CFG_FULL_CONTEXT))
+    if (c.sliding_window < 0 || (c.flags & ~(AETH_CFG_FULL_CONTEXT | AETH_CFG_KV_INT8)))
         return aeth_set_error(AETH_EINVAL, "aeth_runner_create: sliding_window %d / flags %d", c.sliding_window, c.flags);
     // LlamaRunner::new and new_streaming size the cache and the RoPE table at
     // min(max_seq_len, 4096) (runner.rs:225, :339); a longer cache is an opt-in
     const int32_t eff_seq = (c.flags & AETH_CFG_FULL_CONTEXT) ? c.max_seq_len
                                                              : std::min<int32_t>(c.max_seq_len, AETH_RUNNER_MAX_SEQ);
-    if (eff_seq > 8192)
+    const bool int8 = (c.flags & AETH_CFG_KV_INT8) != 0;
+    const int32_t most = int8 ? 1 << 20 : 8192;
+    if (eff_seq > most)
         return aeth_set_error(AETH_EUNSUPPORTED, "aeth_runner_create: a cache of %d positions (the decode attention "
-                                                 "holds up to 8192)", eff_seq);
+                                                 "holds up to %d)", eff_seq, most);
     c.max_seq_len = eff_seq;
     bool need_seed = !lm_head || !embeddings || !final_norm || !layer_weights || !norms;
     if (need_seed && seed == 0)
@@ -570,8 +598,12 @@ int runner_create_impl(const aeth_llama_config* cfg, const void* const* layer_we
         hipMemcpy(r->rope_cos, rcs.data(), rcs.size() * 4, hipMemcpyHostToDevice) != hipSuccess) {
         return aeth_set_error(AETH_EHIP, "runner: rope upload failed");
     }
-    RC(dmalloc(&r->kv, (int64_t)c.num_layers * kv_layer_floats(c)));
-    if (hipMemsetAsync(r->kv, 0, sizeof(float) * (size_t)c.num_layers * kv_layer_floats(c), s) != hipSuccess) {
+    void* kv = nullptr;  // zeroed, as StaticKVCache's: code 0 times scale 0 in 8 bits
+    const size_t kv_bytes = (size_t)c.num_layers * (size_t)(int8 ? kv8_layer_bytes(c) : (int64_t)sizeof(float) * kv_layer_floats(c));
+    RC(dmalloc((uint8_t**)&kv, (int64_t)kv_bytes));
+    if (int8) r->kv8 = (uint8_t*)kv;
+    else r->kv = (float*)kv;
+    if (hipMemsetAsync(kv, 0, kv_bytes, s) != hipSuccess) {
         return aeth_set_error(AETH_EHIP, "runner: kv clear failed");
     }
     RC(dmalloc(&r->x, d));
@@ -580,8 +612,9 @@ int runner_create_impl(const aeth_llama_config* cfg, const void* const* layer_we
     RC(dmalloc(&r->attn, qd));
     RC(dmalloc(&r->gu, 2 * dff));  // h, or g | u when gate and up are separate
     RC(dmalloc(&r->logits, c.vocab_size));
-    RC(dmalloc(&r->attn_ws, aeth_attn_ws_floats(c.num_heads, c.head_dim, c.max_seq_len)));
-    if (hipMemset(r->attn_ws, 0, sizeof(float) * aeth_attn_ws_floats(c.num_heads, c.head_dim, c.max_seq_len)) !=
+    if (int8) RC(dmalloc((uint8_t**)&r->a8_ws, aeth_attn_kv8_ws(1, 1, c.num_heads, c.num_kv_heads, c.head_dim, c.max_seq_len)));
+    else RC(dmalloc(&r->attn_ws, aeth_attn_ws_floats(c.num_heads, c.head_dim, c.max_seq_len)));
+    if (!int8 && hipMemset(r->attn_ws, 0, sizeof(float) * aeth_attn_ws_floats(c.num_heads, c.head_dim, c.max_seq_len)) !=
         hipSuccess) {
         return aeth_set_error(AETH_EHIP, "runner: workspace clear failed");
     }
@@ -625,11 +658,73 @@ extern "C" AETH_API void* aeth_runner_stream(const aeth_runner* r) { return r ? 
 
 extern "C" AETH_API int aeth_runner_seq_len(const aeth_runner* r) { return r ? r->fill : -1; }
 
+namespace {
+// A layer of the cache in f32, [2][kv_heads][max_seq][head_dim], between the host and the 8-bit slices
+struct LayerCopy {
+    float* p = nullptr;
+    explicit LayerCopy(int64_t floats) {
+        if (hipMalloc((void**)&p, sizeof(float) * (size_t)floats) != hipSuccess) {
+            (void)hipGetLastError();
+            p = nullptr;
+        }
+    }
+    ~LayerCopy() {
+        if (p) (void)hipFree(p);  // (waits for the device)
+    }
+};
+
+int kv8_to_host(aeth_runner* r, float* host) {
+    const aeth_llama_config& c = r->cfg;
+    const int64_t hd = c.head_dim, ms = c.max_seq_len, lf = kv_layer_floats(c);
+    LayerCopy f(lf);
+    if (!f.p) return aeth_set_error(AETH_ENOMEM, "aeth_runner_kv_to_host: no memory for a layer in f32");
+    for (int l = 0; l < c.num_layers; l++) {
+        const int rc = aeth_kv8_read_launch(r->kv8 + l * kv8_layer_bytes(c), f.p, f.p + lf / 2, hd, ms * hd, ms, c.num_kv_heads, hd, ms, 0, r->stream);
+        if (rc) return rc;
+        AETH_HIP_CHECK(hipStreamSynchronize(r->stream));
+        AETH_HIP_CHECK(hipMemcpy(host + l * lf, f.p, sizeof(float) * (size_t)lf, hipMemcpyDeviceToHost));
+    }
+    return AETH_OK;
+}
+
+int kv8_from_host(aeth_runner* r, const float* host) {
+    const aeth_llama_config& c = r->cfg;
+    const int64_t hd = c.head_dim, ms = c.max_seq_len, lf = kv_layer_floats(c);
+    LayerCopy f(lf);
+    if (!f.p) return aeth_set_error(AETH_ENOMEM, "aeth_runner_kv_from_host: no memory for a layer in f32");
+    for (int l = 0; l < c.num_layers; l++) {
+        AETH_HIP_CHECK(hipMemcpy(f.p, host + l * lf, sizeof(float) * (size_t)lf, hipMemcpyHostToDevice));
+        const int rc = aeth_kv8_append_launch(r->kv8 + l * kv8_layer_bytes(c), 0, nullptr, 1, f.p, f.p + lf / 2, hd, ms * hd, ms, c.num_kv_heads, hd,
+                                              ms, 0, r->stream);
+        if (rc) return rc;
+        AETH_HIP_CHECK(hipStreamSynchronize(r->stream));
+    }
+    return AETH_OK;
+}
+}  // namespace
+
 extern "C" AETH_API int aeth_runner_fill_kv(aeth_runner* r, uint64_t seed, int32_t seq_len) {
     if (!r || seq_len < 0 || seq_len > r->cfg.max_seq_len)
         return aeth_set_error(AETH_EINVAL, "aeth_runner_fill_kv: bad argument");
     std::lock_guard<std::mutex> lk(r->mu);
     const aeth_llama_config& c = r->cfg;
+    if (r->kv8) {
+        // the f32 cache's numbers of the first seq_len positions, quantised; the rest cleared
+        const int64_t nkv = c.num_kv_heads, hd = c.head_dim, ms = c.max_seq_len, lf = kv_layer_floats(c);
+        AETH_HIP_CHECK(hipMemsetAsync(r->kv8, 0, (size_t)(c.num_layers * kv8_layer_bytes(c)), r->stream));
+        LayerCopy f(lf);
+        if (!f.p) return aeth_set_error(AETH_ENOMEM, "aeth_runner_fill_kv: no memory for a layer in f32");
+        for (int l = 0; l < c.num_layers; l++) {
+            int rc = aeth_fill_normal_launch(seed, f.p, l * lf, lf, 0.0f, 1.0f, r->stream);
+            if (rc || (rc = aeth_kv8_append_launch(r->kv8 + l * kv8_layer_bytes(c), 0, nullptr, 1, f.p, f.p + lf / 2, hd, ms * hd, seq_len,
+                                                   nkv, hd, ms, 0, r->stream)))
+                return rc;
+        }
+        AETH_HIP_CHECK(hipStreamSynchronize(r->stream));
+        r->fill = seq_len;
+        r->partial_valid = false;
+        return AETH_OK;
+    }
     // N(0,1) over the whole storage, then the unfilled tail cleared per head.
     int64_t tot = (int64_t)c.num_layers * kv_layer_floats(c);
     int rc = aeth_fill_normal_f32(seed, r->kv, tot, 0.0f, 1.0f, r->stream);
@@ -651,7 +746,12 @@ extern "C" AETH_API int aeth_runner_kv_to_host(aeth_runner* r, float* host, int3
     std::lock_guard<std::mutex> lk(r->mu);
     int64_t tot = (int64_t)r->cfg.num_layers * kv_layer_floats(r->cfg);
     AETH_HIP_CHECK(hipStreamSynchronize(r->stream));
-    AETH_HIP_CHECK(hipMemcpy(host, r->kv, sizeof(float) * tot, hipMemcpyDeviceToHost));
+    if (r->kv8) {
+        const int rc = kv8_to_host(r, host);
+        if (rc) return rc;
+    } else {
+        AETH_HIP_CHECK(hipMemcpy(host, r->kv, sizeof(float) * tot, hipMemcpyDeviceToHost));
+    }
     if (seq_len) *seq_len = r->fill;
     return AETH_OK;
 }
@@ -662,7 +762,12 @@ extern "C" AETH_API int aeth_runner_kv_from_host(aeth_runner* r, const float* ho
     std::lock_guard<std::mutex> lk(r->mu);
     int64_t tot = (int64_t)r->cfg.num_layers * kv_layer_floats(r->cfg);
     AETH_HIP_CHECK(hipStreamSynchronize(r->stream));
-    AETH_HIP_CHECK(hipMemcpy(r->kv, host, sizeof(float) * tot, hipMemcpyHostToDevice));
+    if (r->kv8) {
+        const int rc = kv8_from_host(r, host);
+        if (rc) return rc;
+    } else {
+        AETH_HIP_CHECK(hipMemcpy(r->kv, host, sizeof(float) * tot, hipMemcpyHostToDevice));
+    }
     r->fill = seq_len;
     r->partial_valid = false;
     return AETH_OK;

@@ -534,20 +534,24 @@ extern "C" AETH_API int aeth_fill_synthetic_raw(int dtype, uint64_t seed, void* 
     return AETH_OK;
 }
 
-__global__ void k_fill_normal(uint64_t seed, float* __restrict__ out, int64_t n, float mean, float stdv) {
+__global__ void k_fill_normal(uint64_t seed, float* __restrict__ out, int64_t n, float mean, float stdv, int64_t first) {
     int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n) return;
-    out[i] = mean + stdv * normal_at(splitmix64(seed ^ 0x6E6F726D616CULL), (uint64_t)i);
+    out[i] = mean + stdv * normal_at(splitmix64(seed ^ 0x6E6F726D616CULL), (uint64_t)(first + i));
+}
+
+// elements first .. first + n - 1 of the sequence that aeth_fill_normal_f32 writes
+int aeth_fill_normal_launch(uint64_t seed, float* d_out, int64_t first, int64_t n, float mean, float stdv, hipStream_t s) {
+    if (n == 0) return AETH_OK;
+    hipLaunchKernelGGL(k_fill_normal, dim3((unsigned)aeth_cdiv(n, 256)), dim3(256), 0, s, seed, d_out, n, mean, stdv, first);
+    AETH_LAUNCH_CHECK();
+    return AETH_OK;
 }
 
 extern "C" AETH_API int aeth_fill_normal_f32(uint64_t seed, float* d_out, int64_t n, float mean, float stdv,
                                              void* stream) {
     if (!d_out || n < 0) return aeth_set_error(AETH_EINVAL, "aeth_fill_normal_f32: bad argument");
-    if (n == 0) return AETH_OK;
-    hipLaunchKernelGGL(k_fill_normal, dim3((unsigned)aeth_cdiv(n, 256)), dim3(256), 0, (hipStream_t)stream, seed,
-                       d_out, n, mean, stdv);
-    AETH_LAUNCH_CHECK();
-    return AETH_OK;
+    return aeth_fill_normal_launch(seed, d_out, 0, n, mean, stdv, (hipStream_t)stream);
 }
 
 // ── measurement: a plain streaming read ──────────────────────────────────

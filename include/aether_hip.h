@@ -399,7 +399,12 @@ AETH_API int aeth_mfma_rate(int kind, int iters, int workgroups, float* d_sink, 
  * (runner.rs:225, :339), the runner's cache and RoPE table hold
  * min(max_seq_len, 4096) positions; flags AETH_CFG_FULL_CONTEXT keeps
  * max_seq_len instead (up to 8192, the decode attention's limit) — an
- * opt-in with no counterpart in the reference. */
+ * opt-in with no counterpart in the reference. AETH_CFG_KV_INT8 (none either)
+ * holds the cache in 8 bits, as aeth_kv8_append writes it: a quarter of the
+ * memory, contexts of up to 2^20 positions with AETH_CFG_FULL_CONTEXT, logits off
+ * by what 8 bits of K and V cost. aeth_runner_kv_from_host then quantises what
+ * it is given and aeth_runner_kv_to_host gives the values that the codes stand
+ * for; aeth_runner_fill_kv fills with the same numbers, quantised. */
 typedef struct aeth_llama_config {
     int32_t vocab_size, d_model, num_layers, num_heads, num_kv_heads, head_dim, d_ff, max_seq_len;
     float rope_base, rms_norm_eps;
@@ -407,6 +412,7 @@ typedef struct aeth_llama_config {
     int32_t flags;
 } aeth_llama_config;
 #define AETH_CFG_FULL_CONTEXT 1
+#define AETH_CFG_KV_INT8 2
 #define AETH_RUNNER_MAX_SEQ 4096
 
 typedef struct aeth_runner aeth_runner;

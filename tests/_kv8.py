@@ -122,3 +122,54 @@ def qk_norm_rope(x, nq, nk, hd, qw, kw, eps, positions, sin, cos):
     out = torch.cat([a * c - b * s, a * s + b * c], -1)
     mag = torch.cat([(a * c).abs() + (b * s).abs()] * 2, -1).maximum(torch.cat([(a * s).abs() + (b * c).abs()] * 2, -1))
     return out.reshape(n, -1), ((hd / 16 + 14) * U * mag).reshape(n, -1) + 1e-37
+
+
+def quantised(x):
+    """numpy [..., hd] f32 → the values its codes stand for (f32)."""
+    import numpy as np
+
+    c, s = codes(torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32)))
+    return (c.float() * s[..., None]).numpy()
+
+
+def model_logits(c, m, tokens):
+    """The last position's logits of a small test model (tests/_models.py) in float64, with every token's K and V
+    held in 8 bits: causal over `tokens` at positions 0 .. len-1, c["sliding_window"] as the runner's."""
+    import numpy as np
+
+    from oracle import oracle as O
+    from tests._model64 import _deq
+
+    d, nh, nkv, hd, dff, ms = (c[k] for k in ("d_model", "num_heads", "num_kv_heads", "head_dim", "d_ff", "max_seq_len"))
+    shapes = [(nh * hd, d), (nkv * hd, d), (nkv * hd, d), (d, nh * hd), (dff, d), (dff, d), (d, dff)]
+    sin, cos = (t.reshape(ms, hd // 2).astype(np.float64) for t in O.precompute_rope(ms, hd, c["rope_base"]))
+    n = len(tokens)
+    at = np.minimum(np.arange(n), ms - 1)
+    ago = np.arange(n)[:, None] - np.arange(n)
+    seen = (ago >= 0) & (ago < (c.get("sliding_window") or n))
+
+    def norm(v, w):
+        return v / np.sqrt((v * v).mean(-1, keepdims=True) + c["rms_norm_eps"]) * w.astype(np.float64)
+
+    def rotated(v):
+        a, b, s, k = v[..., :hd // 2], v[..., hd // 2:], sin[at][:, None], cos[at][:, None]
+        return np.concatenate([a * k - b * s, a * s + b * k], -1)
+
+    x = m["emb"].astype(np.float64)[np.asarray(tokens)]
+    for weights, (w_attn, w_ffn) in zip(m["layers"], m["norms"]):
+        wq, wk, wv, wo, wg, wu, wd = (_deq(t, w, *s) for t, w, s in zip(m["layer_dtype"], weights, shapes))
+        h = norm(x, w_attn)
+        q = rotated((h @ wq.T).reshape(n, nh, hd))
+        k = quantised(rotated((h @ wk.T).reshape(n, nkv, hd))).astype(np.float64)
+        v = quantised((h @ wv.T).reshape(n, nkv, hd)).astype(np.float64)
+        heads = []
+        for j in range(nh):
+            s = np.where(seen, q[:, j] @ k[:, j * nkv // nh].T / math.sqrt(hd), -np.inf)
+            p = np.exp(s - s.max(1, keepdims=True))
+            heads.append(p @ v[:, j * nkv // nh] / p.sum(1, keepdims=True))
+        x = x + np.concatenate(heads, 1) @ wo.T
+        h = norm(x, w_ffn)
+        g, u = h @ wg.T, h @ wu.T
+        with np.errstate(over="ignore"):
+            x = x + (g / (1 + np.exp(-g)) * u) @ wd.T
+    return _deq(m["lm_dtype"], m["lm"], c["vocab_size"], d) @ norm(x[-1], m["final"])

@@ -5,8 +5,8 @@ import math
 
 import pytest
 
-import _kv8 as R
 import aether_amd as A
+from tests import _kv8 as R
 
 pytestmark = pytest.mark.gpu
 
