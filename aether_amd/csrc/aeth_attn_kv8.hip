@@ -19,6 +19,8 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 
 #include "aeth_common.hpp"
 #include "aeth_internal.hpp"
@@ -46,7 +48,21 @@ struct A8 {
     int qvec, ovec;         // q rows / out 16-byte aligned
 };
 
-__device__ __forceinline__ float a8_max_rows(float v) { return aeth_max_rows(v); }
+// f(0) .. f(N - 1), each with its number as a constant
+template <int... I, class F>
+__device__ __forceinline__ void a8_unroll_(std::integer_sequence<int, I...>, F&& f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void a8_unroll(F&& f) {
+    a8_unroll_(std::make_integer_sequence<int, N>{}, f);
+}
+
+// lane I of the lane's row of 16: an operand modifier of the instruction that uses it
+template <int I>
+__device__ __forceinline__ float a8_row(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x150 + I, 0xF, 0xF, true));  // row_newbcast
+}
 
 // 2^j of the largest j with |x|·2^j <= 0x7F7F00 for |x| <= mx (three balanced digits), as its exponent;
 // 0 for mx = 0, infinite or NaN
@@ -90,15 +106,18 @@ __device__ __forceinline__ void a8_tiles(const A8& A, int len, int c0, int count
     if (end < beg) end = beg;
 }
 
-// Workgroup (KV head, column block of 16·NC, chunk, sequence): its four waves take the chunk's tiles round
-// robin, each with its own running softmax, and merge through LDS.
-template <int HD, int NC>
+// Workgroup (KV head, column block of 16, chunk, sequence): its four waves take the chunk's tiles round robin,
+// each with its own running softmax, and merge through LDS.
+// A token's scales belong to one register of every lane (lane group g holds tokens 16j + 4g + r in registers
+// 4j + r): lane i of a row of 16 holds the one of register i's token, and the multiplication takes it from there.
+template <int HD>
 __global__ void __launch_bounds__(256) k_attn8(A8 A) {
     constexpr int KS = HD / 64, DT = HD / 16, PLD = HD + 4;
     constexpr float TH = 8.0f;
-    __shared__ __attribute__((aligned(16))) float po[4][16 * NC][PLD];
-    __shared__ float pm[4][16 * NC], pl[4][16 * NC];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, g = lane >> 4;
+    __shared__ __attribute__((aligned(16))) float po[4][16][PLD];
+    __shared__ float pm[4][16], pl[4][16];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = blockIdx.x;
     const int h = id % A.nkv;
     id /= A.nkv;
@@ -106,34 +125,37 @@ __global__ void __launch_bounds__(256) k_attn8(A8 A) {
     const int chunk = id / A.ncb, seq = blockIdx.y;
     const int len = a8_len(A, seq);
     int beg, end;
-    a8_tiles(A, len, cb * 16 * NC, 16 * NC, beg, end);
+    a8_tiles(A, len, cb * 16, 16, beg, end);
     const int t0 = beg + chunk * A.tpc, t1 = min(t0 + A.tpc, end);
     if (t0 >= t1 && chunk > 0) return;  // (uniform) the merge leaves it out
     const uint8_t* head = A.cache + seq * A.seq_bytes + (int64_t)h * A.tiles * aeth_kv8_tile_bytes(HD);
 
     a8_i4 kf[4][KS], vf[DT];
-    a8_f4 sk[4], sv[4];
-    // codes read once go past the caches (131000 tokens: 47.6 µs against 51.4)
-    auto ld = [](const uint8_t* p) { return NC == 1 && HD <= 128 ? __builtin_nontemporal_load((const a8_i4*)p) : *(const a8_i4*)p; };
+    float sk, sv;
+    // codes that one workgroup alone reads go past the caches (131000 tokens: 47.6 µs against 51.4)
+    const bool once = A.ncb == 1;
     auto load = [&](int t) {
         const uint8_t* p = head + (int64_t)t * aeth_kv8_tile_bytes(HD);
+        const int st = 16 * ((lane >> 2) & 3) + 4 * g + (lane & 3);
+        sk = *(const float*)(p + 2 * KV8_TILE * HD + 4 * st);
+        sv = *(const float*)(p + 2 * KV8_TILE * HD + 4 * (KV8_TILE + st));
+        auto codes = [&](auto ld) {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+            for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int s = 0; s < KS; s++) kf[j][s] = ld(p + (16 * j + c) * HD + 64 * s + 16 * g);
+                for (int s = 0; s < KS; s++) kf[j][s] = ld((const a8_i4*)(p + (16 * j + c) * HD + 64 * s + 16 * g));
 #pragma unroll
-        for (int j = 0; j < 4; j++) sk[j] = *(const a8_f4*)(p + 2 * KV8_TILE * HD + 4 * (16 * j + 4 * g));
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) vf[dt] = ld(p + KV8_TILE * HD + (16 * dt + c) * KV8_TILE + 16 * g);
-#pragma unroll
-        for (int j = 0; j < 4; j++) sv[j] = *(const a8_f4*)(p + 2 * KV8_TILE * HD + 4 * (KV8_TILE + 16 * j + 4 * g));
+            for (int dt = 0; dt < DT; dt++) vf[dt] = ld((const a8_i4*)(p + KV8_TILE * HD + (16 * dt + c) * KV8_TILE + 16 * g));
+        };
+        if (once) codes([](const a8_i4* a) { return __builtin_nontemporal_load(a); });
+        else codes([](const a8_i4* a) { return *a; });
     };
-    // the columns: q (its loads go out first), the keys [lo, hi) they see
-    float qv[NC][KS][16];
-#pragma unroll
-    for (int u = 0; u < NC; u++) {
-        const int xc = min(cb * 16 * NC + 16 * u + c, A.cols - 1), i = xc / A.G;
-        const float* src = A.q + ((int64_t)seq * A.n + i) * A.q_stride + (int64_t)(h * A.G + xc % A.G) * HD + 16 * g;
+
+    // the column: q (its loads go out first), the keys [lo, hi) it sees
+    const int x = cb * 16 + c, xc = min(x, A.cols - 1), qi = xc / A.G;
+    float qv[KS][16];
+    {
+        const float* src = A.q + ((int64_t)seq * A.n + qi) * A.q_stride + (int64_t)(h * A.G + xc % A.G) * HD + 16 * g;
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -141,171 +163,139 @@ __global__ void __launch_bounds__(256) k_attn8(A8 A) {
                 float4 y;
                 if (A.qvec) y = *(const float4*)(src + 64 * s + e);
                 else y = make_float4(src[64 * s + e], src[64 * s + e + 1], src[64 * s + e + 2], src[64 * s + e + 3]);
-                qv[u][s][e] = y.x;
-                qv[u][s][e + 1] = y.y;
-                qv[u][s][e + 2] = y.z;
-                qv[u][s][e + 3] = y.w;
+                qv[s][e] = y.x;
+                qv[s][e + 1] = y.y;
+                qv[s][e + 2] = y.z;
+                qv[s][e + 3] = y.w;
             }
     }
     __builtin_amdgcn_sched_barrier(0);
     if (t0 + w < t1) load(t0 + w);
     __builtin_amdgcn_sched_barrier(0);
-    uint32_t qd[NC][3][KS][4];
-    float qs[NC], m[NC], l[NC];
-    int lo[NC], hi[NC];
-    a8_f4 o[NC][DT];
-#pragma unroll
-    for (int u = 0; u < NC; u++) {
-        const int x = cb * 16 * NC + 16 * u + c, xc = min(x, A.cols - 1), i = xc / A.G;
-        float mx;
+    a8_i4 qd[3][KS];  // q's digits
+    float qs;
+    {
         uint32_t mb = 0;
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                mb = max(mb, __float_as_uint(qv[u][s][e]) & 0x7FFFFFFFu);
-            }
-        {   // over the four lane groups, as integers: a NaN's bits are above an infinity's
-            const auto a = __builtin_amdgcn_permlane16_swap(mb, mb, false, false);
-            mb = max(a[0], a[1]);
-            const auto b = __builtin_amdgcn_permlane32_swap(mb, mb, false, false);
-            mb = max(b[0], b[1]);
-        }
-        mx = __uint_as_float(mb);
-        const int e2 = a8_exponent(mx);
+            for (int e = 0; e < 16; e++) mb = max(mb, __float_as_uint(qv[s][e]) & 0x7FFFFFFFu);
+        // over the four lane groups, as integers: a NaN's bits are above an infinity's
+        const auto a = __builtin_amdgcn_permlane16_swap(mb, mb, false, false);
+        mb = max(a[0], a[1]);
+        const auto b = __builtin_amdgcn_permlane32_swap(mb, mb, false, false);
+        mb = max(b[0], b[1]);
+        const int e2 = a8_exponent(__uint_as_float(mb));
         const float f = a8_pow2(e2);
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-                a8_digits((uint32_t)(int)rintf(qv[u][s][e] * f), (uint32_t)(int)rintf(qv[u][s][e + 1] * f),
-                          (uint32_t)(int)rintf(qv[u][s][e + 2] * f), (uint32_t)(int)rintf(qv[u][s][e + 3] * f), qd[u][0][s][e / 4],
-                          qd[u][1][s][e / 4], qd[u][2][s][e / 4]);
+            for (int e = 0; e < 4; e++) {
+                uint32_t d0, d1, d2;
+                a8_digits((uint32_t)(int)rintf(qv[s][4 * e] * f), (uint32_t)(int)rintf(qv[s][4 * e + 1] * f),
+                          (uint32_t)(int)rintf(qv[s][4 * e + 2] * f), (uint32_t)(int)rintf(qv[s][4 * e + 3] * f), d0, d1, d2);
+                qd[0][s][e] = (int)d0;
+                qd[1][s][e] = (int)d1;
+                qd[2][s][e] = (int)d2;
+            }
         // an infinity or NaN in q: every score NaN
-        qs[u] = mb >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : a8_pow2(-e2) * (1.4426950408889634f / sqrtf((float)HD));
-        m[u] = -INFINITY;
-        l[u] = 0.0f;
-        hi[u] = len - A.n + i + 1;
-        lo[u] = A.window > 0 ? hi[u] - A.window : 0;
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) o[u][dt] = (a8_f4){0.0f, 0.0f, 0.0f, 0.0f};
+        qs = mb >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : a8_pow2(-e2) * (1.4426950408889634f / sqrtf((float)HD));
     }
+    const int hi = len - A.n + qi + 1, lo = A.window > 0 ? hi - A.window : 0;
     // every column of the block sees the keys [all_lo, all_hi)
-    const int all_hi = len - A.n + (cb * 16 * NC) / A.G + 1;
-    const int all_lo = A.window > 0 ? len - A.n + (min(cb * 16 * NC + 16 * NC, A.cols) - 1) / A.G + 1 - A.window : 0;
+    const int all_hi = len - A.n + (cb * 16) / A.G + 1;
+    const int all_lo = A.window > 0 ? len - A.n + (min(cb * 16 + 16, A.cols) - 1) / A.G + 1 - A.window : 0;
+    float m = -INFINITY, l = 0.0f;
+    a8_f4 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) o[dt] = (a8_f4){0.0f, 0.0f, 0.0f, 0.0f};
 
     const a8_i4 zero = {0, 0, 0, 0};
     for (int t = t0 + w; t < t1; t += 4) {
-        const bool edge = 64 * t < all_lo || 64 * t + 64 > all_hi;  // (uniform) some key is masked
-        // V scales that are no numbers (append writes NaN): rare
-        uint32_t vb = 0;
+        {   // a V scale that is no number goes to the token's K scale: its scores are NaN where it is seen
+            const bool fine = fabsf(sv) < INFINITY;
+            sk = fine ? sk : __uint_as_float(0x7FC00000u);
+            sv = fine ? sv : 0.0f;
+        }
+        float s[16];
+        a8_unroll<4>([&](auto jj) {
+            constexpr int j = jj;
+            a8_i4 d[3];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+            for (int p = 0; p < 3; p++) {
+                d[p] = zero;
 #pragma unroll
-            for (int r = 0; r < 4; r++) vb = max(vb, __float_as_uint(sv[j][r]) & 0x7FFFFFFFu);
-        const bool vbad = __any(vb >= 0x7F800000u);
-#pragma unroll
-        for (int u = 0; u < NC; u++) {
-            float s[16];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                a8_i4 d[3];
-#pragma unroll
-                for (int p = 0; p < 3; p++) {
-                    d[p] = zero;
-#pragma unroll
-                    for (int ks = 0; ks < KS; ks++) {
-                        const a8_i4 b = {(int)qd[u][p][ks][0], (int)qd[u][p][ks][1], (int)qd[u][p][ks][2], (int)qd[u][p][ks][3]};
-                        d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[j][ks], b, d[p], 0, 0, 0);
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    s[4 * j + r] = fmaf((float)((d[2][r] << 8) + d[1][r]), 256.0f, (float)d[0][r]) * (sk[j][r] * qs[u]);
+                for (int ks = 0; ks < KS; ks++) d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[j][ks], qd[p][ks], d[p], 0, 0, 0);
             }
-            float wv[16];
-#pragma unroll
-            for (int i = 0; i < 16; i++) wv[i] = sv[i >> 2][i & 3];
-            if (edge) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int key = 64 * t + 16 * (i >> 2) + 4 * g + (i & 3);
-                    const bool seen = key >= lo[u] && key < hi[u];
-                    s[i] = seen ? s[i] : -INFINITY;
-                    wv[i] = seen ? wv[i] : 0.0f;
-                }
-            }
-            if (vbad) {
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    if (!(fabsf(wv[i]) < INFINITY)) {
-                        wv[i] = 0.0f;
-                        l[u] = __uint_as_float(0x7FC00000u);
-                    }
-            }
-            float mx = s[0];
-#pragma unroll
-            for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
-            mx = a8_max_rows(mx);
-            if (__any(mx > m[u] + TH)) {  // (uniform)
-                const float mn = fmaxf(m[u], mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
-                l[u] *= al;
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++) o[u][dt] *= al;
-                m[u] = mn;
-            }
-            const float mo = m[u] == -INFINITY ? 0.0f : m[u];  // every key masked so far: s - mo is -Inf
-            float wm = 0.0f, ps = 0.0f;
+            a8_unroll<4>([&](auto rr) {
+                constexpr int r = rr, i = 4 * j + r;
+                s[i] = fmaf((float)((d[2][r] << 8) + d[1][r]), 256.0f, (float)d[0][r]) * a8_row<i>(sk);
+            });
+        });
+        if (64 * t < all_lo || 64 * t + 64 > all_hi) {  // (uniform) some key is masked
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const float p = __builtin_amdgcn_exp2f(s[i] - mo);
-                ps += p;
-                wv[i] *= p;
-                wm = fmaxf(wm, wv[i]);
+                const int key = 64 * t + 16 * (i >> 2) + 4 * g + (i & 3);
+                s[i] = key >= lo && key < hi ? s[i] : -INFINITY;
             }
-            l[u] += ps;
-            wm = a8_max_rows(wm);
-            if (!(wm < INFINITY)) l[u] = __uint_as_float(0x7FC00000u);  // values past 2^119: no number rather than a wrong one
-            const int j2 = a8_exponent(wm);
-            const float f = a8_pow2(j2), fi = a8_pow2(-j2);
-            uint32_t pd[3][4];
+        }
+        float mx = s[0];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t x[4];
+        for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
+        mx = aeth_max_rows(mx) * qs;
+        if (__any(mx > m + TH)) {  // (uniform)
+            const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= al;
 #pragma unroll
-                for (int r = 0; r < 4; r++) x[r] = __float_as_uint(fmaf(wv[4 * j + r], f, 8388608.0f));
-                a8_digits(x[0], x[1], x[2], x[3], pd[0][j], pd[1][j], pd[2][j]);
-            }
+            for (int dt = 0; dt < DT; dt++) o[dt] *= al;
+            m = mn;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;  // every key masked so far: s is -Inf
+        float wm = 0.0f, ps = 0.0f;
+        a8_unroll<16>([&](auto at) {
+            constexpr int i = at;
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[i], qs, -ref));
+            ps += p;
+            s[i] = p * a8_row<i>(sv);
+            wm = fmaxf(wm, s[i]);
+        });
+        l += ps;
+        wm = aeth_max_rows(wm);
+        if (!(wm < INFINITY)) l = __uint_as_float(0x7FC00000u);  // values past 2^119: no number rather than a wrong one
+        const int j2 = a8_exponent(wm);
+        const float f = a8_pow2(j2), fi = a8_pow2(-j2), fi8 = a8_pow2(8 - j2);
+        a8_i4 pd[3];
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) {
-                a8_i4 d[3];
+        for (int j = 0; j < 4; j++) {
+            uint32_t y[4], d0, d1, d2;
 #pragma unroll
-                for (int p = 0; p < 3; p++) {
-                    const a8_i4 b = {(int)pd[p][0], (int)pd[p][1], (int)pd[p][2], (int)pd[p][3]};
-                    d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[dt], b, zero, 0, 0, 0);
-                }
+            for (int r = 0; r < 4; r++) y[r] = __float_as_uint(fmaf(s[4 * j + r], f, 8388608.0f));
+            a8_digits(y[0], y[1], y[2], y[3], d0, d1, d2);
+            pd[0][j] = (int)d0;
+            pd[1][j] = (int)d1;
+            pd[2][j] = (int)d2;
+        }
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    o[u][dt][r] = fmaf(fmaf((float)((d[2][r] << 8) + d[1][r]), 256.0f, (float)d[0][r]), fi, o[u][dt][r]);
-            }
+        for (int dt = 0; dt < DT; dt++) {
+            a8_i4 d[3];
+#pragma unroll
+            for (int p = 0; p < 3; p++) d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[dt], pd[p], zero, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; r++) o[dt][r] = fmaf((float)((d[2][r] << 8) + d[1][r]), fi8, fmaf((float)d[0][r], fi, o[dt][r]));
         }
         if (t + 4 < t1) load(t + 4);
     }
+    l = aeth_sum_rows(l);
 #pragma unroll
-    for (int u = 0; u < NC; u++) {
-        l[u] = aeth_sum_rows(l[u]);
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) *(a8_f4*)&po[w][16 * u + c][16 * dt + 4 * g] = o[u][dt];
-        if (g == 0) {
-            pm[w][16 * u + c] = m[u];
-            pl[w][16 * u + c] = l[u];
-        }
+    for (int dt = 0; dt < DT; dt++) *(a8_f4*)&po[w][c][16 * dt + 4 * g] = o[dt];
+    if (g == 0) {
+        pm[w][c] = m;
+        pl[w][c] = l;
     }
     __syncthreads();
-    const int unit = (seq * A.nkv + h) * A.ncb + cb;
-    float* part = A.ws + ((int64_t)unit * A.chunks + chunk) * (16 * NC) * (HD + 2);
-    for (int at = tid; at < 16 * NC * HD / 4; at += 256) {
-        const int cc = at / (HD / 4), d = 4 * (at % (HD / 4)), x = cb * 16 * NC + cc;
+    float* part = A.ws + ((int64_t)((seq * A.nkv + h) * A.ncb + cb) * A.chunks + chunk) * 16 * (HD + 2);
+    for (int at = tid; at < 16 * HD / 4; at += 256) {
+        const int cc = at / (HD / 4), d = 4 * (at % (HD / 4)), x = cb * 16 + cc;
         if (x >= A.cols) continue;
         float M = -INFINITY;
 #pragma unroll
@@ -321,8 +311,8 @@ __global__ void __launch_bounds__(256) k_attn8(A8 A) {
         if (A.chunks > 1) {
             *(a8_f4*)(part + cc * HD + d) = acc;
             if (d == 0) {
-                part[16 * NC * HD + 2 * cc] = M;
-                part[16 * NC * HD + 2 * cc + 1] = L;
+                part[16 * HD + 2 * cc] = M;
+                part[16 * HD + 2 * cc + 1] = L;
             }
             continue;
         }
@@ -350,6 +340,7 @@ __global__ void __launch_bounds__(256) k_attn8(A8 A) {
 typedef _Float16 a8_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 a8_h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 a8_h2 __attribute__((ext_vector_type(2)));
+typedef float a8_f2 __attribute__((ext_vector_type(2)));
 typedef float a8_f16 __attribute__((ext_vector_type(16)));
 
 // four signed bytes as fp16
@@ -367,9 +358,11 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
     static_assert(CH >= 1 && CH * NT == 4 * HD, "16-byte pieces of a plane a thread");
     constexpr int KF = 1040;  // bytes from one K fragment to the next: eight threads of a row store to eight bank groups
     constexpr float TH = 8.0f;
+    // V's buffers: three spare a barrier a tile; two let two workgroups of four waves share a CU's LDS
+    constexpr int NB = NW == 8 ? 3 : 2;
     __shared__ __attribute__((aligned(16))) char kb[2][2 * KS * KF];
-    __shared__ __attribute__((aligned(16))) char vb[2][DT * 4 * 1024];
-    __shared__ __attribute__((aligned(16))) float sc[2][2 * KV8_TILE];
+    __shared__ __attribute__((aligned(16))) char vb[NB][DT * 4 * 1024];
+    __shared__ __attribute__((aligned(16))) float sc[NB][2 * KV8_TILE];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = blockIdx.x;
@@ -399,7 +392,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
 #pragma unroll
         for (int u = 0; u < CH; u++) rv[u] = *(const uint4*)(p + 16 * (tid + NT * u));
     };
-    auto stage_k = [&](int b) {  // token t, dimensions 16·ks .. + 15 → lanes t%32 and 32 + t%32 of fragment (t/32, ks)
+    auto stage_k = [&](int b, int b3) {  // token t, dimensions 16·ks .. + 15 → lanes t%32 and 32 + t%32 of fragment (t/32, ks)
 #pragma unroll
         for (int u = 0; u < CH; u++) {
             const int at = tid + NT * u, t = at / KS, ks = at % KS;
@@ -411,8 +404,8 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
         // a V scale that is no number goes to the token's K scale: its scores are NaN where it is seen
         if (tid < KV8_TILE) {
             const bool fine = fabsf(rsv) < INFINITY;
-            sc[b][tid] = fine ? rsk : __uint_as_float(0x7FC00000u);
-            sc[b][KV8_TILE + tid] = fine ? rsv : 0.0f;
+            sc[b3][tid] = fine ? rsk : __uint_as_float(0x7FC00000u);
+            sc[b3][KV8_TILE + tid] = fine ? rsv : 0.0f;
         }
     };
     auto stage_v = [&](int b) {  // dimension d, token group g = 2a + half → half of a lane's eight tokens of fragments (d/32, j)
@@ -433,10 +426,9 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
 
     const int x0 = cb * 32 * NW + 32 * w, x = x0 + c, xc = min(x, A.cols - 1), qi = xc / A.G;
     const int hi = len - A.n + qi + 1, lo = A.window > 0 ? hi - A.window : 0;
-    // of the wave: every column sees [all_lo, all_hi), none outside [any_lo, any_hi)
+    // every column of the wave sees the keys [all_lo, all_hi)
     const int i0 = min(x0, A.cols - 1) / A.G, i1 = min(x0 + 31, A.cols - 1) / A.G;
-    const int all_hi = len - A.n + i0 + 1, any_hi = len - A.n + i1 + 1;
-    const int all_lo = A.window > 0 ? any_hi - A.window : 0, any_lo = A.window > 0 ? all_hi - A.window : 0;
+    const int all_hi = len - A.n + i0 + 1, all_lo = A.window > 0 ? len - A.n + i1 + 1 - A.window : 0;
     a8_h8 qh[KS], ql[KS];
     float qs;
     {
@@ -471,50 +463,27 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
         // an infinity or NaN in q: every score NaN
         qs = mb >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : a8_pow2(-e2) * (1.4426950408889634f / sqrtf((float)HD));
     }
-    float m = -INFINITY, l = 0.0f, top = 0.0f, fw = 1.0f;  // the largest p·sv so far; its power of two
+    // m: the largest score so far, up to 2^TH stale; a probability is 2^(score - ref), ref = m - lf, lf a whole number
+    // that keeps the largest p·sv so far (top) in [2^9, 2^15)
+    float m = -INFINITY, l = 0.0f, top = 0.0f, lf = 0.0f, ref = 0.0f;
     a8_f16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) o[dt] = (a8_f16){};
+    a8_f16 s = (a8_f16){}, sn = (a8_f16){};  // this step's scores, the next one's products as they form
+    constexpr int EK = 16 / KS, EV = 8 / DT;  // scores beside a k-step's products, beside a value fragment's
 
-    if (t0 < t1) {
-        stage_k(0);
-        stage_v(0);
-        if (t0 + 1 < t1) {
-            fetch_k(t0 + 1);
-            fetch_v(t0 + 1);
-        }
-    }
-    a8_f16 s;
-    a8_h8 ph[2], pl[2];
-    auto scores = [&](int b, int T) {
-        s = (a8_f16){};
+    // A token's scale belongs to a register of every lane: lane i of a row of 16 holds the one of register i's token, and
+    // the multiplication takes it from there (one LDS word a lane and step in place of sixteen)
+    const int st = 8 * ((lane >> 2) & 3) + 4 * hf + (lane & 3);
+    auto scales = [&](int b3, int T, int part) { return sc[b3][KV8_TILE * part + 32 * T + st]; };
+    auto rescale = [&](float al) {
+        l *= al;
+        top *= al;
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const a8_h8 kf = *(const a8_h8*)(kb[b] + (T * KS + ks) * KF + lane * 16);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[ks], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[ks], s, 0, 0, 0);
-        }
+        for (int dt = 0; dt < DT; dt++) o[dt] *= al;
     };
-    auto values = [&](int b, int T) {
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) {
-                const a8_h8 vf = *(const a8_h8*)(vb[b] + (dt * 4 + 2 * T + u) * 1024 + lane * 16);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[u], o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[u], o[dt], 0, 0, 0);
-            }
-    };
-    auto softmax = [&](int t, int b, int T) {
-        const int k0 = 64 * t + 32 * T;
-        a8_f4 sk[4], sv[4];
-#pragma unroll
-        for (int a = 0; a < 4; a++) {
-            sk[a] = *(const a8_f4*)&sc[b][32 * T + 8 * a + 4 * hf];
-            sv[a] = *(const a8_f4*)&sc[b][KV8_TILE + 32 * T + 8 * a + 4 * hf];
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[i] *= sk[i >> 2][i & 3];
+    // s, times its K scales, is a step's scores: masks them and follows their maximum
+    auto bound_scores = [&](int k0) {
         if (k0 < all_lo || k0 + 32 > all_hi) {  // (uniform) some key is masked
 #pragma unroll
             for (int i = 0; i < 16; i++) {
@@ -525,77 +494,134 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
-        {
-            const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-            mx = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])) * qs;
-        }
+        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])) * qs;
         if (__any(mx > m + TH)) {  // (uniform)
-            const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-            l *= al;
-            top *= al;
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) o[dt] *= al;
+            const float mn = fmaxf(m, mx);
+            rescale(mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn));
             m = mn;
-        }
-        const float mo = m == -INFINITY ? 0.0f : m;
-        float wm = 0.0f, ps = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[i], qs, -mo));
-            ps += p;
-            s[i] = p * sv[i >> 2][i & 3];
-            wm = fmaxf(wm, s[i]);
-        }
-        l += ps;
-        {
-            const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(wm), __float_as_uint(wm), false, false);
-            wm = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-        }
-        top = fmaxf(top, wm);
-        if (__any(top > 0.0f && !(top * fw >= 512.0f && top * fw < 32768.0f))) {  // (uniform) out of its power of two's range
-            if (!(top < INFINITY)) l = __uint_as_float(0x7FC00000u);  // values past 2^119: no number rather than a wrong one
-            const float fn = top > 0.0f ? a8_pow2(a8_exponent(top) - 12) : fw;  // top·fn in [2^10, 2^11)
-            const float fi = 1.0f / fw;
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) o[dt] = o[dt] * fi * fn;
-            fw = fn;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float v = s[i] * fw;
-            asm("" : "+v"(v));  // (one product for both parts)
-            const _Float16 y = (_Float16)v;
-            ph[i >> 3][i & 7] = y;
-            pl[i >> 3][i & 7] = (_Float16)(v - (float)y);
+            ref = (m == -INFINITY ? 0.0f : m) - lf;
         }
     };
-    __syncthreads();
-    for (int t = t0; t < t1; t++) {
-        const int b = (t - t0) & 1;
-        if (t + 1 < t1) {
-            stage_k(b ^ 1);
-            stage_v(b ^ 1);
-            if (t + 2 < t1) {
-                fetch_k(t + 2);
-                fetch_v(t + 2);
-            }
-        }
+    // One step of 32 keys whose scores stand in s: its probabilities beside the products of the next step's scores,
+    // its values' products beside what turns those into scores. The two run on different units, and the SIMD's
+    // other wave fills what one leaves.
+    auto step = [&](int b3, int T, const char* kp, int nb3, int nT, auto between) {
+        const float sv = scales(b3, T, 1);
+        a8_h8 kf[2] = {*(const a8_h8*)kp, *(const a8_h8*)(kp + KF)};
+        sn = (a8_f16){};
+        float wm = 0.0f, ps = 0.0f;
+        auto add = [&](auto at) {
+            constexpr int i = at;
+            ps += s[i];
+            s[i] *= a8_row<i>(sv);
+            wm = fmaxf(wm, s[i]);
+        };
+        a8_unroll<KS>([&](auto ks) {
+            sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks & 1], ql[ks], sn, 0, 0, 0);
+            sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks & 1], qh[ks], sn, 0, 0, 0);
+            if (ks + 2 < KS) kf[ks & 1] = *(const a8_h8*)(kp + (ks + 2) * KF);
+            a8_unroll<EK>([&](auto e) {
+                constexpr int i = EK * ks + e;
+                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], qs, -ref));
+                if constexpr (ks > 0) add(std::integral_constant<int, i - EK>{});
+            });
+        });
+        a8_unroll<EK>([&](auto e) { add(std::integral_constant<int, 16 - EK + e>{}); });
+        l += ps;
+        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(wm), __float_as_uint(wm), false, false);
+        top = fmaxf(top, fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+        if (__any(top > 0.0f && !(top >= 512.0f && top < 32768.0f))) {  // (uniform)
+            if (!(top < INFINITY)) l = __uint_as_float(0x7FC00000u);  // values past 2^119: no number rather than a wrong one
+            const int d = top > 0.0f && top < INFINITY ? a8_exponent(top) - 12 : 0;  // top·2^d in [2^10, 2^11)
+            const float al = a8_pow2(min(max(d, -126), 126));
+            rescale(al);
 #pragma unroll
-        for (int T = 0; T < 2; T++) {
-            const int k0 = 64 * t + 32 * T;
-            if (k0 >= any_hi || k0 + 32 <= any_lo) continue;  // (uniform in the wave) no column sees any
-            scores(b, T);
-            softmax(t, b, T);
-            values(b, T);
+            for (int i = 0; i < 16; i++) s[i] *= al;
+            lf += (float)d;
+            ref = (m == -INFINITY ? 0.0f : m) - lf;
         }
+        between();
+        const char* vp = vb[b3] + 2 * T * 1024 + lane * 16;
+        a8_h8 vf[2] = {*(const a8_h8*)vp, *(const a8_h8*)(vp + 4096)}, ph[2], pl[2];
+        const float sk = scales(nb3, nT, 0);
+        auto part = [&](int i) {  // hi and lo of s[i] and s[i + 1]: one packed conversion, two mixed-precision subtractions
+            const a8_h2 y = __builtin_convertvector((a8_f2){s[i], s[i + 1]}, a8_h2);
+            ph[i >> 3][i & 7] = y[0];
+            ph[i >> 3][(i & 7) + 1] = y[1];
+            a8_h2 z;
+            asm("v_fma_mixlo_f16 %0, %1, 1.0, -%2 op_sel_hi:[0,0,1]" : "=v"(z) : "v"(s[i]), "v"(y));
+            asm("v_fma_mixhi_f16 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(z) : "v"(s[i + 1]), "v"(y));
+            pl[i >> 3][i & 7] = z[0];
+            pl[i >> 3][(i & 7) + 1] = z[1];
+        };
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) part(i);
+        a8_unroll<2 * DT>([&](auto f) {  // (token half u, dimensions dt)
+            constexpr int u = f / DT, dt = f % DT, n = f + 2;
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[f & 1], pl[u], o[dt], 0, 0, 0);
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[f & 1], ph[u], o[dt], 0, 0, 0);
+            if (n < 2 * DT) vf[f & 1] = *(const a8_h8*)(vp + (n % DT) * 4096 + n / DT * 1024);
+            a8_unroll<EV>([&](auto e) {
+                constexpr int i = EV * f + e;
+                if (f < DT && i % 2 == 0) part(i + 8);
+                s[i] = sn[i] * a8_row<i>(sk);
+            });
+        });
+    };
+    if (t0 < t1) {
+        stage_k(0, 0);
+        stage_v(0);
+        if (t0 + 1 < t1) {
+            fetch_k(t0 + 1);
+            fetch_v(t0 + 1);
+        }
+    }
+    __syncthreads();
+    if (t0 < t1) {  // the first step's scores
+        const char* kp = kb[0] + lane * 16;
+        const float sk = scales(0, 0, 0);
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const a8_h8 kf = *(const a8_h8*)(kp + ks * KF);
+            sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[ks], sn, 0, 0, 0);
+            sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[ks], sn, 0, 0, 0);
+        }
+        a8_unroll<16>([&](auto at) {
+            constexpr int i = at;
+            s[i] = sn[i] * a8_row<i>(sk);
+        });
+        bound_scores(64 * t0);
+    }
+    // One barrier a tile, between its two steps: the codes of the next tile are stored before it, to K's other buffer,
+    // whose last readers were two steps back, and V's third, whose readers were three (of two: one, behind a second
+    // barrier). (Behind the last tile a step's
+    // "next" scores are of what the other buffer holds: all masked.)
+    int b3 = 0;
+    for (int t = t0; t < t1; t++) {
+        const int b = (t - t0) & 1, n3 = b3 == NB - 1 ? 0 : b3 + 1;
+        step(b3, 0, kb[b] + KS * KF + lane * 16, b3, 1, [&] {
+            if (t + 1 < t1) {
+                stage_k(b ^ 1, n3);
+                stage_v(n3);
+                if (t + 2 < t1) {
+                    fetch_k(t + 2);
+                    fetch_v(t + 2);
+                }
+            }
+        });
+        bound_scores(64 * t + 32);
         __syncthreads();
+        step(b3, 1, kb[b ^ 1] + lane * 16, n3, 0, [] {});
+        bound_scores(64 * t + 64);
+        if (NB == 2) __syncthreads();
+        b3 = n3;
     }
     {
         const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
         l = __uint_as_float(a[0]) + __uint_as_float(a[1]);
     }
     if (x >= A.cols) return;
-    const float fi = 1.0f / fw;  // exact: a power of two
     if (A.chunks > 1) {
         const int cc = 32 * w + c;
         float* part = A.ws + ((int64_t)((seq * A.nkv + h) * A.ncb + cb) * A.chunks + chunk) * (32 * NW) * (HD + 2);
@@ -604,14 +630,14 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
 #pragma unroll
             for (int a = 0; a < 4; a++)
                 *(a8_f4*)(part + cc * HD + 32 * dt + 8 * a + 4 * hf) =
-                    (a8_f4){o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]} * fi;
+                    (a8_f4){o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]};
         if (hf == 0) {
-            part[32 * NW * HD + 2 * cc] = m;
+            part[32 * NW * HD + 2 * cc] = m == -INFINITY ? m : ref;
             part[32 * NW * HD + 2 * cc + 1] = l;
         }
         return;
     }
-    const float inv = l == 0.0f ? 0.0f : fi / l;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     float* dst = A.out + ((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + 4 * hf;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
@@ -663,33 +689,60 @@ __global__ void __launch_bounds__(256) k_attn8_merge(A8 A, int cw) {
     A.out[((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + tid] = L == 0.0f ? 0.0f : y * (1.0f / L);
 }
 
-// The form a call takes: the columns of a workgroup, and the workgroups its tiles are split into where there are
-// fewer. Lengths that only the device knows (ragged) get twice as many: the longest sequence's no longer decide
-// (48 sequences of 1 .. 4096 tokens: 51.3 µs against 58.0).
+// The form a call takes: the columns of a workgroup and, where its column blocks are fewer than `target`, the chunks of at
+// least tiles_min tiles that they are split into.
 struct Form {
-    int cw;
-    int64_t target;
-    int tiles_min;  // tiles a chunk has at least
+    int cw, chunks, tpc;
 };
-Form a8_form(int64_t seqs, int64_t cols, int64_t nkv, int64_t hd, bool ragged) {
-    const int64_t cus = aeth_num_cus(), small = (ragged ? 4 : 2) * cus;
-    if (hd > 128 || cols <= 16) return {16, small, 4};
-    if (cols <= 64) return {32, small, 4};
-    if (hd == 128 && seqs * nkv * aeth_cdiv(cols, 256) >= cus) return {256, cus, 8};
-    return {128, 2 * cus, 8};
+Form a8_split(int cw, int64_t units, int64_t span, int64_t target, int64_t tiles_min) {
+    const int64_t want = std::max<int64_t>(1, std::min(aeth_cdiv(target, units), aeth_cdiv(span, tiles_min)));
+    const int64_t tpc = std::max<int64_t>(4, aeth_cdiv(aeth_cdiv(span, want), 4) * 4);
+    return {cw, (int)std::max<int64_t>(1, aeth_cdiv(span, tpc)), (int)tpc};
+}
+// tiles a block of cw columns sees at most: a window's, or all of max_len
+int64_t a8_span(int64_t cw, int64_t n, int64_t G, int64_t max_len, int64_t window) {
+    const int64_t all = aeth_cdiv(max_len, KV8_TILE), rows = std::min(aeth_cdiv(cw, G) + 1, n);
+    return window > 0 ? std::min(all, (window + rows + 62) / KV8_TILE + 1) : all;
+}
+// (column blocks of cw) x (tiles each sees), over one head
+double a8_blocks_tiles(int64_t cw, int64_t cols, int64_t n, int64_t G, int64_t max_len, int64_t window) {
+    const double blocks = (double)aeth_cdiv(cols, cw), most = (double)a8_span(cw, n, G, max_len, window);
+    if (window > 0) return blocks * most;
+    return blocks * ((double)max_len - 0.5 * (double)n) / KV8_TILE + 0.5 * blocks;
+}
+Form a8_form(int64_t seqs, int64_t n, int64_t G, int64_t nkv, int64_t hd, int64_t max_len, int64_t window, bool ragged) {
+    const int64_t cus = aeth_num_cus(), cols = n * G, heads = seqs * nkv;
+    auto span = [&](int64_t cw) { return a8_span(cw, n, G, max_len, window); };
+    auto units = [&](int64_t cw) { return heads * aeth_cdiv(cols, cw); };
+    // 16 columns: split until two workgroups a CU have work. Lengths that only the device knows get twice as many: the
+    // longest sequence's do not decide (48 sequences of 1 .. 4096 tokens: 51.3 µs against 58.0).
+    const Form small = a8_split(16, units(16), span(16), (ragged ? 4 : 2) * cus, 4);
+    if (hd > 128 || cols <= 64 || ragged) return small;
+    // 128 and 256: not past one workgroup a CU, a split's join costs more than it gains (1000 tokens, 32 / 8 heads: 44 µs,
+    // 83 in two chunks). 256 shares its codes among more columns and has one on each CU: over a long past
+    // (250 queries over 20000 tokens 179 µs, 188 with 128 columns), or where a prompt's triangle fills the chip half as often
+    // again (3500 tokens: 211 against 228; 2500: 141 against 127).
+    Form big = a8_split(128, units(128), span(128), cus, 8);
+    const int64_t u = units(256);
+    if (hd == 128 && (2 * u >= 3 * cus || (2 * u <= cus && u * span(256) >= 16 * cus))) big = a8_split(256, u, span(256), cus, 8);
+    // µs on 256 CUs, 32 / 8 heads of 128, measured and (as reckoned here): 16 columns 18.6 (18.3) for 512 tokens, 41 (40) for 1000,
+    // 75 (76) for 1500, 115 (125) for 2000, 39 (40) for 128 queries over 4096; the wider forms 26 (34), 44 (47), 64 (61),
+    // 89 (84), 36 (36). At head_dim 64 both cost about half.
+    const double per = 256.0 / (double)cus;
+    const double t16 = 10.0 + 1.8e-3 * per * (double)heads * a8_blocks_tiles(16, cols, n, G, max_len, window);
+    const double tbig = 20.0 + std::max(1.7 * (double)std::min<int64_t>(big.tpc, span(big.cw)),
+                                        8e-3 * per * (double)heads * a8_blocks_tiles(128, cols, n, G, max_len, window));
+    return tbig < t16 ? big : small;
 }
 
 template <int HD>
 int a8_launch(const A8& A, const Form& f, int64_t seqs, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)A.nkv * A.ncb * A.chunks), (unsigned)seqs);
-    if constexpr (HD == 256) {
-        hipLaunchKernelGGL((k_attn8<HD, 1>), grid, dim3(256), 0, s, A);
-    } else {
-        if (f.cw == 16) hipLaunchKernelGGL((k_attn8<HD, 1>), grid, dim3(256), 0, s, A);
-        else if (f.cw == 32) hipLaunchKernelGGL((k_attn8<HD, 2>), grid, dim3(256), 0, s, A);
-        else if (f.cw == 128) hipLaunchKernelGGL((k_attn8p<HD, 4>), grid, dim3(256), 0, s, A);
-        else if constexpr (HD == 128) hipLaunchKernelGGL((k_attn8p<HD, 8>), grid, dim3(512), 0, s, A);
-    }
+    if (f.cw == 16) hipLaunchKernelGGL(k_attn8<HD>, grid, dim3(256), 0, s, A);
+    if constexpr (HD <= 128)
+        if (f.cw == 128) hipLaunchKernelGGL((k_attn8p<HD, 4>), grid, dim3(256), 0, s, A);
+    if constexpr (HD == 128)
+        if (f.cw == 256) hipLaunchKernelGGL((k_attn8p<HD, 8>), grid, dim3(512), 0, s, A);
     AETH_LAUNCH_CHECK();
     if (A.chunks > 1) {
         hipLaunchKernelGGL(k_attn8_merge<HD>, dim3((unsigned)((int64_t)A.nkv * A.cols), (unsigned)seqs), dim3(256), 0, s, A, f.cw);
@@ -709,8 +762,9 @@ int64_t aeth_attn_kv8_ws(int64_t seqs, int64_t n, int64_t nq, int64_t nkv, int64
         const int64_t units = seqs * nkv * aeth_cdiv(cols, cw);
         return (target + std::min(units, target)) * cw;
     };
-    int64_t most = hd > 128 || cols <= 16 ? need(16, 4 * cus) : need(32, 4 * cus);
-    if (hd <= 128 && cols > 64) most = std::max(most, need(128, 2 * cus));
+    int64_t most = need(16, 4 * cus);
+    if (hd <= 128 && cols > 64) most = std::max(most, need(128, cus));
+    if (hd == 128 && cols > 64) most = std::max(most, need(256, cus));
     return most * (hd + 2) * (int64_t)sizeof(float);
 }
 
@@ -737,17 +791,10 @@ int aeth_attn_kv8_launch(const float* q, int64_t q_stride, const void* cache, in
     A.ws = (float*)ws;
     A.qvec = ((uintptr_t)q & 15) == 0 && (q_stride & 3) == 0;
     A.ovec = ((uintptr_t)out & 15) == 0;
-    const Form f = a8_form(seqs, A.cols, nkv, hd, lens != nullptr);
+    const Form f = a8_form(seqs, n, A.G, nkv, hd, max_len, A.window, lens != nullptr);
     A.ncb = (int)aeth_cdiv(A.cols, f.cw);
-    // the most tiles a column block sees, and the chunks that fill the chip
-    const int64_t rows = aeth_cdiv(f.cw, A.G) + 1;
-    const int64_t span = A.window ? std::min(aeth_cdiv(max_len, KV8_TILE), (A.window + std::min(rows, n) + 62) / KV8_TILE + 1)
-                                  : aeth_cdiv(max_len, KV8_TILE);
-    const int64_t units = seqs * nkv * A.ncb;
-    const int64_t want = std::max<int64_t>(1, std::min(aeth_cdiv(f.target, units), aeth_cdiv(span, f.tiles_min)));
-    A.tpc = (int)(aeth_cdiv(aeth_cdiv(span, want), 4) * 4);
-    if (A.tpc < 4) A.tpc = 4;
-    A.chunks = (int)std::max<int64_t>(1, aeth_cdiv(span, A.tpc));
+    A.tpc = f.tpc;
+    A.chunks = f.chunks;
     if (hd == 64) return a8_launch<64>(A, f, seqs, s);
     if (hd == 128) return a8_launch<128>(A, f, seqs, s);
     return a8_launch<256>(A, f, seqs, s);

@@ -223,6 +223,10 @@ ATTN = [
     (64, 64, 4, 4, 64, 0), (65, 65, 32, 8, 128, 0), (100, 163, 10, 2, 128, 0), (250, 1250, 8, 2, 128, 0), (129, 129, 3, 1, 256, 0), (200, 333, 7, 1, 64, 90),
     (512, 512, 32, 8, 128, 0), (700, 700, 16, 2, 128, 1), (1000, 1000, 8, 8, 128, 333), (333, 2000, 14, 2, 128, 0), (1999, 1999, 4, 1, 128, 0),
     (150, 900, 6, 1, 128, 65), (257, 700, 9, 3, 64, 0),
+    # every form and its splits: prompts past the small workgroups (hd 64 and 128), a few queries and a chunk over a long past,
+    # a window, a prompt for the largest
+    (1700, 1700, 32, 8, 128, 0), (3100, 3100, 24, 8, 64, 0), (70, 30000, 16, 8, 128, 0), (250, 20001, 32, 8, 128, 0), (330, 12000, 7, 1, 64, 0),
+    (4000, 6000, 32, 8, 128, 555), (3500, 3500, 32, 8, 128, 0), (2000, 2100, 3, 3, 256, 0),
 ]
 
 
