@@ -463,9 +463,10 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
         // an infinity or NaN in q: every score NaN
         qs = mb >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : a8_pow2(-e2) * (1.4426950408889634f / sqrtf((float)HD));
     }
-    // m: the largest score so far, up to 2^TH stale; a probability is 2^(score - ref), ref = m - lf, lf a whole number
-    // that keeps the largest p·sv so far (top) in [2^9, 2^15)
-    float m = -INFINITY, l = 0.0f, top = 0.0f, lf = 0.0f, ref = 0.0f;
+    // m: the largest score so far, up to 2^TH stale. The step's probabilities are formed times 2^lf, as 2^(score - ref) with
+    // ref = m - lf; lf keeps the largest p·sv so far (top, and o, times 2^lf) in [2^9, 2^15). l is of the p themselves.
+    float m = -INFINITY, l = 0.0f, top = 0.0f, ref = 0.0f;
+    int lf = 0;
     a8_f16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) o[dt] = (a8_f16){};
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
             const float mn = fmaxf(m, mx);
             rescale(mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn));
             m = mn;
-            ref = (m == -INFINITY ? 0.0f : m) - lf;
+            ref = (m == -INFINITY ? 0.0f : m) - (float)lf;
         }
     };
     // One step of 32 keys whose scores stand in s: its probabilities beside the products of the next step's scores,
@@ -528,18 +529,21 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
             });
         });
         a8_unroll<EK>([&](auto e) { add(std::integral_constant<int, 16 - EK + e>{}); });
-        l += ps;
+        l = fmaf(ps, a8_pow2(-lf), l);
         const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(wm), __float_as_uint(wm), false, false);
         top = fmaxf(top, fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
         if (__any(top > 0.0f && !(top >= 512.0f && top < 32768.0f))) {  // (uniform)
             if (!(top < INFINITY)) l = __uint_as_float(0x7FC00000u);  // values past 2^119: no number rather than a wrong one
-            const int d = top > 0.0f && top < INFINITY ? a8_exponent(top) - 12 : 0;  // top·2^d in [2^10, 2^11)
+            // top·2^d in [2^10, 2^11), as far as p·2^lf keeps clear of overflow (p·sv above 2^-90)
+            const int d = top > 0.0f && top < INFINITY ? min(max(a8_exponent(top) - 12 + lf, -120), 100) - lf : 0;
             const float al = a8_pow2(min(max(d, -126), 126));
-            rescale(al);
+            top *= al;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) o[dt] *= al;
 #pragma unroll
             for (int i = 0; i < 16; i++) s[i] *= al;
-            lf += (float)d;
-            ref = (m == -INFINITY ? 0.0f : m) - lf;
+            lf += min(max(d, -126), 126);
+            ref = (m == -INFINITY ? 0.0f : m) - (float)lf;
         }
         between();
         const char* vp = vb[b3] + 2 * T * 1024 + lane * 16;
@@ -622,6 +626,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
         l = __uint_as_float(a[0]) + __uint_as_float(a[1]);
     }
     if (x >= A.cols) return;
+    const float un = a8_pow2(-lf);
     if (A.chunks > 1) {
         const int cc = 32 * w + c;
         float* part = A.ws + ((int64_t)((seq * A.nkv + h) * A.ncb + cb) * A.chunks + chunk) * (32 * NW) * (HD + 2);
@@ -630,9 +635,9 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
 #pragma unroll
             for (int a = 0; a < 4; a++)
                 *(a8_f4*)(part + cc * HD + 32 * dt + 8 * a + 4 * hf) =
-                    (a8_f4){o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]};
+                    (a8_f4){o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]} * un;
         if (hf == 0) {
-            part[32 * NW * HD + 2 * cc] = m == -INFINITY ? m : ref;
+            part[32 * NW * HD + 2 * cc] = m;
             part[32 * NW * HD + 2 * cc + 1] = l;
         }
         return;
@@ -643,7 +648,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
         for (int a = 0; a < 4; a++) {
-            const a8_f4 y = (a8_f4){o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]} * inv;
+            const a8_f4 y = (a8_f4){o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]} * inv * un;
             float* d = dst + 32 * dt + 8 * a;
             if (A.ovec) *(a8_f4*)d = y;
             else d[0] = y[0], d[1] = y[1], d[2] = y[2], d[3] = y[3];

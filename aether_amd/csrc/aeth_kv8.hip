@@ -80,29 +80,23 @@ struct AppendArgs {
     int vec;              // rows are 16-byte aligned
 };
 
-// Workgroup = (tile, KV head, sequence): 16 lanes a token, four rounds of 16 tokens. K codes go out from
+// Workgroup = (tile, KV head): 16 lanes a token, four rounds of 16 tokens. K codes go out from
 // registers; V codes are transposed through LDS and go out 16 bytes at a time where the tile's tokens
 // are all new, in words or bytes where some are not (those are left as they were).
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_append(AppendArgs A) {
     constexpr int V4 = HD / 64, LW = HD / 4 + 4;  // float4s a lane and token; words of an LDS row
     __shared__ uint32_t vs[KV8_TILE * LW];
-    const int h = blockIdx.x % A.nkv, seq = blockIdx.y, tid = threadIdx.x, l16 = tid & 15, grp = tid >> 4;
-    int64_t slot = A.slot, n = A.n, row0 = 0;
-    if (A.slots) {
-        slot = A.slots[seq];
-        n = 1;
-        row0 = seq;
-        if (slot < 0 || slot >= A.max_seq) return;  // (uniform) a full cache takes nothing
-    }
+    const int h = blockIdx.x % A.nkv, tid = threadIdx.x, l16 = tid & 15, grp = tid >> 4;
+    const int64_t slot = A.slot, n = A.n;
     const int64_t tile = (slot >> 6) + blockIdx.x / A.nkv;
     const int64_t first = tile * KV8_TILE - slot;  // the token at the tile's slot 0 (below 0: an older one)
-    uint8_t* base = A.cache + seq * A.seq_bytes + ((int64_t)h * A.tiles + tile) * aeth_kv8_tile_bytes(HD);
+    uint8_t* base = A.cache + ((int64_t)h * A.tiles + tile) * aeth_kv8_tile_bytes(HD);
     float4 x[4][2][V4];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         const int64_t i = min(max(first + 16 * r + grp, (int64_t)0), n - 1);  // clamped: loaded, not stored
-        const int64_t off = (row0 + i) * A.token_stride + h * A.head_stride + 4 * l16;
+        const int64_t off = i * A.token_stride + h * A.head_stride + 4 * l16;
 #pragma unroll
         for (int u = 0; u < V4; u++) {
             x[r][0][u] = kv8_ld4(A.k + off + 64 * u, A.vec);
@@ -167,6 +161,45 @@ __global__ void __launch_bounds__(256) k_kv8_append(AppendArgs A) {
             }
         }
     }
+}
+
+// A token's K (v = 0) or V (1) of one head into slot `slot` of its head's tiles: HD / 8 lanes, each dimensions e .. e + 3 (a)
+// and HD / 2 further on (b). Every lane of the wave has to call it.
+template <int HD>
+__device__ __forceinline__ void kv8_put(uint8_t* tiles, int64_t slot, int v, int e, float4 a, float4 b, bool store) {
+    const uint32_t m = kv8_umax<HD / 8>(kv8_abs_max(kv8_abs_max(0, a), b));
+    if (!store) return;
+    const bool finite = m < 0x7F800000u;
+    const float amax = __uint_as_float(m);
+    const double inv = finite && m > 0 ? kv8_inverse(amax) : 0.0;
+    const uint32_t wa = kv8_code4(a, inv, finite), wb = kv8_code4(b, inv, finite);
+    const int t = (int)(slot & 63);
+    uint8_t* base = tiles + (slot >> 6) * aeth_kv8_tile_bytes(HD);
+    if (v) {
+        uint8_t* dst = base + KV8_TILE * HD + e * KV8_TILE + aeth_kv8_vbyte(t);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            dst[i * KV8_TILE] = (uint8_t)(wa >> (8 * i));
+            dst[(HD / 2 + i) * KV8_TILE] = (uint8_t)(wb >> (8 * i));
+        }
+    } else {
+        *(uint32_t*)(base + t * HD + e) = wa;
+        *(uint32_t*)(base + t * HD + HD / 2 + e) = wb;
+    }
+    if (e == 0) *(float*)(base + 2 * KV8_TILE * HD + 4 * (KV8_TILE * v + t)) = finite ? amax / 127.0f : __uint_as_float(0x7FC00000u);
+}
+
+// Without a tile's staging, for a few tokens or one for each of many sequences: HD / 8 lanes a token, head and K or V; V's codes go out as bytes
+template <int HD>
+__global__ void __launch_bounds__(256) k_kv8_append_few(AppendArgs A, int rows) {
+    constexpr int L = HD / 8;
+    const int unit = (blockIdx.x * 256 + threadIdx.x) / L, all = 2 * rows * A.nkv, u = min(unit, all - 1), e = 4 * (threadIdx.x % L);
+    const int v = u & 1, h = (u >> 1) % A.nkv, row = (u >> 1) / A.nkv;
+    const float* src = (v ? A.v : A.k) + row * A.token_stride + h * A.head_stride + e;
+    const float4 a = kv8_ld4(src, A.vec), b = kv8_ld4(src + HD / 2, A.vec);
+    const int64_t slot = A.slots ? (int64_t)A.slots[row] : A.slot + row;
+    uint8_t* tiles = A.cache + (A.slots ? row : 0) * A.seq_bytes + (int64_t)h * A.tiles * aeth_kv8_tile_bytes(HD);
+    kv8_put<HD>(tiles, slot, v, e, a, b, unit < all && slot >= 0 && slot < A.max_seq);  // a full cache takes nothing
 }
 
 struct ReadArgs {
@@ -245,6 +278,10 @@ bool aligned16(const void* a, const void* b, int64_t ts, int64_t hs) {
 
 }  // namespace
 
+// Tokens whose rows go a 16th of a wave each rather than by tiles: while rows times heads leave the chip half idle. 8 heads of
+// 128: 1 token 2.4 µs against 4.3, 256 tokens 3.9 and 5.1, 512 tokens 5.5 and 5.2, 1000 tokens 8.8 and 5.2.
+static bool append_few(int64_t rows, int64_t nkv) { return rows < 14 * (int64_t)aeth_num_cus() / nkv; }
+
 int aeth_kv8_append_launch(void* cache, int64_t seq_bytes, const int* d_slots, int64_t seqs, const float* k, const float* v,
                            int64_t token_stride, int64_t head_stride, int64_t n, int64_t nkv, int64_t hd, int64_t max_seq,
                            int64_t slot, hipStream_t s) {
@@ -263,8 +300,17 @@ int aeth_kv8_append_launch(void* cache, int64_t seq_bytes, const int* d_slots, i
     A.nkv = (int)nkv;
     A.tiles = (int)aeth_cdiv(max_seq, KV8_TILE);
     A.vec = aligned16(k, v, token_stride, head_stride);
-    const int64_t touched = d_slots ? 1 : ((slot + n - 1) >> 6) - (slot >> 6) + 1;
-    const dim3 grid((unsigned)(touched * nkv), (unsigned)seqs), block(256);
+    const dim3 block(256);
+    const int64_t rows = d_slots ? seqs : n;
+    if (d_slots || append_few(n, nkv)) {
+        const dim3 grid((unsigned)aeth_cdiv(2 * rows * nkv * (hd / 8), 256));
+        if (hd == 64) hipLaunchKernelGGL(k_kv8_append_few<64>, grid, block, 0, s, A, (int)rows);
+        else if (hd == 128) hipLaunchKernelGGL(k_kv8_append_few<128>, grid, block, 0, s, A, (int)rows);
+        else hipLaunchKernelGGL(k_kv8_append_few<256>, grid, block, 0, s, A, (int)rows);
+        AETH_LAUNCH_CHECK();
+        return AETH_OK;
+    }
+    const dim3 grid((unsigned)((((slot + n - 1) >> 6) - (slot >> 6) + 1) * nkv));
     if (hd == 64) hipLaunchKernelGGL(k_kv8_append<64>, grid, block, 0, s, A);
     else if (hd == 128) hipLaunchKernelGGL(k_kv8_append<128>, grid, block, 0, s, A);
     else hipLaunchKernelGGL(k_kv8_append<256>, grid, block, 0, s, A);
@@ -437,32 +483,13 @@ __global__ void __launch_bounds__(256) k_kv8_step(float* qkv, int nq, int nkv, c
         a = make_float4(qk_rot0(x.x, y.x, sn.x, cs.x), qk_rot0(x.y, y.y, sn.y, cs.y), qk_rot0(x.z, y.z, sn.z, cs.z), qk_rot0(x.w, y.w, sn.w, cs.w));
         b = make_float4(qk_rot1(x.x, y.x, sn.x, cs.x), qk_rot1(x.y, y.y, sn.y, cs.y), qk_rot1(x.z, y.z, sn.z, cs.z), qk_rot1(x.w, y.w, sn.w, cs.w));
     }
-    const uint32_t m = kv8_umax<L>(kv8_abs_max(kv8_abs_max(0, a), b));
-    if (unit >= nq + 2 * nkv) return;
-    if (h < nq) {
+    if (unit < nq) {
         *(float4*)src = a;
         *(float4*)(src + HALF) = b;
-        return;
     }
-    if (slot < 0 || slot >= max_seq) return;
-    const bool finite = m < 0x7F800000u;
-    const float amax = __uint_as_float(m);
-    const double inv = finite && m > 0 ? kv8_inverse(amax) : 0.0;
-    const uint32_t wa = kv8_code4(a, inv, finite), wb = kv8_code4(b, inv, finite);
-    const int v = h >= nq + nkv, t = (int)(slot & 63);
-    uint8_t* base = cache + ((int64_t)(h - nq - v * nkv) * tiles + (slot >> 6)) * aeth_kv8_tile_bytes(HD);
-    if (v) {
-        uint8_t* dst = base + KV8_TILE * HD + e * KV8_TILE + aeth_kv8_vbyte(t);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            dst[i * KV8_TILE] = (uint8_t)(wa >> (8 * i));
-            dst[(HALF + i) * KV8_TILE] = (uint8_t)(wb >> (8 * i));
-        }
-    } else {
-        *(uint32_t*)(base + t * HD + e) = wa;
-        *(uint32_t*)(base + t * HD + HALF + e) = wb;
-    }
-    if (e == 0) *(float*)(base + 2 * KV8_TILE * HD + 4 * (KV8_TILE * v + t)) = finite ? amax / 127.0f : __uint_as_float(0x7FC00000u);
+    const int v = h >= nq + nkv;
+    kv8_put<HD>(cache + (int64_t)max(h - nq - v * nkv, 0) * tiles * aeth_kv8_tile_bytes(HD), slot, v, e, a, b,
+                h >= nq && unit < nq + 2 * nkv && slot >= 0 && slot < max_seq);
 }
 
 // any even hd, any alignment: a wave a head, lanes over the pairs (read again for the rotation: the row is in cache)

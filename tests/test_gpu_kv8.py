@@ -313,16 +313,17 @@ def test_queries_that_are_no_numbers(gpu):
         within(torch, got[i], want[i], bound[i])
 
 
-@pytest.mark.parametrize("n", [1, 120])
-def test_attention_over_uneven_rows(gpu, n):
+@pytest.mark.parametrize("n,seq", [(1, 1000), (120, 1000), (1000, 3000)])
+def test_attention_over_uneven_rows(gpu, n, seq):
     """What the maximum, the digits and the tiles' exponents have to stand: one key far above the rest, with a value
     of no size; scores that rise from tile to tile by hundreds; a flat row; V scales from 1e-20 to 1e20."""
     torch = gpu
-    nkv, hd, heads, seq = 1, 128, 2, 1000
-    base = rand(torch, 40, nkv, seq + 24, hd)
-    val = rand(torch, 41, nkv, seq + 24, hd)
+    nkv, hd, heads = 1, 128, 16 if n == 1000 else 2
+    slots = -(-seq // 64) * 64
+    base = rand(torch, 40, nkv, slots, hd)
+    val = rand(torch, 41, nkv, slots, hd)
     q = rand(torch, 42, n, heads * hd)
-    t = torch.arange(seq + 24, device="cuda").float()[None, :, None]
+    t = torch.arange(slots, device="cuda").float()[None, :, None]
     cases = []
     k, v = base.clone(), val.clone()
     k[:, 3] = 12.0 * q[0, :hd] / q[0, :hd].norm()
@@ -333,12 +334,14 @@ def test_attention_over_uneven_rows(gpu, n):
     cases.append((base * 0.0, val))
     cases.append((base * 1e-3, val * torch.pow(10.0, (t % 41) - 20.0)))
     cases.append((base, val * torch.pow(10.0, -t / 50.0)))
+    cases.append((base, val * 1e-24))
+    cases.append((base, val * 1e33))
     for k, v in cases:
         kc, ks = R.codes(k)
         vc, vs = R.codes(v)
         layer = R.pack(kc, ks, vc, vs)
-        got = attend(torch, q, layer, nkv, hd, seq + 24, seq)
-        want, bound = R.attention(q, layer, nkv, hd, seq + 24, seq, 0)
+        got = attend(torch, q, layer, nkv, hd, slots, seq)
+        want, bound = R.attention(q, layer, nkv, hd, slots, seq, 0)
         within(torch, got, want, bound)
 
 
