@@ -46,6 +46,10 @@ struct A8 {
     float* out;             // [seqs][n][nq·hd]
     float* ws;              // partials when chunks > 1
     int qvec, ovec;         // q rows / out 16-byte aligned
+    // a decode step (k_attn8<HD, true>): q is q | k | v unrotated, lens the cache fill, len_add 1
+    const int* pos;         // device position of the token
+    const float *sin_t, *cos_t;
+    int64_t max_seq;
 };
 
 // f(0) .. f(N - 1), each with its number as a constant
@@ -110,12 +114,16 @@ __device__ __forceinline__ void a8_tiles(const A8& A, int len, int c0, int count
 // each with its own running softmax, and merge through LDS.
 // A token's scales belong to one register of every lane (lane group g holds tokens 16j + 4g + r in registers
 // 4j + r): lane i of a row of 16 holds the one of register i's token, and the multiplication takes it from there.
-template <int HD>
-__global__ void __launch_bounds__(256) k_attn8(A8 A) {
+// STEP (HD = 128, one column block): a decode step's token with it. Each workgroup rotates q; the wave that takes the token's
+// tile also rotates k, quantises k and v, stores them and puts the codes into the fragments it loaded.
+template <int HD, bool STEP>
+__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
+    static_assert(!STEP || HD == 128, "a lane holds both halves of a rotated pair");
     constexpr int KS = HD / 64, DT = HD / 16, PLD = HD + 4;
     constexpr float TH = 8.0f;
     __shared__ __attribute__((aligned(16))) float po[4][16][PLD];
     __shared__ float pm[4][16], pl[4][16];
+    __shared__ __attribute__((aligned(16))) uint32_t fresh[2][HD / 4];  // STEP: the token's codes of K and V
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = blockIdx.x;
@@ -169,9 +177,54 @@ __global__ void __launch_bounds__(256) k_attn8(A8 A) {
                 qv[s][e + 3] = y.w;
             }
     }
+    // STEP: the table's row; k and v of the token, a row of 16 lanes each, if this wave takes their tile
+    const int slot = STEP ? A.lens[0] : -1, fresh_t = slot >> 6;
+    const bool mine = STEP && slot >= 0 && slot < len && fresh_t >= t0 && fresh_t < t1 && ((fresh_t - t0) & 3) == w;  // (uniform)
+    float sn[STEP ? 16 : 1], cs[STEP ? 16 : 1];
+    float4 xa, xb, xs, xc4;
+    const float *sin_r = nullptr, *cos_r = nullptr;
+    if constexpr (STEP) {
+        const int64_t p = min(max((int64_t)A.pos[0], (int64_t)0), A.max_seq - 1);
+        sin_r = A.sin_t + p * (HD / 2);
+        cos_r = A.cos_t + p * (HD / 2);
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            *(float4*)&sn[e] = *(const float4*)(sin_r + 16 * g + e);
+            *(float4*)&cs[e] = *(const float4*)(cos_r + 16 * g + e);
+        }
+        if (mine) {
+            const float* src = A.q + (int64_t)(A.nq + (lane >> 4 & 1) * A.nkv + h) * HD + 4 * c;
+            xa = *(const float4*)src;
+            xb = *(const float4*)(src + HD / 2);
+            xs = *(const float4*)(sin_r + 4 * c);
+            xc4 = *(const float4*)(cos_r + 4 * c);
+        }
+    }
     __builtin_amdgcn_sched_barrier(0);
     if (t0 + w < t1) load(t0 + w);
     __builtin_amdgcn_sched_barrier(0);
+    float fresh_s = 0.0f;  // the scale of K (lanes of rows 0 and 2) or V (1 and 3)
+    if constexpr (STEP) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const float a = qv[0][e], b = qv[KS - 1][e];
+            qv[0][e] = kv8_rot0(a, b, sn[e], cs[e]);
+            qv[KS - 1][e] = kv8_rot1(a, b, sn[e], cs[e]);
+        }
+        if (mine) {
+            const int v = lane >> 4 & 1;
+            float4 ra = xa, rb = xb;
+            kv8_rotate(ra, rb, xs, xc4);
+            if (v) ra = xa, rb = xb;
+            const Kv8Row q = kv8_quantise<HD>(ra, rb);
+            fresh_s = q.scale;
+            if (lane < 32) {
+                fresh[v][c] = q.a;
+                fresh[v][c + 16] = q.b;
+                kv8_put<HD>((uint8_t*)head, slot, v, 4 * c, q);
+            }
+        }
+    }
     a8_i4 qd[3][KS];  // q's digits
     float qs;
     {
@@ -212,6 +265,33 @@ __global__ void __launch_bounds__(256) k_attn8(A8 A) {
 
     const a8_i4 zero = {0, 0, 0, 0};
     for (int t = t0 + w; t < t1; t += 4) {
+        if (STEP && mine && t == fresh_t) {  // (uniform) the token's codes and scales in place of what was loaded from its slot
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's stores of them
+            const int j = slot >> 4 & 3, r8 = 8 * (slot & 3);
+            a8_i4 row[KS];
+#pragma unroll
+            for (int s = 0; s < KS; s++) row[s] = *(const a8_i4*)&fresh[0][16 * s + 4 * g];
+            uint32_t byte[DT];
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) byte[dt] = fresh[1][4 * dt + (c >> 2)] >> (8 * (c & 3)) & 0xFFu;
+            const bool k_here = c == (slot & 15), v_here = g == (slot >> 2 & 3);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (i != j) continue;  // (uniform)
+#pragma unroll
+                for (int s = 0; s < KS; s++) kf[i][s] = k_here ? row[s] : kf[i][s];
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+                    const uint32_t x = ((uint32_t)vf[dt][i] & ~(0xFFu << r8)) | byte[dt] << r8;
+                    vf[dt][i] = v_here ? (int)x : vf[dt][i];
+                }
+            }
+            const float fk = __shfl(fresh_s, 0, 64), fv = __shfl(fresh_s, 16, 64);
+            if ((slot & 63) == 16 * ((lane >> 2) & 3) + 4 * g + (lane & 3)) {
+                sk = fk;
+                sv = fv;
+            }
+        }
         {   // a V scale that is no number goes to the token's K scale: its scores are NaN where it is seen
             const bool fine = fabsf(sv) < INFINITY;
             sk = fine ? sk : __uint_as_float(0x7FC00000u);
@@ -743,7 +823,7 @@ Form a8_form(int64_t seqs, int64_t n, int64_t G, int64_t nkv, int64_t hd, int64_
 template <int HD>
 int a8_launch(const A8& A, const Form& f, int64_t seqs, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)A.nkv * A.ncb * A.chunks), (unsigned)seqs);
-    if (f.cw == 16) hipLaunchKernelGGL(k_attn8<HD>, grid, dim3(256), 0, s, A);
+    if (f.cw == 16) hipLaunchKernelGGL((k_attn8<HD, false>), grid, dim3(256), 0, s, A);
     if constexpr (HD <= 128)
         if (f.cw == 128) hipLaunchKernelGGL((k_attn8p<HD, 4>), grid, dim3(256), 0, s, A);
     if constexpr (HD == 128)
@@ -777,7 +857,7 @@ int aeth_attn_kv8_launch(const float* q, int64_t q_stride, const void* cache, in
                          int64_t seqs, int64_t n, int64_t nq, int64_t nkv, int64_t hd, int64_t max_seq, int64_t max_len,
                          int64_t window, float* out, void* ws, hipStream_t s) {
     if (n <= 0 || seqs <= 0) return AETH_OK;
-    A8 A;
+    A8 A = {};
     A.q = q;
     A.q_stride = q_stride;
     A.cache = (const uint8_t*)cache;
@@ -803,6 +883,44 @@ int aeth_attn_kv8_launch(const float* q, int64_t q_stride, const void* cache, in
     if (hd == 64) return a8_launch<64>(A, f, seqs, s);
     if (hd == 128) return a8_launch<128>(A, f, seqs, s);
     return a8_launch<256>(A, f, seqs, s);
+}
+
+int aeth_attn_kv8_step_launch(const float* qkv, int64_t nq, int64_t nkv, int64_t hd, const int* st, const float* sin_t,
+                              const float* cos_t, int64_t max_seq, int64_t window, void* cache, float* out, void* ws, hipStream_t s) {
+    const int64_t G = nq / nkv;
+    if (hd != 128 || G > 16 || (((uintptr_t)qkv | (uintptr_t)out | (uintptr_t)sin_t | (uintptr_t)cos_t) & 15))
+        return aeth_set_error(AETH_EUNSUPPORTED, "8-bit cache step: %lld heads of %lld a KV head", (long long)G, (long long)hd);
+    A8 A = {};
+    A.q = qkv;
+    A.q_stride = nq * hd;
+    A.cache = (const uint8_t*)cache;
+    A.lens = st + 2;
+    A.len_add = 1;
+    A.max_len = (int)max_seq;
+    A.n = 1;
+    A.nq = (int)nq;
+    A.nkv = (int)nkv;
+    A.G = A.cols = (int)G;
+    A.tiles = (int)aeth_cdiv(max_seq, KV8_TILE);
+    A.window = window > 0 && window < max_seq ? (int)window : 0;
+    A.out = out;
+    A.ws = (float*)ws;
+    A.qvec = A.ovec = 1;
+    A.pos = st + 1;
+    A.sin_t = sin_t;
+    A.cos_t = cos_t;
+    A.max_seq = max_seq;
+    const Form f = a8_form(1, 1, G, nkv, hd, max_seq, A.window, true);
+    A.ncb = 1;
+    A.tpc = f.tpc;
+    A.chunks = f.chunks;
+    hipLaunchKernelGGL((k_attn8<128, true>), dim3((unsigned)(nkv * A.chunks)), dim3(256), 0, s, A);
+    AETH_LAUNCH_CHECK();
+    if (A.chunks > 1) {
+        hipLaunchKernelGGL(k_attn8_merge<128>, dim3((unsigned)nq), dim3(256), 0, s, A, 16);
+        AETH_LAUNCH_CHECK();
+    }
+    return AETH_OK;
 }
 
 // what the two entry points ask of their arguments in common

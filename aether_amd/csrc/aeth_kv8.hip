@@ -19,41 +19,6 @@ typedef float kv8_f4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
-template <int L>
-__device__ __forceinline__ uint32_t kv8_umax(uint32_t v) {  // max over aligned groups of L lanes (8, 16 or 32)
-    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));
-    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));
-    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));
-    if (L >= 16) v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));
-    if (L >= 32) {
-        const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-        v = max(a[0], a[1]);
-    }
-    return v;
-}
-
-__device__ __forceinline__ uint32_t kv8_abs_max(uint32_t m, float4 y) {  // as integers: a NaN's bits are above an infinity's
-    m = max(max(m, __float_as_uint(y.x) & 0x7FFFFFFFu), __float_as_uint(y.y) & 0x7FFFFFFFu);
-    return max(max(m, __float_as_uint(y.z) & 0x7FFFFFFFu), __float_as_uint(y.w) & 0x7FFFFFFFu);
-}
-
-// 127 / amax in f64 to 2^-50 relative (amax > 0), by two Newton steps on the reciprocal instruction
-__device__ __forceinline__ double kv8_inverse(float amax) {
-    const double a = (double)amax;
-    double r = __builtin_amdgcn_rcp(a);
-    r = fma(fma(-a, r, 1.0), r, r);
-    r = fma(fma(-a, r, 1.0), r, r);
-    return 127.0 * r;
-}
-
-// rint(127·x / amax): the quotient of two f32 is a tie or at least 2^-26 away from one, so the f64
-// product (off by under 2^-42) rounded to a multiple of 2^-40 is a tie exactly where the quotient is.
-__device__ __forceinline__ uint32_t kv8_code(float x, double inv) {
-    const double t = (double)x * inv;
-    const double u = (t + 6144.0) - 6144.0;
-    return (uint32_t)__double2loint(u + 6755399441055744.0) & 0xFFu;  // 1.5·2^52
-}
-
 // Rows read or written once, past the caches: 30000 tokens of 8 heads of 128 appended in 55 µs (72 with plain
 // loads), read back in 48 (90 with plain stores, which displace the codes that a workgroup reads in pieces).
 __device__ __forceinline__ float4 kv8_ld4(const float* p, bool vec) {
@@ -62,11 +27,6 @@ __device__ __forceinline__ float4 kv8_ld4(const float* p, bool vec) {
         return make_float4(v.x, v.y, v.z, v.w);
     }
     return make_float4(p[0], p[1], p[2], p[3]);
-}
-
-__device__ __forceinline__ uint32_t kv8_code4(float4 y, double inv, bool finite) {
-    const uint32_t w = kv8_code(y.x, inv) | kv8_code(y.y, inv) << 8 | kv8_code(y.z, inv) << 16 | kv8_code(y.w, inv) << 24;
-    return finite ? w : 0;
 }
 
 struct AppendArgs {
@@ -163,32 +123,6 @@ __global__ void __launch_bounds__(256) k_kv8_append(AppendArgs A) {
     }
 }
 
-// A token's K (v = 0) or V (1) of one head into slot `slot` of its head's tiles: HD / 8 lanes, each dimensions e .. e + 3 (a)
-// and HD / 2 further on (b). Every lane of the wave has to call it.
-template <int HD>
-__device__ __forceinline__ void kv8_put(uint8_t* tiles, int64_t slot, int v, int e, float4 a, float4 b, bool store) {
-    const uint32_t m = kv8_umax<HD / 8>(kv8_abs_max(kv8_abs_max(0, a), b));
-    if (!store) return;
-    const bool finite = m < 0x7F800000u;
-    const float amax = __uint_as_float(m);
-    const double inv = finite && m > 0 ? kv8_inverse(amax) : 0.0;
-    const uint32_t wa = kv8_code4(a, inv, finite), wb = kv8_code4(b, inv, finite);
-    const int t = (int)(slot & 63);
-    uint8_t* base = tiles + (slot >> 6) * aeth_kv8_tile_bytes(HD);
-    if (v) {
-        uint8_t* dst = base + KV8_TILE * HD + e * KV8_TILE + aeth_kv8_vbyte(t);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            dst[i * KV8_TILE] = (uint8_t)(wa >> (8 * i));
-            dst[(HD / 2 + i) * KV8_TILE] = (uint8_t)(wb >> (8 * i));
-        }
-    } else {
-        *(uint32_t*)(base + t * HD + e) = wa;
-        *(uint32_t*)(base + t * HD + HD / 2 + e) = wb;
-    }
-    if (e == 0) *(float*)(base + 2 * KV8_TILE * HD + 4 * (KV8_TILE * v + t)) = finite ? amax / 127.0f : __uint_as_float(0x7FC00000u);
-}
-
 // Without a tile's staging, for a few tokens or one for each of many sequences: HD / 8 lanes a token, head and K or V; V's codes go out as bytes
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_append_few(AppendArgs A, int rows) {
@@ -199,7 +133,8 @@ __global__ void __launch_bounds__(256) k_kv8_append_few(AppendArgs A, int rows) 
     const float4 a = kv8_ld4(src, A.vec), b = kv8_ld4(src + HD / 2, A.vec);
     const int64_t slot = A.slots ? (int64_t)A.slots[row] : A.slot + row;
     uint8_t* tiles = A.cache + (A.slots ? row : 0) * A.seq_bytes + (int64_t)h * A.tiles * aeth_kv8_tile_bytes(HD);
-    kv8_put<HD>(tiles, slot, v, e, a, b, unit < all && slot >= 0 && slot < A.max_seq);  // a full cache takes nothing
+    const Kv8Row q = kv8_quantise<HD>(a, b);
+    if (unit < all && slot >= 0 && slot < A.max_seq) kv8_put<HD>(tiles, slot, v, e, q);  // a full cache takes nothing
 }
 
 struct ReadArgs {
@@ -421,10 +356,6 @@ __device__ __forceinline__ int64_t qk_row(const QkArgs& A, int64_t i) {
     return min(max(p, (int64_t)0), A.max_seq - 1);
 }
 
-// the rotated pair, rounded as k_rope's is: a head without a norm gets aeth_rope's bits
-__device__ __forceinline__ float qk_rot0(float a, float b, float sn, float cs) { return fmaf(a, cs, -(b * sn)); }
-__device__ __forceinline__ float qk_rot1(float a, float b, float sn, float cs) { return fmaf(a, sn, b * cs); }
-
 // sum over aligned groups of L lanes (8, 16 or 32), the same value in each
 template <int L>
 __device__ __forceinline__ float qk_sum(float v) {
@@ -461,35 +392,10 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_v(QkArgs A) {
     }
     if (unit >= all) return;
     float* dst = A.out + i * A.out_stride + (int64_t)h * HD + e;
+    kv8_rotate(a, b, sn, cs);
     // streaming stores: 4000 rows of 32 + 8 heads of 128 in 25.1 µs (6.6 TB/s) against 27.4
-    __builtin_nontemporal_store((kv8_f4){qk_rot0(a.x, b.x, sn.x, cs.x), qk_rot0(a.y, b.y, sn.y, cs.y), qk_rot0(a.z, b.z, sn.z, cs.z),
-                                         qk_rot0(a.w, b.w, sn.w, cs.w)}, (kv8_f4*)dst);
-    __builtin_nontemporal_store((kv8_f4){qk_rot1(a.x, b.x, sn.x, cs.x), qk_rot1(a.y, b.y, sn.y, cs.y), qk_rot1(a.z, b.z, sn.z, cs.z),
-                                         qk_rot1(a.w, b.w, sn.w, cs.w)}, (kv8_f4*)(dst + HALF));
-}
-
-// One token at device position and slot: hd / 8 lanes a head of q | k | v
-template <int HD>
-__global__ void __launch_bounds__(256) k_kv8_step(float* qkv, int nq, int nkv, const int* st, const float* sin_t, const float* cos_t,
-                                                  int64_t max_seq, int tiles, uint8_t* cache) {
-    constexpr int L = HD / 8, HALF = HD / 2;
-    const int unit = (blockIdx.x * 256 + threadIdx.x) / L, h = min(unit, nq + 2 * nkv - 1), e = 4 * (threadIdx.x % L);
-    float* src = qkv + (int64_t)h * HD + e;
-    float4 a = *(const float4*)src, b = *(const float4*)(src + HALF);
-    const int64_t p = min(max((int64_t)st[1], (int64_t)0), max_seq - 1), slot = st[2];
-    const float4 sn = *(const float4*)(sin_t + p * HALF + e), cs = *(const float4*)(cos_t + p * HALF + e);
-    if (h < nq + nkv) {
-        const float4 x = a, y = b;
-        a = make_float4(qk_rot0(x.x, y.x, sn.x, cs.x), qk_rot0(x.y, y.y, sn.y, cs.y), qk_rot0(x.z, y.z, sn.z, cs.z), qk_rot0(x.w, y.w, sn.w, cs.w));
-        b = make_float4(qk_rot1(x.x, y.x, sn.x, cs.x), qk_rot1(x.y, y.y, sn.y, cs.y), qk_rot1(x.z, y.z, sn.z, cs.z), qk_rot1(x.w, y.w, sn.w, cs.w));
-    }
-    if (unit < nq) {
-        *(float4*)src = a;
-        *(float4*)(src + HALF) = b;
-    }
-    const int v = h >= nq + nkv;
-    kv8_put<HD>(cache + (int64_t)max(h - nq - v * nkv, 0) * tiles * aeth_kv8_tile_bytes(HD), slot, v, e, a, b,
-                h >= nq && unit < nq + 2 * nkv && slot >= 0 && slot < max_seq);
+    __builtin_nontemporal_store((kv8_f4){a.x, a.y, a.z, a.w}, (kv8_f4*)dst);
+    __builtin_nontemporal_store((kv8_f4){b.x, b.y, b.z, b.w}, (kv8_f4*)(dst + HALF));
 }
 
 // any even hd, any alignment: a wave a head, lanes over the pairs (read again for the rotation: the row is in cache)
@@ -515,8 +421,8 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(QkArgs A) {
             a = a / rms * w[e];
             b = b / rms * w[e + half];
         }
-        dst[e] = qk_rot0(a, b, sn, cs);
-        dst[e + half] = qk_rot1(a, b, sn, cs);
+        dst[e] = kv8_rot0(a, b, sn, cs);
+        dst[e + half] = kv8_rot1(a, b, sn, cs);
     }
 }
 }  // namespace
@@ -537,16 +443,6 @@ int aeth_qk_norm_rope_launch(const float* x, int64_t x_stride, int64_t n, int64_
     } else {
         hipLaunchKernelGGL(k_qk_norm_rope, dim3((unsigned)aeth_cdiv(n * heads, 4)), dim3(256), 0, s, A);
     }
-    AETH_LAUNCH_CHECK();
-    return AETH_OK;
-}
-
-int aeth_kv8_step_launch(float* qkv, int64_t nq, int64_t nkv, int64_t hd, const int* st, const float* sin_t, const float* cos_t,
-                         int64_t max_seq, void* cache, hipStream_t s) {
-    const dim3 grid((unsigned)aeth_cdiv((nq + 2 * nkv) * (hd / 8), 256)), block(256);
-    const int tiles = (int)aeth_cdiv(max_seq, KV8_TILE);
-    if (hd != 128) return aeth_set_error(AETH_EUNSUPPORTED, "8-bit cache step: head_dim %lld (needs 128)", (long long)hd);
-    hipLaunchKernelGGL(k_kv8_step<128>, grid, block, 0, s, qkv, (int)nq, (int)nkv, st, sin_t, cos_t, max_seq, tiles, (uint8_t*)cache);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }

@@ -54,7 +54,8 @@ int aeth_attn_kv8_launch(const float* q, int64_t q_stride, const void* cache, in
 int aeth_qk_norm_rope_launch(const float* x, int64_t x_stride, int64_t n, int64_t n_heads, int64_t kv_heads, int64_t hd,
                              const float* qw, const float* kw, float eps, int64_t pos, const int* d_pos, const float* sin_t,
                              const float* cos_t, int64_t max_seq, float* out, int64_t out_stride, hipStream_t s);
-// A decode step's token: the q and k heads of qkv = q | k | v rotated at position st[1] (q in place), k and v into the
-// cache at slot st[2] (nowhere if it is full). The bits of the two calls above; rows and tables 16-byte aligned.
-int aeth_kv8_step_launch(float* qkv, int64_t nq, int64_t nkv, int64_t hd, const int* st, const float* sin_t, const float* cos_t,
-                         int64_t max_seq, void* cache, hipStream_t s);
+// A decode step in one call: qkv = q | k | v unrotated, st = device {token, pos, fill}. q and k are rotated at position pos, k and
+// v go into the cache at slot fill (nowhere if it is full) with the bytes of the calls above, and the attention is over
+// fill + 1 slots. head_dim 128, at most 16 query heads a KV head; rows and tables 16-byte aligned; ws as above (1, 1, .., max_seq).
+int aeth_attn_kv8_step_launch(const float* qkv, int64_t nq, int64_t nkv, int64_t hd, const int* st, const float* sin_t,
+                              const float* cos_t, int64_t max_seq, int64_t window, void* cache, float* out, void* ws, hipStream_t s);

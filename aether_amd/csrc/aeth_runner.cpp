@@ -224,11 +224,10 @@ int enqueue_layers(aeth_runner* r, int l0, int l1) {
                 (rc = aeth_gemv_launch_ex(r->wv[l], r->x, 1, r->qkv + qd + kvd, e1, s)))
                 return rc;
         }
-        if (r->kv8) {  // RoPE and the quantised append of the token, then the attention over fill + 1 slots
+        if (r->kv8) {  // RoPE, the quantised append of the token and the attention over fill + 1 slots
             uint8_t* lkv = r->kv8 + l * kv8_layer_bytes(c);
-            if ((rc = aeth_kv8_step_launch(r->qkv, nh, nkv, hd, r->st, r->rope_sin, r->rope_cos, c.max_seq_len, lkv, s)) ||
-                (rc = aeth_attn_kv8_launch(r->qkv, nh * hd, lkv, 0, r->st + 2, 1, 1, 1, nh, nkv, hd, c.max_seq_len,
-                                           c.max_seq_len, c.sliding_window, r->attn, r->a8_ws, s)))
+            if ((rc = aeth_attn_kv8_step_launch(r->qkv, nh, nkv, hd, r->st, r->rope_sin, r->rope_cos, c.max_seq_len,
+                                                c.sliding_window, lkv, r->attn, r->a8_ws, s)))
                 return rc;
         } else {
             float* lkv = r->kv + (int64_t)l * kv_layer_floats(c);

@@ -111,8 +111,43 @@ def test_prefill_and_steps_match_the_exact_model(gpu, layer_dtype, n, window):
             tokens.append((31 * i + 5) % c["vocab_size"])
             got = decode(r, c, int(tokens[-1]), n + i)
             assert_close_logits(got, R.model_logits(c, m, tokens), floor=FLOOR, what="step %d" % i)
+        kv, fill = cache_of(r, c)
+        assert fill == n + 3 and np.array_equal(kv, R.quantised(kv)) and not kv[:, :, :, n + 3:].any()
     finally:
         L.aeth_runner_free(r)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (8, 1), (3, 3)])
+def test_steps_fill_the_cache_as_a_prompt_does(gpu, heads, kv_heads):
+    """Token by token through every place of two tiles, against the same tokens as a prompt. Layer 0 has the same
+    inputs: its sums differ in their order, so an entry by at most one code, a step of 1/127 of its row's largest;
+    layer 1's inputs then differ by about 2e-3 of their size, and its rows by twice that at most."""
+    L = A.lib()
+    c = dict(INT8, num_heads=heads, num_kv_heads=kv_heads)
+    m = build_tiny(seed=26, c=c)
+    tokens = list(np.random.default_rng(8).integers(0, c["vocab_size"], 130))
+    r, p = make_runner(m, c), make_runner(m, c)
+    try:
+        for i, t in enumerate(tokens):
+            logits = decode(r, c, int(t), i)
+        want = prefill(p, c, tokens)
+        (a, fa), (b, fb) = cache_of(r, c), cache_of(p, c)
+        assert fa == fb == 130 and not a[:, :, :, 130:].any()
+        for layer, slack in ((0, 1.01 / 127), (1, 1.01 / 127 + 8e-3)):
+            big = np.abs(b[layer, :, :, :130]).max(-1, keepdims=True)
+            assert (np.abs(a[layer, :, :, :130] - b[layer, :, :, :130]) <= slack * big).all(), layer
+        # The logits, as near as the model itself stands: how far the exact one moves when its embeddings move by 4e-7
+        # (1e-8 of the largest logit for the first two models; the third's attention has two keys so close that it
+        # moves by more than the largest: its cache above is what it shows).
+        exact, moved = R.model_logits(c, m, tokens), 0.0
+        for s in range(3):
+            noise = 1.0 + 4e-7 * np.random.default_rng(s).standard_normal(m["emb"].shape)
+            moved = max(moved, np.abs(R.model_logits(c, dict(m, emb=m["emb"] * noise), tokens) - exact).max())
+        for got in (logits, want):
+            assert np.abs(got - exact).max() <= FLOOR * np.abs(exact).max() + 4 * moved
+    finally:
+        L.aeth_runner_free(r)
+        L.aeth_runner_free(p)
 
 
 def test_long_prompt(gpu):
