@@ -679,8 +679,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
     }
     // One barrier a tile, between its two steps: the codes of the next tile are stored before it, to K's other buffer,
     // whose last readers were two steps back, and V's third, whose readers were three (of two: one, behind a second
-    // barrier). (Behind the last tile a step's
-    // "next" scores are of what the other buffer holds: all masked.)
+    // barrier). Behind the chunk's last tile a step's "next" products are of what the other buffer holds, and are dropped.
     int b3 = 0;
     for (int t = t0; t < t1; t++) {
         const int b = (t - t0) & 1, n3 = b3 == NB - 1 ? 0 : b3 + 1;
@@ -697,7 +696,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
         bound_scores(64 * t + 32);
         __syncthreads();
         step(b3, 1, kb[b ^ 1] + lane * 16, n3, 0, [] {});
-        bound_scores(64 * t + 64);
+        if (t + 1 < t1) bound_scores(64 * t + 64);
         if (NB == 2) __syncthreads();
         b3 = n3;
     }

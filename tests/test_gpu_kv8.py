@@ -345,6 +345,26 @@ def test_attention_over_uneven_rows(gpu, n, seq):
         within(torch, got, want, bound)
 
 
+@pytest.mark.parametrize("n,seq,heads,nkv,hd", [(250, 8448, 32, 8, 128), (70, 9000, 16, 8, 128), (90, 9000, 16, 8, 64), (1, 9000, 32, 8, 128)])
+def test_split_rows_of_tiles_that_differ(gpu, n, seq, heads, nkv, hd):
+    """Every other tile holds keys a hundred times as long that no query points at: codes of one tile beside the
+    scales of another would give scores far above any there is, at the end of a chunk as within it."""
+    torch = gpu
+    slots = -(-seq // 64) * 64
+    k, v = rand(torch, 45, nkv, slots, hd), rand(torch, 46, nkv, slots, hd)
+    q = 2.0 * rand(torch, 47, n, heads * hd)
+    q.view(n, heads, hd)[..., hd // 2:] = 0.0
+    odd = (torch.arange(slots, device="cuda") // 64) % 2 == 1
+    for which in (odd, ~odd):
+        long = k.clone()
+        long[:, which, :hd // 2] = 0.0
+        long[:, which, hd // 2:] *= 100.0
+        layer = R.pack(*R.codes(long), *R.codes(v))
+        got = attend(torch, q, layer, nkv, hd, slots, seq)
+        want, bound = R.attention(q, layer, nkv, hd, slots, seq, 0)
+        within(torch, got, want, bound)
+
+
 @pytest.mark.parametrize("heads,nkv,hd,window", [(32, 8, 128, 0), (5, 1, 64, 0), (16, 4, 256, 0), (8, 2, 128, 300), (34, 2, 128, 0)])
 def test_batch_attention(gpu, heads, nkv, hd, window):
     """Sequences of no, one and many tokens in one call; rows behind the last one as they were."""
