@@ -321,6 +321,8 @@ extern "C" AETH_API int aeth_kv8_append_batch(void* d_layers, int64_t layer_stri
     if (!strides_ok(n_seqs, kv_heads, head_dim, token_stride, head_stride))
         return aeth_set_error(AETH_EINVAL, "%s: strides %lld / %lld of rows of %lld", what, (long long)token_stride,
                               (long long)head_stride, (long long)head_dim);
+    if (n_seqs * kv_heads > (int64_t)1 << 25)  // 2·hd/8 threads each within the grid's 2^32
+        return aeth_set_error(AETH_EUNSUPPORTED, "%s: %lld sequences of %lld heads in one call", what, (long long)n_seqs, (long long)kv_heads);
     return aeth_kv8_append_launch(d_layers, layer_stride, d_slots, n_seqs, d_k, d_v, token_stride, head_stride, 1, kv_heads,
                                   head_dim, max_seq, 0, (hipStream_t)stream);
 }

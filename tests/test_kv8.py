@@ -62,6 +62,12 @@ def test_batch_append_refuses(change, rc):
     assert "aeth_kv8_append_batch" in A.last_error()
 
 
+def test_batch_append_refuses_more_than_a_grid():
+    heads = 60000
+    change = dict(seqs=60000, nkv=heads, stride=heads * 64 * 264, ts=heads * 128)
+    assert call("aeth_kv8_append_batch", BATCH_APPEND, change) == -4
+
+
 ATTN = dict(q=P, qs=4096, layer=P, n=2, nq=32, nkv=8, hd=128, ms=4096, seq=4096, window=0, out=P, ws=P, wsb=1 << 40, stream=None)
 BATCH = dict(q=P, qs=4096, layers=P, stride=64 * BYTES, lens=P, seqs=3, nq=32, nkv=8, hd=128, ms=4096, ml=4096, window=0, out=P, ws=P,
              wsb=1 << 40, stream=None)
