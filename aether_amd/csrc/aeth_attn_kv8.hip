@@ -773,6 +773,57 @@ __global__ void __launch_bounds__(256) k_attn8_merge(A8 A, int cw) {
     A.out[((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + tid] = L == 0.0f ? 0.0f : y * (1.0f / L);
 }
 
+// The same for at most 8 chunks: hd / 4 lanes a column, its partials all in flight at once
+template <int HD>
+__global__ void __launch_bounds__(256) k_attn8_merge_few(A8 A, int cw) {
+    constexpr int MOST = 8;
+    const int unit = (blockIdx.x * 256 + threadIdx.x) / (HD / 4), d = 4 * (threadIdx.x % (HD / 4)), seq = blockIdx.y;
+    if (unit >= A.nkv * A.cols) return;
+    const int h = unit / A.cols, x = unit % A.cols, cb = x / cw, cc = x % cw;
+    int beg, end;
+    a8_tiles(A, a8_len(A, seq), cb * cw, cw, beg, end);
+    const int live = max(1, (end - beg + A.tpc - 1) / A.tpc);
+    const int64_t step = (int64_t)cw * (HD + 2);
+    const float* part = A.ws + (int64_t)((seq * A.nkv + h) * A.ncb + cb) * A.chunks * step;
+    float2 ml[MOST];
+    a8_f4 v[MOST];
+#pragma unroll
+    for (int k = 0; k < MOST; k++)
+        if (k < A.chunks) {  // (uniform)
+            const int64_t at = min(k, live - 1) * step;
+            ml[k] = *(const float2*)(part + at + cw * HD + 2 * cc);
+            v[k] = *(const a8_f4*)(part + at + cc * HD + d);
+        }
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int k = 0; k < MOST; k++)
+        if (k < A.chunks) M = fmaxf(M, ml[k].x);
+    a8_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < MOST; k++)
+        if (k < A.chunks) {
+            const float w = ml[k].x == -INFINITY || k >= live ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - M);
+            const bool in = k < live;
+            L += in ? w * ml[k].y : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] += in ? v[k][e] * w : 0.0f;
+        }
+    acc = L == 0.0f ? (a8_f4){0.0f, 0.0f, 0.0f, 0.0f} : acc * (1.0f / L);
+    float* dst = A.out + ((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + d;
+    if (A.ovec) *(a8_f4*)dst = acc;
+    else dst[0] = acc[0], dst[1] = acc[1], dst[2] = acc[2], dst[3] = acc[3];
+}
+
+// A workgroup a column costs a µs for each thousand of them (16000 columns in 2 chunks: 25 µs, 9 with 32 lanes each; 8000 in 8:
+// 15 and 8); of a few columns it has more of many chunks in flight (256 columns in 8 chunks: 0.8 µs less, 1024: 0.2).
+template <int HD>
+void a8_merge(const A8& A, int cw, int64_t seqs, hipStream_t s) {
+    const int64_t cols = (int64_t)A.nkv * A.cols;
+    if (A.chunks <= 4 || (A.chunks <= 8 && cols * seqs >= 6 * (int64_t)aeth_num_cus()))
+        hipLaunchKernelGGL(k_attn8_merge_few<HD>, dim3((unsigned)aeth_cdiv(cols * (HD / 4), 256), (unsigned)seqs), dim3(256), 0, s, A, cw);
+    else hipLaunchKernelGGL(k_attn8_merge<HD>, dim3((unsigned)cols, (unsigned)seqs), dim3(256), 0, s, A, cw);
+}
+
 // The form a call takes: the columns of a workgroup and, where its column blocks are fewer than `target`, the chunks of at
 // least tiles_min tiles that they are split into.
 struct Form {
@@ -802,21 +853,42 @@ Form a8_form(int64_t seqs, int64_t n, int64_t G, int64_t nkv, int64_t hd, int64_
     // longest sequence's do not decide (48 sequences of 1 .. 4096 tokens: 51.3 µs against 58.0).
     const Form small = a8_split(16, units(16), span(16), (ragged ? 4 : 2) * cus, 4);
     if (hd > 128 || cols <= 64 || ragged) return small;
-    // 128 and 256: not past one workgroup a CU, a split's join costs more than it gains (1000 tokens, 32 / 8 heads: 44 µs,
-    // 83 in two chunks). 256 shares its codes among more columns and has one on each CU: over a long past
-    // (250 queries over 20000 tokens 179 µs, 188 with 128 columns), or where a prompt's triangle fills the chip half as often
-    // again (3500 tokens: 211 against 228; 2500: 141 against 127).
-    Form big = a8_split(128, units(128), span(128), cus, 8);
-    const int64_t u = units(256);
-    if (hd == 128 && (2 * u >= 3 * cus || (2 * u <= cus && u * span(256) >= 16 * cus))) big = a8_split(256, u, span(256), cus, 8);
-    // µs on 256 CUs, 32 / 8 heads of 128, measured and (as reckoned here): 16 columns 18.6 (18.3) for 512 tokens, 41 (40) for 1000,
-    // 75 (76) for 1500, 115 (125) for 2000, 39 (40) for 128 queries over 4096; the wider forms 26 (34), 44 (47), 64 (61),
-    // 89 (84), 36 (36). At head_dim 64 both cost about half.
-    const double per = 256.0 / (double)cus;
-    const double t16 = 10.0 + 1.8e-3 * per * (double)heads * a8_blocks_tiles(16, cols, n, G, max_len, window);
-    const double tbig = 20.0 + std::max(1.7 * (double)std::min<int64_t>(big.tpc, span(big.cw)),
-                                        8e-3 * per * (double)heads * a8_blocks_tiles(128, cols, n, G, max_len, window));
-    return tbig < t16 ? big : small;
+    // Otherwise the least of what the forms take, in µs on a CU's share of the tiles (w; q: the fullest CU's of few workgroups),
+    // its workgroups' rounds (r: three at once, four) and the tiles of one (tpc), at head_dim 128 (64):
+    //   16 columns  max(5.5 + 0.45·tpc, 6 + 0.33·q + 4.5·r) (5 + 0.3·tpc, 5 + 0.185·q + 2.8·r)
+    //   128         max(8 + 2.3·tpc, 22 + 1.96·w) (7 + 1.53·tpc, 15 + 1.25·w): two workgroups a CU
+    //   256         12 + 2.8·max(tpc, w) + 1.5·max(0, w - 0.4·max(tpc, w)): one a CU, whose codes serve twice the columns; the chip
+    //               clocks lower when it is full
+    //   a split's join: 3, and one for each 4 MB of partials (16 columns: 2.5, 2 MB).
+    // 8 KV heads of 128, measured and (as reckoned) with 16 / 128 / 256 columns: 4 query heads each, 1000 tokens 40 (41) / 43 (44) /
+    // 56 (56), 2000 110 (116) / 86 (84) / 104 (101), 4000 375 (383) / 265 (265) / 252 (245), 1000 queries over 6000 in one / two /
+    // two chunks 248 (247) / 206 (202) / 194 (194), 70 over 30000 with 16 columns in 2, 4 and 8 chunks 169 (169), 130 (131), 114 (119);
+    // 2 query heads each, 2000 tokens 59 (61) / 74 (80) / 100 (100); one each, 512 tokens 10 (12), in two chunks 14 (17).
+    // At head_dim 64, 4 query heads each: 2000 tokens 60 (63) / 56 (55), 250 queries over 20000 127 (123), in 8 chunks of 128 112 (120).
+    const double c = (double)cus;
+    Form best = small;
+    double least = INFINITY;
+    for (int64_t cw = 16; cw <= (hd == 128 ? 256 : 128); cw = std::max<int64_t>(128, 2 * cw)) {
+        const double tiles = (double)heads * a8_blocks_tiles(cw, cols, n, G, max_len, window);
+        for (int64_t target : {(int64_t)0, cus, 2 * cus, 4 * cus}) {  // workgroups split for
+            if (target > (cw == 16 ? 4 : cw == 128 ? 2 : 1) * cus) continue;
+            const Form f = a8_split(cw, units(cw), span(cw), std::max<int64_t>(1, target), cw == 16 ? 4 : 8);
+            const int64_t wgs = units(cw) * f.chunks;
+            const double w = tiles / c, tpc = (double)std::min<int64_t>(f.tpc, span(cw));
+            const double u = (double)aeth_cdiv(wgs, cus), q = u * (tiles / (double)wgs);
+            const double own = std::max(tpc, w);
+            double t = cw == 256   ? 12.0 + 2.8 * own + 1.5 * std::max(0.0, w - 0.4 * own)
+                       : cw == 128 ? (hd == 128 ? std::max(8.0 + 2.3 * tpc, 22.0 + 1.96 * w) : std::max(7.0 + 1.53 * tpc, 15.0 + 1.25 * w))
+                       : hd == 128 ? std::max(5.5 + 0.45 * tpc, 6.0 + 0.33 * q + 4.5 * std::ceil(u / 3.0))
+                                   : std::max(5.0 + 0.3 * tpc, 5.0 + 0.185 * q + 2.8 * std::ceil(u / 4.0));
+            if (f.chunks > 1) t += (cw == 16 ? 2.5 : 3.0) + (cw == 16 ? 2e-6 : 1e-6) * (double)(heads * cols * f.chunks) * (double)(hd + 2);
+            if (t < least) {
+                least = t;
+                best = f;
+            }
+        }
+    }
+    return best;
 }
 
 template <int HD>
@@ -829,7 +901,7 @@ int a8_launch(const A8& A, const Form& f, int64_t seqs, hipStream_t s) {
         if (f.cw == 256) hipLaunchKernelGGL((k_attn8p<HD, 8>), grid, dim3(512), 0, s, A);
     AETH_LAUNCH_CHECK();
     if (A.chunks > 1) {
-        hipLaunchKernelGGL(k_attn8_merge<HD>, dim3((unsigned)((int64_t)A.nkv * A.cols), (unsigned)seqs), dim3(256), 0, s, A, f.cw);
+        a8_merge<HD>(A, f.cw, seqs, s);
         AETH_LAUNCH_CHECK();
     }
     return AETH_OK;
@@ -847,7 +919,7 @@ int64_t aeth_attn_kv8_ws(int64_t seqs, int64_t n, int64_t nq, int64_t nkv, int64
         return (target + std::min(units, target)) * cw;
     };
     int64_t most = need(16, 4 * cus);
-    if (hd <= 128 && cols > 64) most = std::max(most, need(128, cus));
+    if (hd <= 128 && cols > 64) most = std::max(most, need(128, 2 * cus));
     if (hd == 128 && cols > 64) most = std::max(most, need(256, cus));
     return most * (hd + 2) * (int64_t)sizeof(float);
 }
@@ -916,7 +988,7 @@ int aeth_attn_kv8_step_launch(const float* qkv, int64_t nq, int64_t nkv, int64_t
     hipLaunchKernelGGL((k_attn8<128, true>), dim3((unsigned)(nkv * A.chunks)), dim3(256), 0, s, A);
     AETH_LAUNCH_CHECK();
     if (A.chunks > 1) {
-        hipLaunchKernelGGL(k_attn8_merge<128>, dim3((unsigned)nq), dim3(256), 0, s, A, 16);
+        a8_merge<128>(A, 16, 1, s);
         AETH_LAUNCH_CHECK();
     }
     return AETH_OK;

@@ -322,9 +322,13 @@ AETH_API int64_t aeth_attn_kv8_ws_bytes(int64_t n_seqs, int64_t n, int64_t n_hea
  * n = 1 is aeth_attn_decode, n = seq aeth_attn_prefill, and what lies between a
  * chunk of a prompt or a drafted continuation. d_out is [n][n_heads·head_dim],
  * not overlapping d_q. q enters a score rounded to 2^-23 of its row's largest
- * component, a probability rounded to 2^-23 of the largest product of
- * probability and V scale in 64 tokens; sums in 32 bits or more. A visible
- * token with an infinity or NaN makes the row NaN, a masked one has no effect. */
+ * component. A probability times its token's V scale enters the sum rounded to
+ * 2^-23 of the largest such product in 64 tokens or, in the forms for many
+ * queries, to 2^-23 of itself or 2^-34 of the row's largest; products below
+ * about 2^-90 keep fewer bits, values past 2^119 make the row NaN. Sums are in
+ * 32 bits or more. A visible token with an infinity or NaN makes the row NaN, a
+ * masked one has no effect. The same call gives the same bits again; a token
+ * attended alone and the same one within a longer call agree to those roundings. */
 AETH_API int aeth_attn_kv8(const float* d_q, int64_t q_stride, const void* d_layer, int64_t n, int64_t n_heads,
                            int64_t kv_heads, int64_t head_dim, int64_t max_seq, int64_t seq, int64_t window,
                            float* d_out, void* d_ws, int64_t ws_bytes, void* stream);

@@ -227,6 +227,11 @@ ATTN = [
     # a window, a prompt for the largest
     (1700, 1700, 32, 8, 128, 0), (3100, 3100, 24, 8, 64, 0), (70, 30000, 16, 8, 128, 0), (250, 20001, 32, 8, 128, 0), (330, 12000, 7, 1, 64, 0),
     (4000, 6000, 32, 8, 128, 555), (3500, 3500, 32, 8, 128, 0), (2000, 2100, 3, 3, 256, 0),
+    # 128 columns whole, in a few chunks, in many; with a window
+    (600, 600, 64, 8, 64, 0), (600, 1600, 64, 8, 64, 700), (333, 3333, 64, 8, 64, 3000), (600, 7600, 7, 1, 64, 0), (200, 20200, 6, 2, 64, 0),
+    (600, 600, 64, 8, 128, 0), (333, 1333, 64, 8, 128, 700), (2000, 3000, 16, 8, 128, 0), (100, 7100, 64, 8, 128, 0), (333, 20333, 8, 8, 128, 0),
+    # 256 columns
+    (333, 1333, 64, 8, 128, 0), (600, 1600, 64, 8, 128, 700), (600, 3600, 16, 8, 128, 0), (600, 3600, 16, 8, 128, 3000 - 7), (100, 7100, 32, 8, 128, 0),
 ]
 
 
@@ -345,7 +350,8 @@ def test_attention_over_uneven_rows(gpu, n, seq):
         within(torch, got, want, bound)
 
 
-@pytest.mark.parametrize("n,seq,heads,nkv,hd", [(250, 8448, 32, 8, 128), (70, 9000, 16, 8, 128), (90, 9000, 16, 8, 64), (1, 9000, 32, 8, 128)])
+@pytest.mark.parametrize("n,seq,heads,nkv,hd", [(250, 8448, 32, 8, 128), (70, 9000, 16, 8, 128), (90, 9000, 16, 8, 64), (1, 9000, 32, 8, 128),
+                                                (100, 7100, 64, 8, 128), (600, 7600, 7, 1, 64), (100, 7100, 32, 8, 128)])
 def test_split_rows_of_tiles_that_differ(gpu, n, seq, heads, nkv, hd):
     """Every other tile holds keys a hundred times as long that no query points at: codes of one tile beside the
     scales of another would give scores far above any there is, at the end of a chunk as within it."""
