@@ -71,7 +71,7 @@ def test_cache_copies_hold_the_quantised_values(gpu):
         L.aeth_runner_free(r)
 
 
-@pytest.mark.parametrize("heads,kv_heads,window", [(4, 2, 0), (8, 1, 0), (3, 3, 0), (4, 2, 300), (6, 2, 0)])
+@pytest.mark.parametrize("heads,kv_heads,window", [(4, 2, 0), (8, 1, 0), (6, 6, 0), (4, 2, 300), (6, 2, 0)])
 def test_decode_over_a_filled_cache_matches_the_oracle(gpu, heads, kv_heads, window):
     """Steps behind 1000 cached tokens, whose values the oracle takes as they stand; the steps' own tokens are
     f32 there (8 bits of one token in a thousand)."""
@@ -117,7 +117,7 @@ def test_prefill_and_steps_match_the_exact_model(gpu, layer_dtype, n, window):
         L.aeth_runner_free(r)
 
 
-@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (8, 1), (3, 3)])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (8, 1), (6, 6)])
 def test_steps_fill_the_cache_as_a_prompt_does(gpu, heads, kv_heads):
     """Token by token through every place of two tiles, against the same tokens as a prompt. Layer 0 has the same
     inputs: its sums differ in their order, so an entry by at most one code, a step of 1/127 of its row's largest;
@@ -136,15 +136,9 @@ def test_steps_fill_the_cache_as_a_prompt_does(gpu, heads, kv_heads):
         for layer, slack in ((0, 1.01 / 127), (1, 1.01 / 127 + 8e-3)):
             big = np.abs(b[layer, :, :, :130]).max(-1, keepdims=True)
             assert (np.abs(a[layer, :, :, :130] - b[layer, :, :, :130]) <= slack * big).all(), layer
-        # The logits, as near as the model itself stands: how far the exact one moves when its embeddings move by 4e-7
-        # (1e-8 of the largest logit for the first two models; the third's attention has two keys so close that it
-        # moves by more than the largest: its cache above is what it shows).
-        exact, moved = R.model_logits(c, m, tokens), 0.0
-        for s in range(3):
-            noise = 1.0 + 4e-7 * np.random.default_rng(s).standard_normal(m["emb"].shape)
-            moved = max(moved, np.abs(R.model_logits(c, dict(m, emb=m["emb"] * noise), tokens) - exact).max())
+        exact = R.model_logits(c, m, tokens)
         for got in (logits, want):
-            assert np.abs(got - exact).max() <= FLOOR * np.abs(exact).max() + 4 * moved
+            assert np.abs(got - exact).max() <= FLOOR * np.abs(exact).max()
     finally:
         L.aeth_runner_free(r)
         L.aeth_runner_free(p)
