@@ -126,11 +126,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
     __shared__ __attribute__((aligned(16))) uint32_t fresh[2][HD / 4];  // STEP: the token's codes of K and V
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int id = blockIdx.x;
-    const int h = id % A.nkv;
-    id /= A.nkv;
-    const int cb = A.ncb - 1 - id % A.ncb;  // late queries, the longest rows, first
-    const int chunk = id / A.ncb, seq = blockIdx.y;
+    const int h = blockIdx.x % A.nkv, cb = A.ncb - 1 - blockIdx.x / A.nkv;  // late queries, the longest rows, first
+    const int seq = blockIdx.y, chunk = blockIdx.z;                         // the first chunks, which every sequence has, first
     const int len = a8_len(A, seq);
     int beg, end;
     a8_tiles(A, len, cb * 16, 16, beg, end);
@@ -445,10 +442,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
     __shared__ __attribute__((aligned(16))) float sc[NB][2 * KV8_TILE];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int id = blockIdx.x;
-    const int h = id % A.nkv;
-    id /= A.nkv;
-    const int cb = A.ncb - 1 - id % A.ncb, chunk = id / A.ncb, seq = blockIdx.y;
+    const int h = blockIdx.x % A.nkv, cb = A.ncb - 1 - blockIdx.x / A.nkv, seq = blockIdx.y, chunk = blockIdx.z;
     const int len = a8_len(A, seq);
     int beg, end;
     a8_tiles(A, len, cb * 32 * NW, 32 * NW, beg, end);
@@ -849,9 +843,31 @@ Form a8_form(int64_t seqs, int64_t n, int64_t G, int64_t nkv, int64_t hd, int64_
     const int64_t cus = aeth_num_cus(), cols = n * G, heads = seqs * nkv;
     auto span = [&](int64_t cw) { return a8_span(cw, n, G, max_len, window); };
     auto units = [&](int64_t cw) { return heads * aeth_cdiv(cols, cw); };
-    // 16 columns: split until two workgroups a CU have work. Lengths that only the device knows get twice as many: the
-    // longest sequence's do not decide (48 sequences of 1 .. 4096 tokens: 51.3 µs against 58.0).
+    // 16 columns: split until two workgroups a CU have work; four, where the device alone knows the length
     const Form small = a8_split(16, units(16), span(16), (ragged ? 4 : 2) * cus, 4);
+    if (ragged && seqs > 1) {
+        // A batch: the least, in µs, of 5 + ((0.34·tpc)^1.5 + max(MB / 6.4, 1.5·r)^1.5)^(2/3) + 0.2·wgs/CU, and where it is split 2.2 +
+        // 0.19 for each 100,000 floats of partials: tpc the longest workgroup's tiles, MB what is read if lengths are spread
+        // evenly up to max_len, r the rounds of workgroups (three on a CU at once). 32 / 8 heads of 128, measured and (as reckoned)
+        // whole / in two / in four chunks: 64 sequences of up to 300 tokens 10 (10) / 13 (13), 1000 18 (19) / 22 (21), 4096 56 (58) / 55 (56) /
+        // 52 (56); 24 of up to 4096 31 (34) / 32 (29) / 29 (27), 8 29 (29) / 21 (20) / 16 (16).
+        const double sp = (double)span(16), f4 = hd == 64 ? 0.5 : hd == 128 ? 1.0 : 2.0;
+        const double mb = (double)units(16) * (window > 0 ? sp : 0.5 * sp + 0.5) * (double)aeth_kv8_tile_bytes((int)hd) * 1e-6;
+        Form best = small;
+        double least = INFINITY;
+        for (int64_t target : {(int64_t)1, cus, 2 * cus, 4 * cus}) {
+            const Form f = a8_split(16, units(16), span(16), target, 4);
+            const double wgs = (double)(units(16) * f.chunks) / (double)cus, rounds = std::ceil(std::ceil(wgs) / (hd == 64 ? 4.0 : 3.0));
+            const double chain = 0.34 * f4 * std::min((double)f.tpc, sp), flow = std::max(mb / 6.4, 1.5 * f4 * rounds);
+            double t = 5.0 + std::cbrt(std::pow(chain * std::sqrt(chain) + flow * std::sqrt(flow), 2.0)) + 0.2 * f4 * wgs;
+            if (f.chunks > 1) t += 2.2 + 1.9e-6 * (double)(heads * cols * f.chunks) * (double)(hd + 2);
+            if (t < least) {
+                least = t;
+                best = f;
+            }
+        }
+        return best;
+    }
     if (hd > 128 || cols <= 64 || ragged) return small;
     // Otherwise the least of what the forms take, in µs on a CU's share of the tiles (w; q: the fullest CU's of few workgroups),
     // its workgroups' rounds (r: three at once, four) and the tiles of one (tpc), at head_dim 128 (64):
@@ -893,7 +909,7 @@ Form a8_form(int64_t seqs, int64_t n, int64_t G, int64_t nkv, int64_t hd, int64_
 
 template <int HD>
 int a8_launch(const A8& A, const Form& f, int64_t seqs, hipStream_t s) {
-    const dim3 grid((unsigned)((int64_t)A.nkv * A.ncb * A.chunks), (unsigned)seqs);
+    const dim3 grid((unsigned)((int64_t)A.nkv * A.ncb), (unsigned)seqs, (unsigned)A.chunks);
     if (f.cw == 16) hipLaunchKernelGGL((k_attn8<HD, false>), grid, dim3(256), 0, s, A);
     if constexpr (HD <= 128)
         if (f.cw == 128) hipLaunchKernelGGL((k_attn8p<HD, 4>), grid, dim3(256), 0, s, A);
@@ -985,7 +1001,7 @@ int aeth_attn_kv8_step_launch(const float* qkv, int64_t nq, int64_t nkv, int64_t
     A.ncb = 1;
     A.tpc = f.tpc;
     A.chunks = f.chunks;
-    hipLaunchKernelGGL((k_attn8<128, true>), dim3((unsigned)(nkv * A.chunks)), dim3(256), 0, s, A);
+    hipLaunchKernelGGL((k_attn8<128, true>), dim3((unsigned)nkv, 1, (unsigned)A.chunks), dim3(256), 0, s, A);
     AETH_LAUNCH_CHECK();
     if (A.chunks > 1) {
         a8_merge<128>(A, 16, 1, s);
