@@ -111,7 +111,10 @@ __device__ __forceinline__ void a8_tiles(const A8& A, int len, int c0, int count
 }
 
 // Workgroup (KV head, column block of 16, chunk, sequence): its four waves take the chunk's tiles round robin,
-// each with its own running softmax, and merge through LDS.
+// each with its own running softmax, and merge through LDS. 32 / 8 heads of 128: a token over 2049 positions 6.7 µs (one tile a
+// wave: its loads and the chain from them to the output, beside 2.3 of an empty launch), over 131000 48 (5.7 TB/s, memory),
+// 48 tokens over up to 4096 46 (4.6 TB/s: uneven lengths); 512 queries 18.5 (eight instructions a score and ten a
+// probability and output share, and two rounds of workgroups that live for two tiles a wave).
 // A token's scales belong to one register of every lane (lane group g holds tokens 16j + 4g + r in registers
 // 4j + r): lane i of a row of 16 holds the one of register i's token, and the multiplication takes it from there.
 // STEP (HD = 128, one column block): a decode step's token with it. Each workgroup rotates q; the wave that takes the token's
@@ -414,6 +417,11 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
 // the order in which V's operand takes its tokens (j = 2T + u, g = 2a + h of aeth_kv8.hpp), so the
 // probabilities stay in their lanes. The next tile's codes are loaded a tile ahead, converted and stored in
 // the other LDS buffer before this tile's products: one barrier a tile.
+// 32 / 8 heads of 128: 4000 tokens 253 µs (0.52 PFLOP/s of the formula, 1.04 of the matrix units'), 250 over 20000 161 with its
+// join. The matrix units are busy 49 % of the cycles, at 2.0 GHz, the vector units 44 %: of two waves a SIMD one is often
+// waiting for the other's instruction to leave the issue port (36 % of the waves' time) or for LDS and the barrier (30 %). The two
+// phases of two waves kept apart by barriers, another priority for one of them, K a step ahead and reads from LDS further
+// ahead took as long or longer.
 typedef _Float16 a8_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 a8_h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 a8_h2 __attribute__((ext_vector_type(2)));
