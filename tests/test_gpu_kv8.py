@@ -350,6 +350,88 @@ def test_attention_over_uneven_rows(gpu, n, seq):
         within(torch, got, want, bound)
 
 
+WIDE = [  # calls of many columns: 128 whole, with a window, split; 256 split, whole
+    (800, 800, 48, 2, 128, 0), (600, 600, 64, 8, 64, 0), (1000, 4000, 32, 2, 128, 600), (600, 7600, 7, 1, 64, 0), (500, 4000, 32, 2, 128, 0),
+    (700, 3000, 32, 1, 128, 0), (1500, 1500, 64, 8, 128, 0),
+]
+
+
+@pytest.mark.parametrize("n,seq,heads,nkv,hd,window", WIDE)
+def test_many_columns_with_no_numbers_and_any_stride(gpu, n, seq, heads, nkv, hd, window):
+    """What the tests above ask of a few columns: slots that no query sees hold infinities and NaN, a token that some
+    see is a NaN, a query is one; rows from an odd address with a gap, the result to one."""
+    torch = gpu
+    max_seq = seq + 70
+    layer = some_layer(torch, 24, nkv, hd, max_seq)
+    kc, vc, ks, vs = R.unpack(layer, nkv, hd, max_seq)
+    ks[:, seq:], vs[:, seq:] = math.nan, math.inf
+    if window:
+        ks[:, :seq - n - window + 1], vs[:, :seq - n - window + 1] = math.inf, math.nan
+    layer = R.pack(kc, ks, vc, vs)
+    q = rand(torch, 25, n, heads * hd)
+    want, bound = R.attention(q, layer, nkv, hd, max_seq, seq, window)
+    within(torch, attend(torch, q, layer, nkv, hd, max_seq, seq, window), want, bound)
+    stride = heads * hd + 3
+    rows = torch.as_strided(torch.zeros((n - 1) * stride + heads * hd + 1, device="cuda"), (n, heads * hd), (stride, 1), 1)
+    rows.copy_(q)
+    out = torch.full((n * heads * hd + 2,), 7.0, device="cuda")
+    L = A.lib()
+    ws = torch.full((max(L.aeth_attn_kv8_ws_bytes(1, n, heads, nkv, hd, seq), 16),), 0xFF, dtype=torch.uint8, device="cuda")
+    A.check(L.aeth_attn_kv8(rows.data_ptr(), stride, layer.data_ptr(), n, heads, nkv, hd, max_seq, seq, window, out[1:].data_ptr(), ws.data_ptr(), ws.numel(),
+                            stream(torch)), "attn")
+    within(torch, out[1:-1].reshape(n, -1), want, bound)
+    assert out[0] == 7.0 and out[-1] == 7.0
+    # a token of a NaN scale in the last KV head, and a query with one
+    at, bad_q = seq - 1 - n // 2, n // 3
+    pos = torch.arange(seq - n, seq, device="cuda")
+    sees = (pos >= at) & ((pos - window < at) if window else True)
+    sees[bad_q] = False
+    q[bad_q, 5] = math.inf
+    for which in (ks, vs):
+        old = which[-1, at].clone()
+        which[-1, at] = math.nan
+        got = attend(torch, q, R.pack(kc, ks, vc, vs), nkv, hd, max_seq, seq, window)
+        which[-1, at] = old
+        nan = torch.isnan(got).reshape(n, nkv, -1)
+        assert torch.isnan(got[bad_q, :hd]).all()
+        rest = torch.arange(n, device="cuda") != bad_q
+        assert nan[sees][:, -1].all() and not nan[rest & ~sees].any() and not nan[rest][:, :-1].any()
+        fine = ~nan & rest[:, None, None]
+        within(torch, got.reshape(n, nkv, -1)[fine], want.reshape(n, nkv, -1)[fine], bound.reshape(n, nkv, -1)[fine])
+
+
+@pytest.mark.parametrize("n,seq,heads,nkv,hd,window", [w for w in WIDE if w[0] < 1000])
+def test_many_columns_over_uneven_rows(gpu, n, seq, heads, nkv, hd, window):
+    torch = gpu
+    slots = -(-seq // 64) * 64
+    base, val = rand(torch, 43, nkv, slots, hd), rand(torch, 44, nkv, slots, hd)
+    q = rand(torch, 48, n, heads * hd)
+    t = torch.arange(slots, device="cuda").float()[None, :, None]
+    for k, v in ((base * (1.0 + t / 20.0), val), (base * (1.0 + (seq - t).clamp_min(0) / 20.0), val), (base * 0.0, val),
+                 (base * 1e-3, val * torch.pow(10.0, (t % 41) - 20.0)), (base, val * torch.pow(10.0, -t / 50.0).clamp_min(1e-30)), (base, val * 1e33)):
+        layer = R.pack(*R.codes(k), *R.codes(v))
+        want, bound = R.attention(q, layer, nkv, hd, slots, seq, window)
+        within(torch, attend(torch, q, layer, nkv, hd, slots, seq, window), want, bound)
+
+
+def test_the_ends_of_the_ranges(gpu):
+    """4096 query heads of one KV head, 300 KV heads, a sequence of 2.5 million tokens, 3000 sequences."""
+    torch = gpu
+    for n, seq, heads, nkv, hd, window in ((1, 70, 4096, 1, 64, 0), (3, 200, 300, 300, 64, 0), (2, 2500000, 4, 1, 64, 0), (1, 2500000, 4, 1, 64, 2 ** 40)):
+        layer = some_layer(torch, 27, nkv, hd, seq)
+        q = rand(torch, 28, n, heads * hd)
+        want, bound = R.attention(q, layer, nkv, hd, seq, seq, 0)
+        within(torch, attend(torch, q, layer, nkv, hd, seq, seq, window), want, bound)
+    nkv, hd, seqs, max_seq = 1, 64, 3000, 300
+    layer = some_layer(torch, 29, nkv, hd, max_seq)
+    lens = torch.arange(seqs, dtype=torch.int32, device="cuda") % 301
+    q = rand(torch, 30, 1, 2 * hd)
+    got = attend_batch(torch, q.expand(seqs, -1).contiguous(), layer[None].expand(seqs, -1, -1, -1).contiguous(), lens, nkv, hd, max_seq, max_seq)
+    for n in (0, 1, 64, 65, 129, 300):
+        want, bound = R.attention(q, layer, nkv, hd, max_seq, n, 0)
+        within(torch, got[n::301], want.expand(len(got[n::301]), -1), bound.expand(len(got[n::301]), -1))
+
+
 @pytest.mark.parametrize("n,seq,heads,nkv,hd", [(250, 8448, 32, 8, 128), (70, 9000, 16, 8, 128), (90, 9000, 16, 8, 64), (1, 9000, 32, 8, 128),
                                                 (100, 7100, 64, 8, 128), (600, 7600, 7, 1, 64), (100, 7100, 32, 8, 128)])
 def test_split_rows_of_tiles_that_differ(gpu, n, seq, heads, nkv, hd):
