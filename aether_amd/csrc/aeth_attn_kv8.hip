@@ -94,6 +94,12 @@ __device__ __forceinline__ void a8_digits(uint32_t a, uint32_t b, uint32_t c, ui
     d2 = __builtin_amdgcn_perm(t, s, 0x05040100u) ^ 0x80808080u;
 }
 
+// Three digits' products, d2·65536 + d1·256 + d0, as f32: the low ones' sum starts from the bits of 1.5·2^23 and so is a
+// float as it stands (|d0| <= 128·127·256 < 2^22), the middle ones' from -1.5·2^23 / 256, which the fused addition takes out exactly
+#define A8_START0 (a8_i4){0x4B400000, 0x4B400000, 0x4B400000, 0x4B400000}
+#define A8_START1 (a8_i4){-49152, -49152, -49152, -49152}
+__device__ __forceinline__ float a8_join(int d0, int d1, int d2) { return fmaf((float)((d2 << 8) + d1), 256.0f, __int_as_float(d0)); }
+
 __device__ __forceinline__ int a8_len(const A8& A, int seq) {
     if (!A.lens) return A.max_len;
     const int64_t l = (int64_t)A.lens[seq] + A.len_add;
@@ -263,7 +269,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) o[dt] = (a8_f4){0.0f, 0.0f, 0.0f, 0.0f};
 
-    const a8_i4 zero = {0, 0, 0, 0};
+    const a8_i4 start[3] = {A8_START0, A8_START1, {0, 0, 0, 0}};
     for (int t = t0 + w; t < t1; t += 4) {
         if (STEP && mine && t == fresh_t) {  // (uniform) the token's codes and scales in place of what was loaded from its slot
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's stores of them
@@ -303,13 +309,13 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
             a8_i4 d[3];
 #pragma unroll
             for (int p = 0; p < 3; p++) {
-                d[p] = zero;
+                d[p] = start[p];
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[j][ks], qd[p][ks], d[p], 0, 0, 0);
             }
             a8_unroll<4>([&](auto rr) {
                 constexpr int r = rr, i = 4 * j + r;
-                s[i] = fmaf((float)((d[2][r] << 8) + d[1][r]), 256.0f, (float)d[0][r]) * a8_row<i>(sk);
+                s[i] = a8_join(d[0][r], d[1][r], d[2][r]) * a8_row<i>(sk);
             });
         });
         if (64 * t < all_lo || 64 * t + 64 > all_hi) {  // (uniform) some key is masked
@@ -343,7 +349,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
         wm = aeth_max_rows(wm);
         if (!(wm < INFINITY)) l = __uint_as_float(0x7FC00000u);  // values past 2^119: no number rather than a wrong one
         const int j2 = a8_exponent(wm);
-        const float f = a8_pow2(j2), fi = a8_pow2(-j2), fi8 = a8_pow2(8 - j2);
+        const float f = a8_pow2(j2), fi = a8_pow2(-j2);
         a8_i4 pd[3];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -359,9 +365,9 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
         for (int dt = 0; dt < DT; dt++) {
             a8_i4 d[3];
 #pragma unroll
-            for (int p = 0; p < 3; p++) d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[dt], pd[p], zero, 0, 0, 0);
+            for (int p = 0; p < 3; p++) d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[dt], pd[p], start[p], 0, 0, 0);
 #pragma unroll
-            for (int r = 0; r < 4; r++) o[dt][r] = fmaf((float)((d[2][r] << 8) + d[1][r]), fi8, fmaf((float)d[0][r], fi, o[dt][r]));
+            for (int r = 0; r < 4; r++) o[dt][r] = fmaf(a8_join(d[0][r], d[1][r], d[2][r]), fi, o[dt][r]);
         }
         if (t + 4 < t1) load(t + 4);
     }
@@ -851,8 +857,9 @@ Form a8_form(int64_t seqs, int64_t n, int64_t G, int64_t nkv, int64_t hd, int64_
     const int64_t cus = aeth_num_cus(), cols = n * G, heads = seqs * nkv;
     auto span = [&](int64_t cw) { return a8_span(cw, n, G, max_len, window); };
     auto units = [&](int64_t cw) { return heads * aeth_cdiv(cols, cw); };
-    // 16 columns: split until two workgroups a CU have work; four, where the device alone knows the length
-    const Form small = a8_split(16, units(16), span(16), (ragged ? 4 : 2) * cus, 4);
+    // 16 columns: split until two workgroups a CU have work; four, where the device alone knows the length; not up to 512
+    // tokens, two tiles a wave (a token over 300: 7.8 µs, 8.4 in two chunks; over 600: 9.7, 8.9 in three)
+    const Form small = a8_split(16, units(16), span(16), span(16) <= 8 ? 1 : (ragged ? 4 : 2) * cus, 4);
     if (ragged && seqs > 1) {
         // A batch: the least, in µs, of 5 + ((0.34·tpc)^1.5 + max(MB / 6.4, 1.5·r)^1.5)^(2/3) + 0.2·wgs/CU, and where it is split 2.2 +
         // 0.19 for each 100,000 floats of partials: tpc the longest workgroup's tiles, MB what is read if lengths are spread
