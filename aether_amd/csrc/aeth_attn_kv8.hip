@@ -80,18 +80,18 @@ __device__ __forceinline__ int a8_exponent(float mx) {
 }
 __device__ __forceinline__ float a8_pow2(int j) { return __int_as_float((127 + j) << 23); }
 
-// four integers of 24 bits (in the low bits of f32 words 2^23 + X or of plain words) → their digits'
-// words; each byte is digit + 128 before the exclusive or
-__device__ __forceinline__ void a8_digits(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t& d0, uint32_t& d1, uint32_t& d2) {
-    a += 0x808080u;
-    b += 0x808080u;
-    c += 0x808080u;
-    d += 0x808080u;
+// Four words X + 0x8080 (24 bits and more) → the words of their digits: bytes 0 and 1 are digit + 128, byte 2 is the digit (of X >= 0)
+__device__ __forceinline__ void a8_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t& d0, uint32_t& d1, uint32_t& d2) {
     const uint32_t p = __builtin_amdgcn_perm(b, a, 0x05010400u), q = __builtin_amdgcn_perm(d, c, 0x05010400u);
     const uint32_t s = __builtin_amdgcn_perm(b, a, 0x0C0C0602u), t = __builtin_amdgcn_perm(d, c, 0x0C0C0602u);
     d0 = __builtin_amdgcn_perm(q, p, 0x05040100u) ^ 0x80808080u;
     d1 = __builtin_amdgcn_perm(q, p, 0x07060302u) ^ 0x80808080u;
-    d2 = __builtin_amdgcn_perm(t, s, 0x05040100u) ^ 0x80808080u;
+    d2 = __builtin_amdgcn_perm(t, s, 0x05040100u);
+}
+// ... of four integers, |X| <= 0x7F7F00
+__device__ __forceinline__ void a8_digits(int a, int b, int c, int d, uint32_t& d0, uint32_t& d1, uint32_t& d2) {
+    a8_bytes((uint32_t)a + 0x808080u, (uint32_t)b + 0x808080u, (uint32_t)c + 0x808080u, (uint32_t)d + 0x808080u, d0, d1, d2);
+    d2 ^= 0x80808080u;
 }
 
 // Three digits' products, d2·65536 + d1·256 + d0, as f32: the low ones' sum starts from the bits of 1.5·2^23 and so is a
@@ -119,8 +119,8 @@ __device__ __forceinline__ void a8_tiles(const A8& A, int len, int c0, int count
 // Workgroup (KV head, column block of 16, chunk, sequence): its four waves take the chunk's tiles round robin,
 // each with its own running softmax, and merge through LDS. 32 / 8 heads of 128: a token over 2049 positions 6.7 µs (one tile a
 // wave: its loads and the chain from them to the output, beside 2.3 of an empty launch), over 131000 48 (5.7 TB/s, memory),
-// 48 tokens over up to 4096 46 (4.6 TB/s: uneven lengths); 512 queries 18.5 (eight instructions a score and ten a
-// probability and output share, and two rounds of workgroups that live for two tiles a wave).
+// 48 tokens over up to 4096 46 (4.6 TB/s: uneven lengths); 512 queries 17.9 (three instructions to join a
+// score's digits, four for an output's, five to make a probability's, and two rounds of workgroups that live for two tiles a wave).
 // A token's scales belong to one register of every lane (lane group g holds tokens 16j + 4g + r in registers
 // 4j + r): lane i of a row of 16 holds the one of register i's token, and the multiplication takes it from there.
 // STEP (HD = 128, one column block): a decode step's token with it. Each workgroup rotates q; the wave that takes the token's
@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 uint32_t d0, d1, d2;
-                a8_digits((uint32_t)(int)rintf(qv[s][4 * e] * f), (uint32_t)(int)rintf(qv[s][4 * e + 1] * f),
-                          (uint32_t)(int)rintf(qv[s][4 * e + 2] * f), (uint32_t)(int)rintf(qv[s][4 * e + 3] * f), d0, d1, d2);
+                a8_digits((int)rintf(qv[s][4 * e] * f), (int)rintf(qv[s][4 * e + 1] * f), (int)rintf(qv[s][4 * e + 2] * f),
+                          (int)rintf(qv[s][4 * e + 3] * f), d0, d1, d2);
                 qd[0][s][e] = (int)d0;
                 qd[1][s][e] = (int)d1;
                 qd[2][s][e] = (int)d2;
@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
         for (int j = 0; j < 4; j++) {
             uint32_t y[4], d0, d1, d2;
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[r] = __float_as_uint(fmaf(s[4 * j + r], f, 8388608.0f));
-            a8_digits(y[0], y[1], y[2], y[3], d0, d1, d2);
+            for (int r = 0; r < 4; r++) y[r] = __float_as_uint(fmaf(s[4 * j + r], f, 8388608.0f + 0x8080));  // below 2^24: rounded to whole
+            a8_bytes(y[0], y[1], y[2], y[3], d0, d1, d2);
             pd[0][j] = (int)d0;
             pd[1][j] = (int)d1;
             pd[2][j] = (int)d2;
@@ -410,8 +410,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
 }
 
 // ── many columns: a prompt, or a chunk of one ─────────────────────────────
-// The int8 form above spends more on joining digits than on the softmax itself: eight instructions a score
-// and ten a probability and output share. Here the codes become fp16 (exactly), once for a workgroup's
+// The int8 form above spends more on joining digits than on the softmax itself: three instructions a score,
+// four an output and tile of 64 tokens, five a probability. Here the codes become fp16 (exactly), once for a workgroup's
 // 32·NW columns, on their way to LDS, and q and the probabilities are each two fp16 parts, x = hi + lo
 // (22 significant bits), so that both products run on v_mfma_f32_32x32x16_f16 in two passes that share
 // their f32 accumulators: nothing is left to join.
