@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
             *(a8_h4*)dst = a8_half4(rv[u].x);
             *(a8_h4*)(dst + 1024) = a8_half4(rv[u].y);
             *(a8_h4*)(dst + 2048) = a8_half4(rv[u].z);
-            *(a8_h4*)(dst + 3072) = a8_half4(rv[u].w);
+            *(a8_h4*)(dst + 3 * 1024) = a8_half4(rv[u].w);
         }
     };
     if (t0 < t1) {
