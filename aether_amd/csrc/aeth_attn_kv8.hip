@@ -434,6 +434,12 @@ typedef _Float16 a8_h2 __attribute__((ext_vector_type(2)));
 typedef float a8_f2 __attribute__((ext_vector_type(2)));
 typedef float a8_f16 __attribute__((ext_vector_type(16)));
 
+// the larger of a column's two lanes
+__device__ __forceinline__ float a8_max_halves(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
 // four signed bytes as fp16
 __device__ __forceinline__ a8_h4 a8_half4(uint32_t w) {
     w ^= 0x80808080u;
@@ -553,7 +559,8 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
     }
     // m: the largest score so far, up to 2^TH stale. The step's probabilities are formed times 2^lf, as 2^(score - ref) with
     // ref = m - lf; lf keeps the largest p·sv so far (top, and o, times 2^lf) in [2^9, 2^15). l is of the p themselves.
-    float m = -INFINITY, l = 0.0f, top = 0.0f, ref = 0.0f;
+    // A column's two lanes follow their own halves of the keys; where one of them finds its bound passed, both agree anew.
+    float m = -INFINITY, limit = -INFINITY, l = 0.0f, top = 0.0f, ref = 0.0f;  // limit: the product that is a score of m + TH
     int lf = 0;
     a8_f16 o[DT];
 #pragma unroll
@@ -583,12 +590,11 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
-        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])) * qs;
-        if (__any(mx > m + TH)) {  // (uniform)
-            const float mn = fmaxf(m, mx);
+        if (__any(mx > limit)) {  // (uniform)
+            const float mn = fmaxf(m, a8_max_halves(mx) * qs);
             rescale(mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn));
             m = mn;
+            limit = (m + TH) / qs;
             ref = (m == -INFINITY ? 0.0f : m) - (float)lf;
         }
     };
@@ -618,9 +624,9 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
         });
         a8_unroll<EK>([&](auto e) { add(std::integral_constant<int, 16 - EK + e>{}); });
         l = fmaf(ps, a8_pow2(-lf), l);
-        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(wm), __float_as_uint(wm), false, false);
-        top = fmaxf(top, fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
-        if (__any(top > 0.0f && !(top >= 512.0f && top < 32768.0f))) {  // (uniform)
+        top = fmaxf(top, wm);
+        if (__any(__float_as_uint(top) - 0x44000000u >= 0x03000000u)) {  // (uniform) not in [2^9, 2^15)
+            top = a8_max_halves(top);
             if (!(top < INFINITY)) l = __uint_as_float(0x7FC00000u);  // values past 2^119: no number rather than a wrong one
             // top·2^d in [2^10, 2^11), as far as p·2^lf keeps clear of overflow (p·sv above 2^-90)
             const int d = top > 0.0f && top < INFINITY ? min(max(a8_exponent(top) - 12 + lf, -120), 100) - lf : 0;
