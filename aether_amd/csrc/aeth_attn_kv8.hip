@@ -578,6 +578,14 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) o[dt] *= al;
     };
+    auto shift = [&](int d) {  // lf becomes lf + d
+        const float al = a8_pow2(d);
+        top *= al;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) o[dt] *= al;
+        lf += d;
+        ref = (m == -INFINITY ? 0.0f : m) - (float)lf;
+    };
     // s, times its K scales, is a step's scores: masks them and follows their maximum
     auto bound_scores = [&](int k0) {
         if (k0 < all_lo || k0 + 32 > all_hi) {  // (uniform) some key is masked
@@ -604,6 +612,9 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
     auto step = [&](int b3, int T, const char* kp, int nb3, int nT, auto between) {
         const float sv = scales(b3, T, 1);
         a8_h8 kf[2] = {*(const a8_h8*)kp, *(const a8_h8*)(kp + KF)};
+        // p is below 2^(lf + TH + 1), lf at most 100: p·sv below 2^127 up to these V scales, and for any with lf at -10, from where
+        // it goes up again as the products are seen (1 % of the time, whether it is ever so or not)
+        if (__any(sv > 0x1p18f)) shift(min(0, -10 - lf));  // (uniform)
         sn = (a8_f16){};
         float wm = 0.0f, ps = 0.0f;
         auto add = [&](auto at) {
@@ -627,17 +638,11 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
         top = fmaxf(top, wm);
         if (__any(__float_as_uint(top) - 0x44000000u >= 0x03000000u)) {  // (uniform) not in [2^9, 2^15)
             top = a8_max_halves(top);
-            if (!(top < INFINITY)) l = __uint_as_float(0x7FC00000u);  // values past 2^119: no number rather than a wrong one
             // top·2^d in [2^10, 2^11), as far as p·2^lf keeps clear of overflow (p·sv above 2^-90)
-            const int d = top > 0.0f && top < INFINITY ? min(max(a8_exponent(top) - 12 + lf, -120), 100) - lf : 0;
-            const float al = a8_pow2(min(max(d, -126), 126));
-            top *= al;
+            const int d = top > 0.0f ? min(max(min(max(a8_exponent(top) - 12 + lf, -120), 100) - lf, -126), 126) : 0;
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) o[dt] *= al;
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[i] *= al;
-            lf += min(max(d, -126), 126);
-            ref = (m == -INFINITY ? 0.0f : m) - (float)lf;
+            for (int i = 0; i < 16; i++) s[i] *= a8_pow2(d);
+            shift(d);
         }
         between();
         const char* vp = vb[b3] + 2 * T * 1024 + lane * 16;
