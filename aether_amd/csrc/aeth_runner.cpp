@@ -280,6 +280,17 @@ int enqueue_step(aeth_runner* r) {
 int set_state(aeth_runner* r, int token, int pos);
 int step_results(aeth_runner* r, float* logits, int32_t* next_token);
 
+// The rows of a prompt that go through the layers at once: over an 8-bit cache, whose attention takes queries behind a cached
+// past, as many as every product takes (rows·k of 2^29 in the GEMMs, 65535 rows elsewhere), in passes of about the same size.
+int64_t prefill_pass_rows(const aeth_runner* r, int64_t n) {
+    const aeth_llama_config& c = r->cfg;
+    if (!r->kv8) return n;
+    const int64_t k = std::max<int64_t>({c.d_model, (int64_t)c.num_heads * c.head_dim, c.d_ff});
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(65535, ((int64_t)1 << 29) / k) / 256) * 256;
+    if (n <= most) return n;
+    return aeth_cdiv(aeth_cdiv(n, aeth_cdiv(n, most)), 256) * 256;
+}
+
 // Batched prefill (forward_batch, runner.rs:833-993; LlamaRunner::prefill :695-704):
 // tokens at positions 0..n-1, K/V at cache slots 0..n-1, per layer
 //   xn = rmsnorm(x, attn_norm); qkv = xn · Wqkvᵀ (GEMM, m = n); RoPE + cache write;
@@ -308,22 +319,15 @@ int ensure_prefill_buffers(aeth_runner* r, int64_t n) {
     }
     int rc = dmalloc(&r->p_tok, n);
     if (rc) return rc;
-    if (r->kv8 && (rc = dmalloc((uint8_t**)&r->p_a8_ws, aeth_attn_kv8_ws(1, n, c.num_heads, c.num_kv_heads, c.head_dim, n)))) return rc;
+    if (r->kv8 && (rc = dmalloc((uint8_t**)&r->p_a8_ws, aeth_attn_kv8_ws(1, n, c.num_heads, c.num_kv_heads, c.head_dim, c.max_seq_len)))) return rc;
     r->p_cap = n;
     return AETH_OK;
 }
 
-int runner_prefill_locked(aeth_runner* r, const int32_t* tokens, int32_t n, float* logits, int32_t* next_token) {
+// The n tokens at positions first .. first + n - 1 through every layer; first is 0 over the f32 cache
+int prefill_pass(aeth_runner* r, const int32_t* tokens, int64_t first, int64_t n) {
     const aeth_llama_config& c = r->cfg;
-    if (!tokens || n <= 0) return aeth_set_error(AETH_EINVAL, "prefill: empty prompt");
-    if (n > c.max_seq_len)
-        return aeth_set_error(AETH_EINVAL, "prefill: %d tokens exceed max_seq %d", n, c.max_seq_len);
-    for (int32_t i = 0; i < n; i++)
-        if (tokens[i] < 0 || tokens[i] >= c.vocab_size)
-            return aeth_set_error(AETH_EINVAL, "prefill: token %d out of range [0, %d)", tokens[i], c.vocab_size);
-    int rc = ensure_prefill_buffers(r, n);
-    if (rc) return rc;
-    r->partial_valid = false;
+    int rc;
     hipStream_t s = r->stream;
     const int64_t d = c.d_model, hd = c.head_dim, nh = c.num_heads, nkv = c.num_kv_heads, dff = c.d_ff;
     AETH_HIP_CHECK(hipMemcpyAsync(r->p_tok, tokens, sizeof(int32_t) * n, hipMemcpyHostToDevice, s));
@@ -369,11 +373,11 @@ int runner_prefill_locked(aeth_runner* r, const int32_t* tokens, int32_t n, floa
         const int64_t row = (nh + 2 * nkv) * hd;
         if (r->kv8) {
             uint8_t* lkv = r->kv8 + l * kv8_layer_bytes(c);
-            if ((rc = aeth_qk_norm_rope_launch(r->p_qkv, row, n, nh, nkv, hd, nullptr, nullptr, 0.0f, 0, nullptr, r->rope_sin,
+            if ((rc = aeth_qk_norm_rope_launch(r->p_qkv, row, n, nh, nkv, hd, nullptr, nullptr, 0.0f, first, nullptr, r->rope_sin,
                                                r->rope_cos, c.max_seq_len, r->p_qkv, row, s)) ||
                 (rc = aeth_kv8_append_launch(lkv, 0, nullptr, 1, r->p_qkv + nh * hd, r->p_qkv + (nh + nkv) * hd, row, hd, n, nkv,
-                                             hd, c.max_seq_len, 0, s)) ||
-                (rc = aeth_attn_kv8_launch(r->p_qkv, row, lkv, 0, nullptr, 0, 1, n, nh, nkv, hd, c.max_seq_len, n,
+                                             hd, c.max_seq_len, first, s)) ||
+                (rc = aeth_attn_kv8_launch(r->p_qkv, row, lkv, 0, nullptr, 0, 1, n, nh, nkv, hd, c.max_seq_len, first + n,
                                            c.sliding_window, r->p_att, r->p_a8_ws, s)))
                 return rc;
         } else {
@@ -422,8 +426,28 @@ int runner_prefill_locked(aeth_runner* r, const int32_t* tokens, int32_t n, floa
                                      : aeth_qmatmul(r->wdown[l], h, n, r->p_x, AETH_MM_ACCUMULATE, s);
         if (rc) return rc;
     }
+    return AETH_OK;
+}
+
+int runner_prefill_locked(aeth_runner* r, const int32_t* tokens, int32_t n, float* logits, int32_t* next_token) {
+    const aeth_llama_config& c = r->cfg;
+    if (!tokens || n <= 0) return aeth_set_error(AETH_EINVAL, "prefill: empty prompt");
+    if (n > c.max_seq_len)
+        return aeth_set_error(AETH_EINVAL, "prefill: %d tokens exceed max_seq %d", n, c.max_seq_len);
+    for (int32_t i = 0; i < n; i++)
+        if (tokens[i] < 0 || tokens[i] >= c.vocab_size)
+            return aeth_set_error(AETH_EINVAL, "prefill: token %d out of range [0, %d)", tokens[i], c.vocab_size);
+    const int64_t rows = prefill_pass_rows(r, n);
+    int rc = ensure_prefill_buffers(r, rows);
+    if (rc) return rc;
+    r->partial_valid = false;
+    int64_t first = 0, m = 0;
+    for (; first < n; first += m) {
+        m = std::min(rows, n - first);
+        if ((rc = prefill_pass(r, tokens + first, first, m))) return rc;
+    }
     // head on the last row; the state update then leaves pos = fill = n
-    AETH_HIP_CHECK(hipMemcpyAsync(r->x, r->p_x + (int64_t)(n - 1) * d, sizeof(float) * d, hipMemcpyDeviceToDevice, s));
+    AETH_HIP_CHECK(hipMemcpyAsync(r->x, r->p_x + (m - 1) * c.d_model, sizeof(float) * c.d_model, hipMemcpyDeviceToDevice, r->stream));
     r->fill = n - 1;
     if ((rc = set_state(r, tokens[n - 1], n - 1))) return rc;
     if ((rc = enqueue_head(r))) return rc;

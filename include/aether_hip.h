@@ -450,7 +450,9 @@ AETH_API int aeth_runner_decode(aeth_runner* r, int32_t token, int32_t pos, floa
 /* Batched prefill (LlamaRunner::prefill, runner.rs:695-704 → forward_batch,
  * :833-993): the n prompt tokens (host) are placed at positions 0..n-1 in
  * one pass (GEMM projections, causal attention_batch :1809-1883), K/V written
- * to cache slots 0..n-1, and the cache fill becomes n. logits (host, vocab
+ * to cache slots 0..n-1, and the cache fill becomes n. Over an 8-bit cache a
+ * prompt of more rows than the products take (37376 at d_ff 14336, 65280 at
+ * most) goes in several passes. logits (host, vocab
  * floats) receive the last token's logits and next_token its greedy argmax;
  * either may be NULL. 1 <= n <= max_seq_len. */
 AETH_API int aeth_runner_prefill(aeth_runner* r, const int32_t* tokens, int32_t n, float* logits,
