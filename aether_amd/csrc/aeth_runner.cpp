@@ -441,6 +441,7 @@ int runner_prefill_locked(aeth_runner* r, const int32_t* tokens, int32_t n, floa
     int rc = ensure_prefill_buffers(r, rows);
     if (rc) return rc;
     r->partial_valid = false;
+    r->fill = 0;  // an error from here on leaves slots of both sequences: none of them counts
     int64_t first = 0, m = 0;
     for (; first < n; first += m) {
         m = std::min(rows, n - first);
@@ -448,8 +449,7 @@ int runner_prefill_locked(aeth_runner* r, const int32_t* tokens, int32_t n, floa
     }
     // head on the last row; the state update then leaves pos = fill = n
     AETH_HIP_CHECK(hipMemcpyAsync(r->x, r->p_x + (m - 1) * c.d_model, sizeof(float) * c.d_model, hipMemcpyDeviceToDevice, r->stream));
-    r->fill = n - 1;
-    if ((rc = set_state(r, tokens[n - 1], n - 1))) return rc;
+    if ((rc = aeth_state_set_launch(r->st, tokens[n - 1], n - 1, n - 1, r->stream))) return rc;
     if ((rc = enqueue_head(r))) return rc;
     if ((rc = step_results(r, logits, next_token))) return rc;
     r->fill = n;

@@ -454,7 +454,9 @@ AETH_API int aeth_runner_decode(aeth_runner* r, int32_t token, int32_t pos, floa
  * prompt of more rows than the products take (37376 at d_ff 14336, 65280 at
  * most) goes in several passes. logits (host, vocab
  * floats) receive the last token's logits and next_token its greedy argmax;
- * either may be NULL. 1 <= n <= max_seq_len. */
+ * either may be NULL. 1 <= n <= max_seq_len. An error behind the first write
+ * leaves an empty cache (aeth_runner_seq_len 0), one of the arguments the cache
+ * as it was. */
 AETH_API int aeth_runner_prefill(aeth_runner* r, const int32_t* tokens, int32_t n, float* logits,
                                  int32_t* next_token);
 /* Greedy decode of n_steps tokens starting from `token` at `pos`; tokens

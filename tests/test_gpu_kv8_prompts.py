@@ -92,3 +92,25 @@ def test_prompts_of_two_passes(gpu, n, dff, layers, dtype):
         assert_close_logits(prefill(r, c, tokens[:100]), exact_run(gpu, c, m, tokens[:100])[1], floor=FLOOR, what="100 tokens")
     finally:
         A.lib().aeth_runner_free(r)
+
+
+def test_a_prompt_refused_midway_leaves_no_sequence(gpu):
+    """Over the f32 cache, whose attention takes a prompt whole, the products of the first test still refuse it, in layer 0 and behind
+    that layer's writes: no slot counts then, and the next sequence is as on a new runner."""
+    L = A.lib()
+    c = dict(TINY, max_seq_len=8192, num_heads=2, num_kv_heads=1, num_layers=1, d_ff=66048, flags=A.CFG_FULL_CONTEXT)
+    r = make_runner(build_tiny(seed=32, c=c), c)
+    tokens = np.random.default_rng(10).integers(0, c["vocab_size"], 8192).astype(np.int32)
+    try:
+        first = prefill(r, c, tokens[:100])
+        assert L.aeth_runner_seq_len(r) == 100
+        assert L.aeth_runner_prefill(r, tokens.ctypes.data, 8192, None, None) == A.AETH_EINVAL
+        assert L.aeth_runner_seq_len(r) == 0 and cache_of(r, c)[1] == 0
+        # arguments refused before anything is written leave the sequence as it is
+        assert np.array_equal(prefill(r, c, tokens[:100]), first)
+        assert L.aeth_runner_prefill(r, tokens.ctypes.data, 8193, None, None) == A.AETH_EINVAL
+        tokens[50] = c["vocab_size"]
+        assert L.aeth_runner_prefill(r, tokens.ctypes.data, 60, None, None) == A.AETH_EINVAL
+        assert L.aeth_runner_seq_len(r) == 100
+    finally:
+        L.aeth_runner_free(r)
