@@ -734,9 +734,9 @@ extern "C" AETH_API int aeth_runner_fill_kv(aeth_runner* r, uint64_t seed, int32
     if (r->kv8) {
         // the f32 cache's numbers of the first seq_len positions, quantised; the rest cleared
         const int64_t nkv = c.num_kv_heads, hd = c.head_dim, ms = c.max_seq_len, lf = kv_layer_floats(c);
-        AETH_HIP_CHECK(hipMemsetAsync(r->kv8, 0, (size_t)(c.num_layers * kv8_layer_bytes(c)), r->stream));
-        LayerCopy f(lf);
+        LayerCopy f(lf);  // before anything is touched
         if (!f.p) return aeth_set_error(AETH_ENOMEM, "aeth_runner_fill_kv: no memory for a layer in f32");
+        AETH_HIP_CHECK(hipMemsetAsync(r->kv8, 0, (size_t)(c.num_layers * kv8_layer_bytes(c)), r->stream));
         for (int l = 0; l < c.num_layers; l++) {
             int rc = aeth_fill_normal_launch(seed, f.p, l * lf, lf, 0.0f, 1.0f, r->stream);
             if (rc || (rc = aeth_kv8_append_launch(r->kv8 + l * kv8_layer_bytes(c), 0, nullptr, 1, f.p, f.p + lf / 2, hd, ms * hd, seq_len,

@@ -11,7 +11,7 @@ from oracle import oracle as O
 from tests import _kv8 as R
 from tests._model64 import _deq
 from tests._models import TINY, build_tiny
-from tests._util import Q4_K, Q8_0, assert_close_logits
+from tests._util import Q2_K, Q4_K, Q8_0, assert_close_logits
 from tests.test_gpu_decode import make_runner
 from tests.test_gpu_kv8_runner import FLOOR, cache_of, prefill
 
@@ -114,3 +114,26 @@ def test_a_prompt_refused_midway_leaves_no_sequence(gpu):
         assert L.aeth_runner_seq_len(r) == 100
     finally:
         L.aeth_runner_free(r)
+
+
+def test_a_fill_without_memory_leaves_the_cache(gpu):
+    """aeth_runner_fill_kv quantises a layer at a time out of an f32 copy; one of 2400 heads over 131072 positions is 322 GB, which no
+    GPU here has. The sequence in the cache goes on as if the call had not been."""
+    L = A.lib()
+    cfg = A.LlamaConfig(vocab_size=512, d_model=256, num_layers=1, num_heads=2400, num_kv_heads=2400, head_dim=128, d_ff=512, max_seq_len=1 << 17,
+                        rope_base=10000.0, rms_norm_eps=1e-5, sliding_window=0, flags=LONG)
+    got = []
+    for fill in (False, True):
+        r = ctypes.c_void_p()
+        A.check(L.aeth_runner_create(ctypes.byref(cfg), None, (ctypes.c_int32 * 7)(*([Q4_K] * 3 + [Q2_K] + [Q4_K] * 3)), None, None, None, Q4_K, None, 5, ctypes.byref(r)), "create")
+        try:
+            logits = np.empty(512, np.float32)
+            A.check(L.aeth_runner_decode(r, 3, 0, None, None), "decode")
+            if fill:
+                assert L.aeth_runner_fill_kv(r, 5, 1000) == A.AETH_ENOMEM
+            assert L.aeth_runner_seq_len(r) == 1
+            A.check(L.aeth_runner_decode(r, 4, 1, logits.ctypes.data, None), "decode")
+            got.append(logits)
+        finally:
+            L.aeth_runner_free(r)
+    assert np.array_equal(got[0], got[1])
