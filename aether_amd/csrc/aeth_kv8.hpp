@@ -59,7 +59,8 @@ __device__ __forceinline__ double kv8_inverse(float amax) {
     return 127.0 * r;
 }
 
-// rint(127·x / amax): the quotient of two f32 is a tie or at least 2^-26 away from one, so the f64
+// rint(127·x / amax): with amax = A·2^a, A below 2^24, and x = X·2^(a - s) a tie's distance |127·X / (A·2^s) - (i + 1/2)| is 0 or at
+// least 1 / (A·2^max(s, 1)). Quotients of a half and more have s up to 8: 2^-32 (smaller ones are far from a tie). So the f64
 // product (off by under 2^-42) rounded to a multiple of 2^-40 is a tie exactly where the quotient is.
 __device__ __forceinline__ uint32_t kv8_code(float x, double inv) {
     const double t = (double)x * inv;
