@@ -28,3 +28,24 @@ def test_values_that_rise(gpu, n, seq, heads, nkv, hd, window, run, low, high):
         got = attend(torch, q, layer, nkv, hd, slots, seq, window)
         want, bound = R.attention(q, layer, nkv, hd, slots, seq, window)
         within(torch, got, want, bound)
+
+
+@pytest.mark.parametrize("n,seq,heads,nkv,hd", [(1, 131000, 4, 1, 128), (1, 9000, 32, 8, 128), (5, 9000, 4, 2, 256), (70, 9001, 16, 8, 128), (250, 8448, 32, 8, 128),
+                                                (100, 7100, 64, 8, 128), (100, 7100, 32, 8, 128), (600, 7600, 7, 1, 64), (333, 20333, 8, 8, 128), (2500, 2500, 64, 8, 128)])
+def test_low_bits_of_the_products_over_long_rows(gpu, n, seq, heads, nkv, hd):
+    """Flat scores; the tokens' values are c and -c in turn, of scales 1 + 2^-13 and 1, so that the result, c·2^-14, is what is left of
+    bits that half a product's number of bits does not hold. Each product may be rounded to 2^-23 of itself (include/aether_hip.h),
+    c·2^-23 a token of the mean; what the 16 products of a matrix instruction and the running sum, never above 16·c and 2·c,
+    lose over it is (2·16·U/16 + 2·2·U/4)·c = 3·U·c a token, three roundings of the result 3·U of it: 2^-21·c covers them and the
+    last token of an odd row."""
+    torch = gpu
+    slots = -(-seq // 64) * 64
+    t = torch.arange(slots, device="cuda")
+    c = 1 + torch.arange(hd, device="cuda") % 31
+    vc = (torch.where(t % 2 == 0, 1, -1)[:, None] * c).to(torch.int8).expand(nkv, slots, hd).contiguous()
+    vs = torch.where(t % 2 == 0, 1.0 + 2.0 ** -13, 1.0).float().expand(nkv, slots).contiguous()
+    layer = R.pack(torch.zeros_like(vc), torch.zeros_like(vs), vc, vs)
+    q = rand(torch, 123, n, heads * hd)
+    got = attend(torch, q, layer, nkv, hd, slots, seq)
+    want, _ = R.attention(q, layer, nkv, hd, slots, seq, 0)
+    within(torch, got, want, (2.0 ** -21 * c.double()).repeat(heads).expand(n, -1))
