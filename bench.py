@@ -276,6 +276,43 @@ def bench_decode_eager(torch, A, n_tokens=128, prefilled=2048):
             "first_tokens": list(toks)[:8]}
 
 
+def bench_kv_cache(A, n_tokens=96):
+    """bench_decode's model over an f32 and an 8-bit key/value cache: microseconds a decode step (graph replays, the
+    best of three runs of n_tokens steps) for cache sizes and fills, milliseconds for a 4000-token prompt (the best of
+    three). Not in the default sections."""
+    L = A.lib()
+    out = {}
+    prompt = (ctypes.c_int32 * 4000)(*[i % 1000 for i in range(4000)])
+    for max_seq, fills in ((4096, (2048,)), (8192, (8000,)), (65536, (65000,)), (131072, (2048, 8000)), (1 << 20, (2048, 8000))):
+        for name, flag in (("f32", 0), ("int8", A.CFG_KV_INT8)):
+            if max_seq > 8192 and not flag:
+                continue
+            cfg = A.LlamaConfig(vocab_size=128256, d_model=4096, num_layers=32, num_heads=32, num_kv_heads=8, head_dim=128, d_ff=14336,
+                                max_seq_len=max_seq, rope_base=500000.0, rms_norm_eps=1e-5, flags=flag | A.CFG_FULL_CONTEXT)
+            r = ctypes.c_void_p()
+            A.check(L.aeth_runner_create(ctypes.byref(cfg), None, (ctypes.c_int32 * 224)(*([12] * 224)), None, None, None, 14, None, 0x8B8B8B,
+                                         ctypes.byref(r)), "runner_create")
+            toks = (ctypes.c_int32 * n_tokens)()
+            for fill in fills:
+                best = float("inf")
+                for i in range(4):  # the first captures the graph
+                    A.check(L.aeth_runner_fill_kv(r, 0x4B56, fill), "fill_kv")
+                    t0 = time.perf_counter()
+                    A.check(L.aeth_runner_generate(r, 1, fill, n_tokens, toks, 1), "generate")
+                    best = min(best, time.perf_counter() - t0) if i else best
+                out["%s_cache_%d_filled_%d_us" % (name, max_seq, fill)] = round(best / n_tokens * 1e6, 1)
+            if max_seq == 4096:
+                best = float("inf")
+                for i in range(4):
+                    t0 = time.perf_counter()
+                    A.check(L.aeth_runner_prefill(r, prompt, 4000, None, None), "prefill")
+                    best = min(best, time.perf_counter() - t0) if i else best
+                out["%s_prompt_4000_ms" % name] = round(best * 1e3, 2)
+            L.aeth_runner_free(r)
+            print("[bench] kv_cache: %s" % out, file=sys.stderr, flush=True)
+    return out
+
+
 def export_decode_model(A, r, cfg, prefilled, tokens):
     """Host copies of what the CPU decode step reads: every layer weight (raw
     GGUF row blocks), the norms, the LM head, the KV cache refilled to
@@ -502,7 +539,8 @@ def main():
                     help="comma-separated extra sections to run: floor, q8, q6, boundary (host-slice calls; after q6), "
                          "q5, dotprod, gemm, gemm_q8, gemm_q6k, gemm_q5k, gemm_q80, "
                          "decode, q4_k_m, q8_0_model (default), f16, q2k (GGUF-order formats), decode_eager (the decode step "
-                         "without its HIP graph; these three not run by default)")
+                         "without its HIP graph), kv_cache (decode and a prompt over f32 and 8-bit caches; these four not "
+                         "run by default)")
     ap.add_argument("--cpu-seconds", type=float, default=10.0)
     ap.add_argument("--calib-copy-mib", type=int, default=0,
                     help="also run one device-to-device copy of this many MiB (HBM counter calibration under rocprofv3)")
@@ -689,6 +727,9 @@ def main():
         extra["decode_8b_q4k_eager"] = {"tok/s": round(d["tok_s"], 1), "ms_per_token": round(d["ms_per_token"], 4),
                                         "tokens": d["tokens"], "prefilled": 2048, "first_tokens": d["first_tokens"]}
         print("[bench] decode 8B eager: %s" % extra["decode_8b_q4k_eager"], file=sys.stderr, flush=True)
+
+    if "kv_cache" in sections:  # not a default section: the cache in 8 bits beside the f32 one
+        extra["kv_cache_8b_q4k"] = bench_kv_cache(A)
 
     cpu = None
     if not args.no_cpu:
