@@ -49,3 +49,22 @@ def test_low_bits_of_the_products_over_long_rows(gpu, n, seq, heads, nkv, hd):
     got = attend(torch, q, layer, nkv, hd, slots, seq)
     want, _ = R.attention(q, layer, nkv, hd, slots, seq, 0)
     within(torch, got, want, (2.0 ** -21 * c.double()).repeat(heads).expand(n, -1))
+
+
+@pytest.mark.parametrize("n,seq,heads,nkv,hd,window", SHAPES)
+def test_the_ends_of_the_numbers(gpu, n, seq, heads, nkv, hd, window):
+    """Keys up to 2^95 and down to 2^-100 with queries that leave scores of ordinary size, scores up to about 2^20, and values whose sum
+    of e^(score - maximum)·|value| stays below 2^119 (tokens times 2^5, what `rand` stays below)."""
+    torch = gpu
+    slots = -(-seq // 64) * 64
+    base, val = rand(torch, 124, nkv, slots, hd), rand(torch, 125, nkv, slots, hd)
+    q = rand(torch, 126, n, heads * hd)
+    assert base.abs().max() < 16 and val.abs().max() < 32  # keys below 16·2^91 = 2^95, sums below 32·2^(118 - 4) = 2^119
+    most = 2.0 ** (118 - 4 - (seq - 1).bit_length())
+    for kf, qf, vf in ((2.0 ** 91, 2.0 ** -91, 1.0), (2.0 ** -100, 2.0 ** 100, 1.0), (2.0 ** 8, 2.0 ** 8, 1.0), (1.0, 1.0, most), (0.0, 1.0, most),
+                       (1.0, 1.0, 2.0 ** -60)):
+        layer = R.pack(*R.codes(base * kf), *R.codes(val * vf))
+        qs = q * qf
+        got = attend(torch, qs, layer, nkv, hd, slots, seq, window)
+        want, bound = R.attention(qs, layer, nkv, hd, slots, seq, window)
+        within(torch, got, want, bound)
