@@ -8,7 +8,9 @@
 // as integers of 24 bits, three balanced base-256 digits d2·65536 + d1·256 + d0 with d in [-128, 127]:
 // three int8 products whose i32 sums are exact. So
 //  * a score carries q rounded to 2^-23 of its row's largest component (|q·2^e| in [2^22, 2^23)), as
-//    keys are held to 2^-8 of theirs, and nothing else but the f32 roundings of its final products;
+//    keys are held to 2^-8 of theirs, and nothing else but the f32 roundings of its final products. More
+//    digits would cost a third more products; where a fourth of q is 30 times larger and of the keys
+//    30 times smaller it costs four times f32's error (4.7e-6 of the result over 2049 tokens), else none;
 //  * p·sv (the probability times the token's V scale) is rounded to 2^-23 of the largest of its column
 //    in a tile of 64 tokens, whatever the running maximum: neither a flat row nor a tile far below
 //    the maximum loses bits. Tiles are summed in f32.
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
         });
         l += ps;
         wm = aeth_max_rows(wm);
-        if (!(wm < INFINITY)) l = __uint_as_float(0x7FC00000u);  // values past 2^119: no number rather than a wrong one
+        if (!(wm < INFINITY)) l = __uint_as_float(0x7FC00000u);  // p (below 2^9) times V past f32: no number rather than a wrong one
         const int j2 = a8_exponent(wm);
         const float f = a8_pow2(j2), fi = a8_pow2(-j2);
         a8_i4 pd[3];
@@ -423,9 +425,10 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
 // the order in which V's operand takes its tokens (j = 2T + u, g = 2a + h of aeth_kv8.hpp), so the
 // probabilities stay in their lanes. The next tile's codes are loaded a tile ahead, converted and stored in
 // the other LDS buffer before this tile's products: one barrier a tile.
-// 32 / 8 heads of 128: 4000 tokens 253 µs (0.52 PFLOP/s of the formula, 1.04 of the matrix units'), 250 over 20000 161 with its
-// join. The matrix units are busy 49 % of the cycles, at 2.0 GHz, the vector units 44 %: of two waves a SIMD one is often
-// waiting for the other's instruction to leave the issue port (36 % of the waves' time) or for LDS and the barrier (30 %). The two
+// 32 / 8 heads of 128: 4000 tokens 253 µs (0.52 PFLOP/s of the formula, 1.04 of the matrix units'), 250 over 20000 159 with its
+// join. The matrix units are busy 49 % of the cycles, at 2.0 GHz, the vector units (their issue of matrix instructions with it)
+// 46 %: of two waves a SIMD one is often waiting for the other's instruction to leave the issue port (35 % of the waves' time) or
+// for LDS and the barrier (32 %). The two
 // phases of two waves kept apart by barriers, another priority for one of them, K a step ahead and reads from LDS further
 // ahead took as long or longer.
 typedef _Float16 a8_h8 __attribute__((ext_vector_type(8)));
@@ -868,8 +871,10 @@ Form a8_form(int64_t seqs, int64_t n, int64_t G, int64_t nkv, int64_t hd, int64_
     const int64_t cus = aeth_num_cus(), cols = n * G, heads = seqs * nkv;
     auto span = [&](int64_t cw) { return a8_span(cw, n, G, max_len, window); };
     auto units = [&](int64_t cw) { return heads * aeth_cdiv(cols, cw); };
-    // 16 columns: split until two workgroups a CU have work; four, where the device alone knows the length; not up to 512
-    // tokens, two tiles a wave (a token over 300: 7.8 µs, 8.4 in two chunks; over 600: 9.7, 8.9 in three)
+    // 16 columns: split until two workgroups a CU have work; four, where the device alone knows the length, so that one below it has
+    // work for more (a decode step's layer of a small model, its products included, one / two / four a CU: 4000 tokens in a cache of
+    // their size 26.6 / 26.7 / 26.6 µs, 8000 28.8 / 27.0 / 27.0, 131000 72.5 / 73.1 / 79.0); not up to 512 tokens, two tiles a wave (a token over
+    // 300: 7.8 µs, 8.4 in two chunks; over 600: 9.7, 8.9 in three)
     const Form small = a8_split(16, units(16), span(16), span(16) <= 8 ? 1 : (ragged ? 4 : 2) * cus, 4);
     if (ragged && seqs > 1) {
         // A batch: the least, in µs, of 5 + ((0.34·tpc)^1.5 + max(MB / 6.4, 1.5·r)^1.5)^(2/3) + 0.2·wgs/CU, and where it is split 2.2 +
@@ -894,6 +899,10 @@ Form a8_form(int64_t seqs, int64_t n, int64_t G, int64_t nkv, int64_t hd, int64_
         }
         return best;
     }
+    // Up to 64 columns half of the smallest of the other forms has none (64 columns over 1000 / 5000 / 30000 tokens: 10.0 / 15.4 /
+    // 34.6 µs, with 128 columns 26 / 27 / 42 at best; at head_dim 64 7.7 / 10.7 / 22.2, 19 / 20 / 30). A call whose length the device
+    // alone knows has at most 64 (one query a sequence) but for more query heads a KV head than that; head_dim 256 has no other
+    // form (4 query heads each: a 512-token prompt 46 µs, 2000 tokens 301, a token over 30000 34).
     if (hd > 128 || cols <= 64 || ragged) return small;
     // Otherwise the least of what the forms take, in µs on a CU's share of the tiles (w; q: the fullest CU's of few workgroups),
     // its workgroups' rounds (r: three at once, four) and the tiles of one (tpc), at head_dim 128 (64):
