@@ -117,8 +117,8 @@ def test_a_prompt_refused_midway_leaves_no_sequence(gpu):
 
 
 def test_a_fill_without_memory_leaves_the_cache(gpu):
-    """aeth_runner_fill_kv quantises a layer at a time out of an f32 copy; one of 2400 heads over 131072 positions is 322 GB, which no
-    GPU here has. The sequence in the cache goes on as if the call had not been."""
+    """aeth_runner_fill_kv quantises a layer at a time out of an f32 copy; one of 2400 heads over 131072 positions is 322 GB, more than the
+    GPU has. The sequence in the cache goes on as if the call had not been."""
     L = A.lib()
     cfg = A.LlamaConfig(vocab_size=512, d_model=256, num_layers=1, num_heads=2400, num_kv_heads=2400, head_dim=128, d_ff=512, max_seq_len=1 << 17,
                         rope_base=10000.0, rms_norm_eps=1e-5, sliding_window=0, flags=LONG)

@@ -68,3 +68,22 @@ def test_the_ends_of_the_numbers(gpu, n, seq, heads, nkv, hd, window):
         got = attend(torch, qs, layer, nkv, hd, slots, seq, window)
         want, bound = R.attention(qs, layer, nkv, hd, slots, seq, window)
         within(torch, got, want, bound)
+
+
+@pytest.mark.parametrize("n,seq,heads,nkv,hd,window", [(1000, 4000, 32, 2, 128, 600), (600, 1600, 64, 8, 64, 700), (600, 1600, 64, 8, 128, 700), (800, 3000, 48, 2, 128, 65)])
+def test_uneven_rows_under_a_window(gpu, n, seq, heads, nkv, hd, window):
+    """Many columns over scores that rise and fall by hundreds from tile to tile, flat ones, and V scales that mix, fall or are
+    large, where every tile has keys that some column does not see. Values of 1e-30 have scales of 2^-104, and products below
+    2^-90 keep fewer bits (include/aether_hip.h): times 2^100, the most that a probability below 2^9 bears beside any V scale up to
+    2^18, they stand in two parts whose last place is fp16's 2^-24, so that each is off by up to 2^-125 and a row by
+    127 · window · 2^-125, its sum of probabilities being 1 or more."""
+    torch = gpu
+    slots = -(-seq // 64) * 64
+    base, val = rand(torch, 127, nkv, slots, hd), rand(torch, 128, nkv, slots, hd)
+    q = rand(torch, 129, n, heads * hd)
+    t = torch.arange(slots, device="cuda").float()[None, :, None]
+    for k, v in ((base * (1.0 + t / 20.0), val), (base * (1.0 + (seq - t).clamp_min(0) / 20.0), val), (base * 0.0, val),
+                 (base * 1e-3, val * torch.pow(10.0, (t % 41) - 20.0)), (base, val * torch.pow(10.0, -t / 50.0).clamp_min(1e-30)), (base, val * 1e30)):
+        layer = R.pack(*R.codes(k), *R.codes(v))
+        want, bound = R.attention(q, layer, nkv, hd, slots, seq, window)
+        within(torch, attend(torch, q, layer, nkv, hd, slots, seq, window), want, bound + 127 * window * 2.0 ** -125)
