@@ -100,6 +100,17 @@ _SIGS = {
     "aeth_attn_kv8_ws_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64]),
     "aeth_attn_kv8": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
     "aeth_attn_kv8_batch": (_INT, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
+    "aeth_qk_norm_rope_axes": (_INT, [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, ctypes.c_float, _P, _I64, _I64, _P, _P, _P, _I64, _P, _I64,
+                                      _P]),
+    "aeth_attn_kv8_shared_ws_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "aeth_attn_kv8_shared": (_INT, [_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
+    "aeth_attn_kv8_weights_ws_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "aeth_attn_kv8_weights": (_INT, [_P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P]),
+    "aeth_attn_kv8_weights_batch": (_INT, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P]),
+    "aeth_kv8_evict_ws_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _INT]),
+    "aeth_kv8_evict": (_INT, [_P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _P]),
+    "aeth_kv8_evict_batch": (_INT, [_P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64,
+                                    _P]),
     "aeth_silu_mul": (_INT, [_P, _P, _I64, _P]),
     "aeth_add": (_INT, [_P, _P, _I64, _P]),
     "aeth_argmax": (_INT, [_P, _I64, _P, _P]),

@@ -28,7 +28,9 @@ SOURCES = [
     "aeth_prefill.hip",
     "aeth_backend.hip",
     "aeth_kv8.hip",
+    "aeth_kv8_evict.hip",
     "aeth_attn_kv8.hip",
+    "aeth_attn_kv8_serve.hip",
     "aeth_host.cpp",
     "aeth_blas.cpp",
     "aeth_runner.cpp",
@@ -55,6 +57,7 @@ EXTRA = {
     "aeth_gemm_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "aeth_gemm_gq.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "aeth_attn_kv8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "aeth_attn_kv8_serve.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 COMMON = [

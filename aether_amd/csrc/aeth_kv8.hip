@@ -10,6 +10,8 @@
 // what is there, and a prompt appended in pieces leaves the bytes of one appended whole.
 #include <math.h>
 
+#include <algorithm>
+
 #include "aeth_common.hpp"
 #include "aeth_internal.hpp"
 #include "aeth_kv8.hpp"
@@ -355,9 +357,18 @@ struct QkArgs {
     int nq, heads, hd;     // query heads; query and key heads
 };
 
+constexpr int QK_MAX_HD = 512, QK_MAX_AXES = 16;  // with several axes: the pairs' axes go as a kernel argument
+struct QkAxes {
+    int64_t pos_stride;                   // d_pos is [axes][pos_stride]
+    uint32_t axis[QK_MAX_HD / 2 / 4];     // the axis of each pair, a byte each
+};
+
 __device__ __forceinline__ int64_t qk_row(const QkArgs& A, int64_t i) {
     const int64_t p = A.d_pos ? (int64_t)A.d_pos[i] : A.pos + i;
     return min(max(p, (int64_t)0), A.max_seq - 1);
+}
+__device__ __forceinline__ int64_t qk_row(const QkArgs& A, const QkAxes& X, int64_t i, int axis) {
+    return min(max((int64_t)A.d_pos[axis * X.pos_stride + i], (int64_t)0), A.max_seq - 1);
 }
 
 // sum over aligned groups of L lanes (8, 16 or 32), the same value in each
@@ -375,8 +386,10 @@ __device__ __forceinline__ float qk_sum(float v) {
 }
 
 // hd / 8 lanes a head, four pairs a lane; rows, weights and tables 16-byte aligned
-template <int HD>
-__global__ void __launch_bounds__(256) k_qk_norm_rope_v(QkArgs A) {
+// Several axes (AXES): pair j's row of the tables is its axis' position of the token, so the four pairs of a lane take their
+// entries one by one. (The table's rows of a token serve all its heads from the cache.)
+template <int HD, bool AXES>
+__device__ __forceinline__ void qk_norm_rope_v(const QkArgs& A, const QkAxes& X) {
     constexpr int L = HD / 8, HALF = HD / 2;
     const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / L, all = (uint32_t)A.n * A.heads;  // at most 2^25 units
     const uint32_t u = min(unit, all - 1), row = u / (uint32_t)A.heads;  // past the end: loaded, not stored (whole waves stay active)
@@ -384,8 +397,18 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_v(QkArgs A) {
     const int h = (int)(u - row * A.heads), e = 4 * (threadIdx.x % L);
     const float* src = A.x + i * A.x_stride + (int64_t)h * HD + e;
     float4 a = *(const float4*)src, b = *(const float4*)(src + HALF);
-    const int64_t p = qk_row(A, i);
-    const float4 sn = *(const float4*)(A.sin_t + p * HALF + e), cs = *(const float4*)(A.cos_t + p * HALF + e);
+    float4 sn, cs;
+    if constexpr (AXES) {
+        const uint32_t axes = X.axis[e / 4];
+        int64_t at[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) at[j] = qk_row(A, X, i, axes >> (8 * j) & 0xFFu) * HALF + e + j;
+        sn = make_float4(A.sin_t[at[0]], A.sin_t[at[1]], A.sin_t[at[2]], A.sin_t[at[3]]);
+        cs = make_float4(A.cos_t[at[0]], A.cos_t[at[1]], A.cos_t[at[2]], A.cos_t[at[3]]);
+    } else {
+        const int64_t p = qk_row(A, i);
+        sn = *(const float4*)(A.sin_t + p * HALF + e), cs = *(const float4*)(A.cos_t + p * HALF + e);
+    }
     const float* w = h < A.nq ? A.qw : A.kw;
     if (A.qw || A.kw) {  // (uniform)
         const float4 wa = w ? *(const float4*)(w + e) : make_float4(1, 1, 1, 1), wb = w ? *(const float4*)(w + e + HALF) : wa;
@@ -402,15 +425,21 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_v(QkArgs A) {
     __builtin_nontemporal_store((kv8_f4){b.x, b.y, b.z, b.w}, (kv8_f4*)(dst + HALF));
 }
 
+template <int HD>
+__global__ void __launch_bounds__(256) k_qk_norm_rope_v(QkArgs A) { qk_norm_rope_v<HD, false>(A, {}); }
+template <int HD>
+__global__ void __launch_bounds__(256) k_qk_norm_rope_axes_v(QkArgs A, QkAxes X) { qk_norm_rope_v<HD, true>(A, X); }
+
 // any even hd, any alignment: a wave a head, lanes over the pairs (read again for the rotation: the row is in cache)
-__global__ void __launch_bounds__(256) k_qk_norm_rope(QkArgs A) {
+template <bool AXES>
+__device__ __forceinline__ void qk_norm_rope(const QkArgs& A, const QkAxes& X) {
     const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (unit >= A.n * A.heads) return;
     const int64_t i = unit / A.heads;
     const int h = (int)(unit % A.heads), lane = threadIdx.x & 63, half = A.hd / 2;
     const float* src = A.x + i * A.x_stride + (int64_t)h * A.hd;
     float* dst = A.out + i * A.out_stride + (int64_t)h * A.hd;
-    const int64_t p = qk_row(A, i);
+    const int64_t p = AXES ? 0 : qk_row(A, i);
     const float* w = h < A.nq ? A.qw : A.kw;
     float rms = 1.0f;
     if (w) {
@@ -419,7 +448,8 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(QkArgs A) {
         rms = sqrtf(aeth_wave_sum(ss) / (float)A.hd + A.eps);
     }
     for (int e = lane; e < half; e += 64) {
-        const float sn = A.sin_t[p * half + e], cs = A.cos_t[p * half + e];
+        const int64_t at = (AXES ? qk_row(A, X, i, X.axis[e >> 2] >> (8 * (e & 3)) & 0xFFu) : p) * half + e;
+        const float sn = A.sin_t[at], cs = A.cos_t[at];
         float a = src[e], b = src[e + half];
         if (w) {
             a = a / rms * w[e];
@@ -429,35 +459,50 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(QkArgs A) {
         dst[e + half] = kv8_rot1(a, b, sn, cs);
     }
 }
+__global__ void __launch_bounds__(256) k_qk_norm_rope(QkArgs A) { qk_norm_rope<false>(A, {}); }
+__global__ void __launch_bounds__(256) k_qk_norm_rope_axes(QkArgs A, QkAxes X) { qk_norm_rope<true>(A, X); }
 }  // namespace
+
+// X: several axes (nullptr: one)
+static int qk_launch(const QkArgs& A, const QkAxes* X, hipStream_t s) {
+    if (A.n <= 0 || A.heads <= 0) return AETH_OK;
+    const bool al16 = ((((uintptr_t)A.x | (uintptr_t)A.out | (uintptr_t)A.qw | (uintptr_t)A.kw | (uintptr_t)A.sin_t | (uintptr_t)A.cos_t) & 15) == 0) &&
+                      ((A.x_stride | A.out_stride) & 3) == 0;
+    const int hd = A.hd;
+    const dim3 block(256);
+    if (al16 && (hd == 64 || hd == 128 || hd == 256)) {
+        const dim3 grid((unsigned)aeth_cdiv(A.n * A.heads * (hd / 8), 256));
+        if (X) {
+            if (hd == 64) hipLaunchKernelGGL(k_qk_norm_rope_axes_v<64>, grid, block, 0, s, A, *X);
+            else if (hd == 128) hipLaunchKernelGGL(k_qk_norm_rope_axes_v<128>, grid, block, 0, s, A, *X);
+            else hipLaunchKernelGGL(k_qk_norm_rope_axes_v<256>, grid, block, 0, s, A, *X);
+        } else {
+            if (hd == 64) hipLaunchKernelGGL(k_qk_norm_rope_v<64>, grid, block, 0, s, A);
+            else if (hd == 128) hipLaunchKernelGGL(k_qk_norm_rope_v<128>, grid, block, 0, s, A);
+            else hipLaunchKernelGGL(k_qk_norm_rope_v<256>, grid, block, 0, s, A);
+        }
+    } else {
+        const dim3 grid((unsigned)aeth_cdiv(A.n * A.heads, 4));
+        if (X) hipLaunchKernelGGL(k_qk_norm_rope_axes, grid, block, 0, s, A, *X);
+        else hipLaunchKernelGGL(k_qk_norm_rope, grid, block, 0, s, A);
+    }
+    AETH_LAUNCH_CHECK();
+    return AETH_OK;
+}
 
 int aeth_qk_norm_rope_launch(const float* x, int64_t x_stride, int64_t n, int64_t n_heads, int64_t kv_heads, int64_t hd,
                              const float* qw, const float* kw, float eps, int64_t pos, const int* d_pos, const float* sin_t,
                              const float* cos_t, int64_t max_seq, float* out, int64_t out_stride, hipStream_t s) {
     const int64_t heads = n_heads + kv_heads;
     if (n <= 0 || heads <= 0) return AETH_OK;
-    QkArgs A{x, x_stride, out, out_stride, qw, kw, eps, pos, d_pos, sin_t, cos_t, n, max_seq, (int)n_heads, (int)heads, (int)hd};
-    const bool al16 = ((((uintptr_t)x | (uintptr_t)out | (uintptr_t)qw | (uintptr_t)kw | (uintptr_t)sin_t | (uintptr_t)cos_t) & 15) == 0) &&
-                      ((x_stride | out_stride) & 3) == 0;
-    if (al16 && (hd == 64 || hd == 128 || hd == 256)) {
-        const dim3 grid((unsigned)aeth_cdiv(n * heads * (hd / 8), 256)), block(256);
-        if (hd == 64) hipLaunchKernelGGL(k_qk_norm_rope_v<64>, grid, block, 0, s, A);
-        else if (hd == 128) hipLaunchKernelGGL(k_qk_norm_rope_v<128>, grid, block, 0, s, A);
-        else hipLaunchKernelGGL(k_qk_norm_rope_v<256>, grid, block, 0, s, A);
-    } else {
-        hipLaunchKernelGGL(k_qk_norm_rope, dim3((unsigned)aeth_cdiv(n * heads, 4)), dim3(256), 0, s, A);
-    }
-    AETH_LAUNCH_CHECK();
-    return AETH_OK;
+    const QkArgs A{x, x_stride, out, out_stride, qw, kw, eps, pos, d_pos, sin_t, cos_t, n, max_seq, (int)n_heads, (int)heads, (int)hd};
+    return qk_launch(A, nullptr, s);
 }
 
-extern "C" AETH_API int aeth_qk_norm_rope(const float* d_x, int64_t x_stride, int64_t n, int64_t n_heads, int64_t kv_heads,
-                                          int64_t head_dim, const float* d_qw, const float* d_kw, float eps, int64_t pos,
-                                          const int32_t* d_pos, const float* d_sin, const float* d_cos, int64_t max_seq,
-                                          float* d_out, int64_t out_stride, void* stream) {
-    const char* what = "aeth_qk_norm_rope";
-    if (!d_x || !d_sin || !d_cos || !d_out || n < 0 || n_heads < 0 || kv_heads < 0 || max_seq <= 0 || pos < 0 ||
-        head_dim <= 0 || head_dim % 2 || pos > INT64_MAX - n)
+// what the two entry points ask of their arguments in common
+static int check_qk(const char* what, const float* d_x, int64_t x_stride, int64_t n, int64_t n_heads, int64_t kv_heads, int64_t head_dim,
+                    const float* d_sin, const float* d_cos, int64_t max_seq, const float* d_out, int64_t out_stride) {
+    if (!d_x || !d_sin || !d_cos || !d_out || n < 0 || n_heads < 0 || kv_heads < 0 || max_seq <= 0 || head_dim <= 0 || head_dim % 2)
         return aeth_set_error(AETH_EINVAL, "%s: bad argument", what);
     if (n_heads > 65535 || kv_heads > 65535 || head_dim > 65536)
         return aeth_set_error(AETH_EUNSUPPORTED, "%s: %lld + %lld heads of %lld", what, (long long)n_heads, (long long)kv_heads, (long long)head_dim);
@@ -470,6 +515,42 @@ extern "C" AETH_API int aeth_qk_norm_rope(const float* d_x, int64_t x_stride, in
         return aeth_set_error(AETH_EINVAL, "%s: in place with another row stride", what);
     if (n * (n_heads + kv_heads) > (int64_t)1 << 25)  // workgroups of 256 threads within the grid's 2^32
         return aeth_set_error(AETH_EUNSUPPORTED, "%s: %lld rows of %lld heads in one call", what, (long long)n, (long long)(n_heads + kv_heads));
+    return AETH_OK;
+}
+
+extern "C" AETH_API int aeth_qk_norm_rope(const float* d_x, int64_t x_stride, int64_t n, int64_t n_heads, int64_t kv_heads,
+                                          int64_t head_dim, const float* d_qw, const float* d_kw, float eps, int64_t pos,
+                                          const int32_t* d_pos, const float* d_sin, const float* d_cos, int64_t max_seq,
+                                          float* d_out, int64_t out_stride, void* stream) {
+    const char* what = "aeth_qk_norm_rope";
+    if (pos < 0 || pos > INT64_MAX - std::max<int64_t>(n, 0)) return aeth_set_error(AETH_EINVAL, "%s: bad argument", what);
+    const int rc = check_qk(what, d_x, x_stride, n, n_heads, kv_heads, head_dim, d_sin, d_cos, max_seq, d_out, out_stride);
+    if (rc) return rc;
     return aeth_qk_norm_rope_launch(d_x, x_stride, n, n_heads, kv_heads, head_dim, d_qw, d_kw, eps, pos, d_pos, d_sin, d_cos, max_seq,
                                     d_out, out_stride, (hipStream_t)stream);
+}
+
+extern "C" AETH_API int aeth_qk_norm_rope_axes(const float* d_x, int64_t x_stride, int64_t n, int64_t n_heads, int64_t kv_heads,
+                                               int64_t head_dim, const float* d_qw, const float* d_kw, float eps, const int32_t* d_pos,
+                                               int64_t pos_stride, int64_t n_axes, const int32_t* pair_axes, const float* d_sin,
+                                               const float* d_cos, int64_t max_seq, float* d_out, int64_t out_stride, void* stream) {
+    const char* what = "aeth_qk_norm_rope_axes";
+    if (!d_pos || ((uintptr_t)d_pos & 3) || !pair_axes) return aeth_set_error(AETH_EINVAL, "%s: bad argument (positions, axes)", what);
+    const int rc = check_qk(what, d_x, x_stride, n, n_heads, kv_heads, head_dim, d_sin, d_cos, max_seq, d_out, out_stride);
+    if (rc) return rc;
+    if (head_dim > QK_MAX_HD || n_axes > QK_MAX_AXES)
+        return aeth_set_error(AETH_EUNSUPPORTED, "%s: heads of %lld turned by %lld axes (at most %d and %d)", what, (long long)head_dim,
+                              (long long)n_axes, QK_MAX_HD, QK_MAX_AXES);
+    int64_t all;
+    if (n_axes < 1 || (n_axes > 1 && pos_stride < n) || pos_stride < 0 || !aeth_mul_ok(n_axes, pos_stride, &all) || all > INT64_MAX / 4)
+        return aeth_set_error(AETH_EINVAL, "%s: %lld axes of positions %lld apart, of %lld rows", what, (long long)n_axes, (long long)pos_stride, (long long)n);
+    QkAxes X = {};
+    X.pos_stride = pos_stride;
+    for (int64_t j = 0; j < head_dim / 2; j++) {
+        if (pair_axes[j] < 0 || pair_axes[j] >= n_axes)
+            return aeth_set_error(AETH_EINVAL, "%s: pair %lld of axis %d of %lld", what, (long long)j, (int)pair_axes[j], (long long)n_axes);
+        X.axis[j / 4] |= (uint32_t)pair_axes[j] << (8 * (j % 4));
+    }
+    const QkArgs A{d_x, x_stride, d_out, out_stride, d_qw, d_kw, eps, 0, d_pos, d_sin, d_cos, n, max_seq, (int)n_heads, (int)(n_heads + kv_heads), (int)head_dim};
+    return qk_launch(A, &X, (hipStream_t)stream);
 }

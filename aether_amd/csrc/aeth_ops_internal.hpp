@@ -50,6 +50,11 @@ int64_t aeth_attn_kv8_ws(int64_t seqs, int64_t n, int64_t nq, int64_t nkv, int64
 int aeth_attn_kv8_launch(const float* q, int64_t q_stride, const void* cache, int64_t seq_bytes, const int* lens, int len_add,
                          int64_t seqs, int64_t n, int64_t nq, int64_t nkv, int64_t hd, int64_t max_seq, int64_t max_len,
                          int64_t window, float* out, void* ws, hipStream_t s);
+// what the attention's entry points ask of their arguments in common; of their workspace; of a batch's slices
+int aeth_attn_kv8_check(const char* what, const float* q, int64_t q_stride, const void* cache, int64_t seqs, int64_t n, int64_t nq,
+                        int64_t nkv, int64_t hd, int64_t max_seq, int64_t max_len, int64_t window, const float* out, const void* ws);
+int aeth_attn_kv8_check_ws(const char* what, const void* ws, int64_t ws_bytes, int64_t need);
+int aeth_attn_kv8_check_slices(const char* what, int64_t n_seqs, int64_t layer_stride, int64_t nkv, int64_t hd, int64_t max_seq);
 // head norms and rotation of q | k rows (weights nullptr: that part unnormalised); row i at d_pos[i], else pos + i
 int aeth_qk_norm_rope_launch(const float* x, int64_t x_stride, int64_t n, int64_t n_heads, int64_t kv_heads, int64_t hd,
                              const float* qw, const float* kw, float eps, int64_t pos, const int* d_pos, const float* sin_t,

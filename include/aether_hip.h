@@ -279,6 +279,18 @@ AETH_API int aeth_qk_norm_rope(const float* d_x, int64_t x_stride, int64_t n, in
                                const int32_t* d_pos, const float* d_sin, const float* d_cos, int64_t max_seq,
                                float* d_out, int64_t out_stride, void* stream);
 
+/* The same with positions of several axes (time, row and column of an image's
+ * patches), 1 to 16 of them: pair j of a head (components j and j + head_dim/2) is
+ * turned by column j of the table row of its axis' position, min(max(d_pos[a·pos_stride + i],
+ * 0), max_seq - 1) with a = pair_axes[j] (host, head_dim/2 int32 in [0, n_axes), read
+ * before the call returns; any order of axes: sections, woven). d_pos (device) holds n_axes rows of
+ * n int32, pos_stride >= n apart. Rows and norms, in place or not, as above, and the same
+ * bits where all axes of a row agree. head_dim even, at most 512. */
+AETH_API int aeth_qk_norm_rope_axes(const float* d_x, int64_t x_stride, int64_t n, int64_t n_heads, int64_t kv_heads,
+                                    int64_t head_dim, const float* d_qw, const float* d_kw, float eps, const int32_t* d_pos,
+                                    int64_t pos_stride, int64_t n_axes, const int32_t* pair_axes, const float* d_sin,
+                                    const float* d_cos, int64_t max_seq, float* d_out, int64_t out_stride, void* stream);
+
 /* ── the key/value cache in 8 bits (no counterpart in the reference) ──────
  * A layer slice of one sequence, aeth_kv8_layer_bytes(...) bytes, 16-byte
  * aligned: [kv_heads][ceil(max_seq/64)] tiles of 64 tokens, a tile being
@@ -343,6 +355,73 @@ AETH_API int aeth_attn_kv8_batch(const float* d_q, int64_t q_stride, const void*
                                  const int32_t* d_lens, int64_t n_seqs, int64_t n_heads, int64_t kv_heads,
                                  int64_t head_dim, int64_t max_seq, int64_t max_len, int64_t window, float* d_out,
                                  void* d_ws, int64_t ws_bytes, void* stream);
+/* Bytes of workspace for aeth_attn_kv8_shared of at most n_seqs sequences behind a
+ * prefix of at most prefix_len tokens; its terms are those of aeth_attn_kv8_ws_bytes. */
+AETH_API int64_t aeth_attn_kv8_shared_ws_bytes(int64_t n_seqs, int64_t n_heads, int64_t kv_heads, int64_t head_dim,
+                                               int64_t prefix_len, int64_t max_len);
+/* aeth_attn_kv8_batch for sequences that begin with the same prefix_len tokens, held
+ * once: the first prefix_len slots of d_prefix, a layer slice of prefix_seq positions
+ * (0 tokens: not read, may be NULL), are followed by the first d_lens[i] slots of
+ * sequence i's own slice, whose slot j stands at position prefix_len + j. Query i sees all of
+ * them or, with a window, the last `window`, which may end in the prefix. The prefix is read
+ * once for many sequences. A row that sees nothing is zeros. prefix_len is taken at the call (a captured call keeps it),
+ * d_lens on the stream. Numerics as for aeth_attn_kv8; the slices may not overlap d_out. */
+AETH_API int aeth_attn_kv8_shared(const float* d_q, int64_t q_stride, const void* d_prefix, int64_t prefix_seq,
+                                  int64_t prefix_len, const void* d_layers, int64_t layer_stride, const int32_t* d_lens,
+                                  int64_t n_seqs, int64_t n_heads, int64_t kv_heads, int64_t head_dim, int64_t max_seq,
+                                  int64_t max_len, int64_t window, float* d_out, void* d_ws, int64_t ws_bytes, void* stream);
+/* Bytes of workspace for the two calls below, in the terms of aeth_attn_kv8_ws_bytes. For
+ * up to 64 queries times query heads of a KV head it holds their scores: 4 bytes for
+ * each of them, position and KV head. */
+AETH_API int64_t aeth_attn_kv8_weights_ws_bytes(int64_t n_seqs, int64_t n, int64_t n_heads, int64_t kv_heads,
+                                                int64_t head_dim, int64_t max_len);
+/* aeth_attn_kv8, and the attention weight that each token receives added up: for slots
+ * t < seq of KV head h
+ *   d_weights[h·max_seq + t] = d_prior[h·max_seq + t] + sum of softmax_i(t)
+ * over the n queries i that see t and the query heads of h; slots from seq on are not
+ * written. d_prior (NULL: zeros) may be d_weights, and else overlaps none of it. A sum
+ * has relative error of the probabilities' (about 2^-23 of a score's terms, as in the attention) and of f32
+ * sums; a query whose row is NaN makes the weights of what it sees NaN. Sums have a fixed
+ * order: the same call gives the same bits again. n = 0 leaves the prior (d_q and d_out
+ * may then be NULL). */
+AETH_API int aeth_attn_kv8_weights(const float* d_q, int64_t q_stride, const void* d_layer, int64_t n, int64_t n_heads,
+                                   int64_t kv_heads, int64_t head_dim, int64_t max_seq, int64_t seq, int64_t window,
+                                   float* d_out, const float* d_prior, float* d_weights, void* d_ws, int64_t ws_bytes,
+                                   void* stream);
+/* The same beside aeth_attn_kv8_batch: weights [n_seqs][kv_heads][max_seq], the slots
+ * below d_lens[i] of sequence i. */
+AETH_API int aeth_attn_kv8_weights_batch(const float* d_q, int64_t q_stride, const void* d_layers, int64_t layer_stride,
+                                         const int32_t* d_lens, int64_t n_seqs, int64_t n_heads, int64_t kv_heads,
+                                         int64_t head_dim, int64_t max_seq, int64_t max_len, int64_t window, float* d_out,
+                                         const float* d_prior, float* d_weights, void* d_ws, int64_t ws_bytes, void* stream);
+/* Bytes of workspace for an eviction of at most n_seqs sequences of max_len tokens to
+ * `keep`; in_place: also for one whose destination is its source. */
+AETH_API int64_t aeth_kv8_evict_ws_bytes(int64_t n_seqs, int64_t kv_heads, int64_t head_dim, int64_t max_len, int64_t keep,
+                                         int in_place);
+/* Cuts a sequence of seq tokens down to `keep` (all of them where seq <= keep): of
+ * every KV head by itself the first `first`, the last `recent` (first + recent <=
+ * keep), and of the others the ones of largest weight d_weights[h·max_seq + t]; of equal weights the
+ * lower slot stays, -0 equals 0, NaN is below all else. Kept tokens move in their order, codes and scales as
+ * they are (keys stay turned by the positions they had), to slots 0 .. of d_dst, a
+ * layer slice of dst_seq positions; its other slots are left as they were. d_dst may be
+ * d_layer (dst_seq = max_seq), and else overlaps none of it. d_dst_weights (NULL: not wanted; may be
+ * d_weights where dst_seq = max_seq, and else overlaps none of it) receives
+ * [kv_heads][dst_seq] the kept tokens' weights and behind them zeros; d_kept (may be NULL)
+ * [kv_heads][keep] the slots they had, ascending, and nothing behind them. What follows an eviction counts slots, not
+ * positions: a window of the attention, `first` and `recent` of the next one. */
+AETH_API int aeth_kv8_evict(const void* d_layer, const float* d_weights, int64_t kv_heads, int64_t head_dim,
+                            int64_t max_seq, int64_t seq, int64_t keep, int64_t first, int64_t recent, void* d_dst,
+                            float* d_dst_weights, int64_t dst_seq, int32_t* d_kept, void* d_ws, int64_t ws_bytes,
+                            void* stream);
+/* The same for n_seqs sequences of d_lens[i] tokens each (device, clamped to [0, max_len]),
+ * slices layer_stride and dst_stride bytes apart, weights and kept slots one sequence behind the other.
+ * d_dst_lens (may be NULL, may be d_lens) receives the lengths left. The slices of one side lie as a
+ * whole apart from those of the other, or are the same with the same stride. */
+AETH_API int aeth_kv8_evict_batch(const void* d_layers, int64_t layer_stride, const float* d_weights, const int32_t* d_lens,
+                                  int64_t n_seqs, int64_t kv_heads, int64_t head_dim, int64_t max_seq, int64_t max_len,
+                                  int64_t keep, int64_t first, int64_t recent, void* d_dst, int64_t dst_stride,
+                                  float* d_dst_weights, int64_t dst_seq, int32_t* d_dst_lens, int32_t* d_kept, void* d_ws,
+                                  int64_t ws_bytes, void* stream);
 /* SiLU-MLP glue (runner.rs:1617-1625): g = g * sigmoid(g) * up. */
 AETH_API int aeth_silu_mul(float* d_gate, const float* d_up, int64_t n, void* stream);
 /* Residual add (runner.rs:1609-1611): x += y. */
