@@ -57,7 +57,7 @@ struct A8 {
     // a prefix that every row sees (A8_FLAT): the rows are sequences of own_lens tokens behind it, clamped to [0, own_max]
     const int* own_lens;
     int own_max;
-    float* stat;            // A8_STAT: [seqs][nkv][cols] maximum and sum of each column
+    float* stat;            // A8_STAT: [seqs][nkv][cols] maximum and 1 / sum of each column
     float* scores;          // A8_SCORE: [seqs][nkv][cols][64·score_tiles], from key 0 on
     int score_tiles;
 };
@@ -67,7 +67,7 @@ enum {
     A8_STEP = 1,   // a decode step's token with it
     A8_FLAT = 2,   // no order: every column sees the keys [0, max_len), those in the window of its sequence
     A8_PART = 4,   // partials also where there is one chunk
-    A8_STAT = 8,   // columns' maxima and sums to A.stat (where chunks are joined, by the join)
+    A8_STAT = 8,   // columns' maxima and 1 / sums to A.stat (where chunks are joined, by the join)
     A8_SCORE = 16, // the scores, in log2 units, of the tiles that some column of the block sees, to A.scores
 };
 
@@ -154,18 +154,15 @@ __device__ __forceinline__ void a8_tiles(const A8& A, int len, int c0, int count
 // STEP (HD = 128, one column block): a decode step's token with it. Each workgroup rotates q; the wave that takes the token's
 // tile also rotates k, quantises k and v, stores them and puts the codes into the fragments it loaded.
 template <int HD, int MODE>
-__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
+__device__ __forceinline__ void a8_few(const A8& A, const int bx, const int seq, const int chunk, float (&po)[4][16][HD + 4], float (&pm)[4][16],
+                                       float (&pl)[4][16], uint32_t (&fresh)[2][HD / 4]) {
     constexpr bool STEP = (MODE & A8_STEP) != 0, FLAT = (MODE & A8_FLAT) != 0, PART = (MODE & A8_PART) != 0;
     static_assert(!STEP || HD == 128, "a lane holds both halves of a rotated pair");
-    constexpr int KS = HD / 64, DT = HD / 16, PLD = HD + 4;
+    constexpr int KS = HD / 64, DT = HD / 16;
     constexpr float TH = 8.0f;
-    __shared__ __attribute__((aligned(16))) float po[4][16][PLD];
-    __shared__ float pm[4][16], pl[4][16];
-    __shared__ __attribute__((aligned(16))) uint32_t fresh[2][HD / 4];  // STEP: the token's codes of K and V
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = blockIdx.x % A.nkv, cb = A.ncb - 1 - blockIdx.x / A.nkv;  // late queries, the longest rows, first
-    const int seq = blockIdx.y, chunk = blockIdx.z;                         // the first chunks, which every sequence has, first
+    const int h = bx % A.nkv, cb = A.ncb - 1 - bx / A.nkv;  // late queries, the longest rows, first
     const int len = a8_len(A, seq);
     int beg, end;
     a8_tiles<MODE>(A, len, cb * 16, 16, beg, end);
@@ -440,12 +437,21 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
             continue;
         }
         if constexpr ((MODE & A8_STAT) != 0)
-            if (d == 0) *(float2*)(A.stat + 2 * ((int64_t)(seq * A.nkv + h) * A.cols + x)) = make_float2(M, L);
+            if (d == 0) *(float2*)(A.stat + 2 * ((int64_t)(seq * A.nkv + h) * A.cols + x)) = make_float2(M, 1.0f / L);
         acc = L == 0.0f ? (a8_f4){0.0f, 0.0f, 0.0f, 0.0f} : acc * (1.0f / L);  // a row that sees nothing: 0
         float* dst = A.out + ((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + d;
         if (A.ovec) *(a8_f4*)dst = acc;
         else dst[0] = acc[0], dst[1] = acc[1], dst[2] = acc[2], dst[3] = acc[3];
     }
+}
+
+// (a grid's first chunks, which every sequence has, first)
+template <int HD, int MODE>
+__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8(A8 A) {
+    __shared__ __attribute__((aligned(16))) float po[4][16][HD + 4];
+    __shared__ float pm[4][16], pl[4][16];
+    __shared__ __attribute__((aligned(16))) uint32_t fresh[2][HD / 4];  // A8_STEP: the token's codes of K and V
+    a8_few<HD, MODE>(A, blockIdx.x, blockIdx.y, blockIdx.z, po, pm, pl, fresh);
 }
 
 // ── many columns: a prompt, or a chunk of one ─────────────────────────────
@@ -489,21 +495,22 @@ __device__ __forceinline__ a8_h4 a8_half4(uint32_t w) {
     return (a8_h4){a[0], a[1], b[0], b[1]};
 }
 
+// V's buffers: three spare a barrier a tile; two let two workgroups of four waves share a CU's LDS
+constexpr int a8_vbufs(int nw) { return nw == 8 ? 3 : 2; }
+constexpr int A8_KF = 1040;  // bytes from one K fragment to the next: eight threads of a row store to eight bank groups
+
 template <int HD, int NW, int MODE>
-__global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
+__device__ __forceinline__ void a8_many(const A8& A, const int bx, const int seq, const int chunk, char (&kb)[2][HD / 8 * A8_KF],
+                                        char (&vb)[a8_vbufs(NW)][HD * 128], float (&sc)[a8_vbufs(NW)][2 * KV8_TILE]) {
     constexpr bool FLAT = (MODE & A8_FLAT) != 0, PART = (MODE & A8_PART) != 0;
     constexpr int KS = HD / 16, DT = HD / 32, NT = 64 * NW, CH = 4 * HD / NT;
     static_assert(CH >= 1 && CH * NT == 4 * HD, "16-byte pieces of a plane a thread");
-    constexpr int KF = 1040;  // bytes from one K fragment to the next: eight threads of a row store to eight bank groups
+    constexpr int KF = A8_KF;
     constexpr float TH = 8.0f;
-    // V's buffers: three spare a barrier a tile; two let two workgroups of four waves share a CU's LDS
-    constexpr int NB = NW == 8 ? 3 : 2;
-    __shared__ __attribute__((aligned(16))) char kb[2][2 * KS * KF];
-    __shared__ __attribute__((aligned(16))) char vb[NB][DT * 4 * 1024];
-    __shared__ __attribute__((aligned(16))) float sc[NB][2 * KV8_TILE];
+    constexpr int NB = a8_vbufs(NW);
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = blockIdx.x % A.nkv, cb = A.ncb - 1 - blockIdx.x / A.nkv, seq = blockIdx.y, chunk = blockIdx.z;
+    const int h = bx % A.nkv, cb = A.ncb - 1 - bx / A.nkv;
     const int len = a8_len(A, seq);
     int beg, end;
     a8_tiles<MODE>(A, len, cb * 32 * NW, 32 * NW, beg, end);
@@ -784,7 +791,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
         return;
     }
     if constexpr ((MODE & A8_STAT) != 0)
-        if (hf == 0) *(float2*)(A.stat + 2 * ((int64_t)(seq * A.nkv + h) * A.cols + x)) = make_float2(m, l);
+        if (hf == 0) *(float2*)(A.stat + 2 * ((int64_t)(seq * A.nkv + h) * A.cols + x)) = make_float2(m, 1.0f / l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     float* dst = A.out + ((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + 4 * hf;
 #pragma unroll
@@ -798,14 +805,22 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
         }
 }
 
+template <int HD, int NW, int MODE>
+__global__ void __launch_bounds__(64 * NW, 2) k_attn8p(A8 A) {
+    constexpr int NB = a8_vbufs(NW);
+    __shared__ __attribute__((aligned(16))) char kb[2][HD / 8 * A8_KF];
+    __shared__ __attribute__((aligned(16))) char vb[NB][HD * 128];
+    __shared__ __attribute__((aligned(16))) float sc[NB][2 * KV8_TILE];
+    a8_many<HD, NW, MODE>(A, blockIdx.x, blockIdx.y, blockIdx.z, kb, vb, sc);
+}
+
 // Joins the chunks of one column (of blocks of cw): 256 threads, four dimensions each of every 1024/hd-th chunk, so
 // that the partials of a long cache are read at once rather than one after the other
 template <int HD, int MODE>
-__global__ void __launch_bounds__(256) k_attn8_merge(A8 A, int cw) {
+__device__ __forceinline__ void a8_merge_one(const A8& A, int cw, const int bx, const int seq, float (&sum)[1024 / HD][HD]) {
     constexpr int NG = 1024 / HD;  // chunk groups
-    __shared__ __attribute__((aligned(16))) float sum[NG][HD];
     const int tid = threadIdx.x, lane = tid & 63, d = 4 * (tid % (HD / 4)), grp = tid / (HD / 4);
-    const int h = blockIdx.x % A.nkv, x = blockIdx.x / A.nkv, seq = blockIdx.y;
+    const int h = bx % A.nkv, x = bx / A.nkv;
     const int cb = x / cw, cc = x % cw;
     int beg, end;
     a8_tiles(A, a8_len(A, seq), cb * cw, cw, beg, end);
@@ -830,7 +845,7 @@ __global__ void __launch_bounds__(256) k_attn8_merge(A8 A, int cw) {
     }
     *(a8_f4*)&sum[grp][d] = acc;
     if constexpr ((MODE & A8_STAT) != 0)
-        if (tid == 0) *(float2*)(A.stat + 2 * ((int64_t)(seq * A.nkv + h) * A.cols + x)) = make_float2(M, L);
+        if (tid == 0) *(float2*)(A.stat + 2 * ((int64_t)(seq * A.nkv + h) * A.cols + x)) = make_float2(M, 1.0f / L);
     __syncthreads();
     if (tid >= HD) return;
     float y = 0.0f;
@@ -839,11 +854,17 @@ __global__ void __launch_bounds__(256) k_attn8_merge(A8 A, int cw) {
     A.out[((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + tid] = L == 0.0f ? 0.0f : y * (1.0f / L);
 }
 
+template <int HD, int MODE>
+__global__ void __launch_bounds__(256) k_attn8_merge(A8 A, int cw) {
+    __shared__ __attribute__((aligned(16))) float sum[1024 / HD][HD];
+    a8_merge_one<HD, MODE>(A, cw, blockIdx.x, blockIdx.y, sum);
+}
+
 // The same for at most 8 chunks: hd / 4 lanes a column, its partials all in flight at once
 template <int HD, int MODE>
-__global__ void __launch_bounds__(256) k_attn8_merge_few(A8 A, int cw) {
+__device__ __forceinline__ void a8_merge_some(const A8& A, int cw, const int bx, const int seq) {
     constexpr int MOST = 8;
-    const int unit = (blockIdx.x * 256 + threadIdx.x) / (HD / 4), d = 4 * (threadIdx.x % (HD / 4)), seq = blockIdx.y;
+    const int unit = (bx * 256 + threadIdx.x) / (HD / 4), d = 4 * (threadIdx.x % (HD / 4));
     if (unit >= A.nkv * A.cols) return;
     const int h = unit / A.cols, x = unit % A.cols, cb = x / cw, cc = x % cw;
     int beg, end;
@@ -875,19 +896,25 @@ __global__ void __launch_bounds__(256) k_attn8_merge_few(A8 A, int cw) {
             for (int e = 0; e < 4; e++) acc[e] += in ? v[k][e] * w : 0.0f;
         }
     if constexpr ((MODE & A8_STAT) != 0)
-        if (d == 0) *(float2*)(A.stat + 2 * ((int64_t)(seq * A.nkv + h) * A.cols + x)) = make_float2(M, L);
+        if (d == 0) *(float2*)(A.stat + 2 * ((int64_t)(seq * A.nkv + h) * A.cols + x)) = make_float2(M, 1.0f / L);
     acc = L == 0.0f ? (a8_f4){0.0f, 0.0f, 0.0f, 0.0f} : acc * (1.0f / L);
     float* dst = A.out + ((int64_t)seq * A.n + x / A.G) * ((int64_t)A.nq * HD) + (int64_t)(h * A.G + x % A.G) * HD + d;
     if (A.ovec) *(a8_f4*)dst = acc;
     else dst[0] = acc[0], dst[1] = acc[1], dst[2] = acc[2], dst[3] = acc[3];
 }
 
+template <int HD, int MODE>
+__global__ void __launch_bounds__(256) k_attn8_merge_few(A8 A, int cw) { a8_merge_some<HD, MODE>(A, cw, blockIdx.x, blockIdx.y); }
+
 // A workgroup a column costs a µs for each thousand of them (16000 columns in 2 chunks: 25 µs, 9 with 32 lanes each; 8000 in 8:
 // 15 and 8); of a few columns it has more of many chunks in flight (256 columns in 8 chunks: 0.8 µs less, 1024: 0.2).
+inline bool a8_merge_is_some(const A8& A, int64_t seqs) {
+    return A.chunks <= 4 || (A.chunks <= 8 && (int64_t)A.nkv * A.cols * seqs >= 6 * (int64_t)aeth_num_cus());
+}
 template <int HD, int MODE>
 void a8_merge(const A8& A, int cw, int64_t seqs, hipStream_t s) {
     const int64_t cols = (int64_t)A.nkv * A.cols;
-    if (A.chunks <= 4 || (A.chunks <= 8 && cols * seqs >= 6 * (int64_t)aeth_num_cus()))
+    if (a8_merge_is_some(A, seqs))
         hipLaunchKernelGGL((k_attn8_merge_few<HD, MODE>), dim3((unsigned)aeth_cdiv(cols * (HD / 4), 256), (unsigned)seqs), dim3(256), 0, s, A, cw);
     else hipLaunchKernelGGL((k_attn8_merge<HD, MODE>), dim3((unsigned)cols, (unsigned)seqs), dim3(256), 0, s, A, cw);
 }
@@ -992,14 +1019,16 @@ template <int HD, int MODE>
 int a8_launch(const A8& A, const Form& f, int64_t seqs, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)A.nkv * A.ncb), (unsigned)seqs, (unsigned)A.chunks);
     if (f.cw == 16) hipLaunchKernelGGL((k_attn8<HD, MODE>), grid, dim3(256), 0, s, A);
-    if constexpr (HD <= 128 && !(MODE & A8_SCORE))
+    if constexpr (HD <= 128)
         if (f.cw == 128) hipLaunchKernelGGL((k_attn8p<HD, 4, MODE>), grid, dim3(256), 0, s, A);
-    if constexpr (HD == 128 && !(MODE & A8_SCORE))
+    if constexpr (HD == 128)
         if (f.cw == 256) hipLaunchKernelGGL((k_attn8p<HD, 8, MODE>), grid, dim3(512), 0, s, A);
     AETH_LAUNCH_CHECK();
-    if (A.chunks > 1 && !(MODE & A8_PART)) {
-        a8_merge<HD, MODE>(A, f.cw, seqs, s);
-        AETH_LAUNCH_CHECK();
+    if constexpr ((MODE & A8_PART) == 0) {
+        if (A.chunks > 1) {
+            a8_merge<HD, MODE>(A, f.cw, seqs, s);
+            AETH_LAUNCH_CHECK();
+        }
     }
     return AETH_OK;
 }

@@ -17,6 +17,31 @@ namespace {
 
 // ── a shared prefix ───────────────────────────────────────────────────────
 
+// Both attentions in one launch, each a share of the workgroups: the prefix's products keep the matrix units busy, the sequences' own
+// tokens the memory. The first `prefixes` workgroups take the prefix in columns of cw (16, or 128 in the form for many), the others a sequence
+// each (its chunks after one another: the first ones, which every sequence has, first).
+template <int HD, int CW>
+__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8_shared(A8 P, A8 O, int prefixes, int seqs) {
+    constexpr int MAX = CW == 128 ? std::max((int)sizeof(float[4][16][HD + 4]), 2 * (HD / 8) * A8_KF) : (int)sizeof(float[4][16][HD + 4]);
+    __shared__ __attribute__((aligned(16))) char lds[MAX];
+    __shared__ float pm[4][16], pl[4][16];
+    uint32_t(&none)[2][HD / 4] = *(uint32_t(*)[2][HD / 4])lds;  // a decode step's, which no form here has
+    float(&po)[4][16][HD + 4] = *(float(*)[4][16][HD + 4])lds;
+    const int bx = blockIdx.x;
+    if (bx >= prefixes) {
+        const int per = O.nkv * O.ncb, at = bx - prefixes, unit = at / per;
+        a8_few<HD, A8_PART>(O, at % per, unit % seqs, unit / seqs, po, pm, pl, none);
+    } else if constexpr (CW == 128) {
+        __shared__ __attribute__((aligned(16))) char vb[2][HD * 128];
+        __shared__ __attribute__((aligned(16))) float sc[2][2 * KV8_TILE];
+        const int per = P.nkv * P.ncb;
+        a8_many<HD, 4, A8_FLAT | A8_PART>(P, bx % per, 0, bx / per, *(char(*)[2][HD / 8 * A8_KF])lds, vb, sc);
+    } else {
+        const int per = P.nkv * P.ncb;
+        a8_few<HD, A8_FLAT | A8_PART>(P, bx % per, 0, bx / per, po, pm, pl, none);
+    }
+}
+
 // Joins a column's parts of the prefix (P, blocks of cw columns) and of its own tokens (O, of 16): HD/4 lanes of four dimensions, GR of such
 // groups take every GR-th part.
 template <int HD, int GR>
@@ -77,7 +102,7 @@ __global__ void __launch_bounds__(256) k_attn8_join(A8 P, int cw, A8 O) {
     }
 }
 
-// The prefix's form: a8_form's reckoning for columns that all see `span` tiles
+// The prefix's form, 16 or 128 columns: a8_form's reckoning for columns that all see `span` tiles
 Form sv_prefix_form(int64_t cols, int64_t nkv, int64_t hd, int64_t span) {
     const int64_t cus = aeth_num_cus();
     const Form small = a8_split(16, nkv * aeth_cdiv(cols, 16), span, 2 * cus, 4);
@@ -85,18 +110,16 @@ Form sv_prefix_form(int64_t cols, int64_t nkv, int64_t hd, int64_t span) {
     const double c = (double)cus;
     Form best = small;
     double least = INFINITY;
-    for (int64_t cw = 16; cw <= (hd == 128 ? 256 : 128); cw = std::max<int64_t>(128, 2 * cw)) {
+    for (int64_t cw : {16, 128}) {
         const int64_t units = nkv * aeth_cdiv(cols, cw);
         const double tiles = (double)units * (double)span;
         for (int64_t target : {(int64_t)0, cus, 2 * cus, 4 * cus}) {
-            if (target > (cw == 16 ? 4 : cw == 128 ? 2 : 1) * cus) continue;
+            if (target > (cw == 16 ? 4 : 2) * cus) continue;
             const Form f = a8_split(cw, units, span, std::max<int64_t>(1, target), cw == 16 ? 4 : 8);
             const int64_t wgs = units * f.chunks;
             const double w = tiles / c, tpc = (double)std::min<int64_t>(f.tpc, span);
             const double u = (double)aeth_cdiv(wgs, cus), q = u * (tiles / (double)wgs);
-            const double own = std::max(tpc, w);
-            double t = cw == 256   ? 12.0 + 2.8 * own + 1.5 * std::max(0.0, w - 0.4 * own)
-                       : cw == 128 ? (hd == 128 ? std::max(8.0 + 2.3 * tpc, 22.0 + 1.96 * w) : std::max(7.0 + 1.53 * tpc, 15.0 + 1.25 * w))
+            double t = cw == 128   ? (hd == 128 ? std::max(8.0 + 2.3 * tpc, 22.0 + 1.96 * w) : std::max(7.0 + 1.53 * tpc, 15.0 + 1.25 * w))
                        : hd == 128 ? std::max(5.5 + 0.45 * tpc, 6.0 + 0.33 * q + 4.5 * std::ceil(u / 3.0))
                                    : std::max(5.0 + 0.3 * tpc, 5.0 + 0.185 * q + 2.8 * std::ceil(u / 4.0));
             t += (cw == 16 ? 2e-6 : 1e-6) * (double)(nkv * cols * f.chunks) * (double)(hd + 2);
@@ -115,7 +138,6 @@ int64_t sv_prefix_ws(int64_t seqs, int64_t nq, int64_t nkv, int64_t hd) {
     auto need = [&](int64_t cw, int64_t target) { return (target + nkv * aeth_cdiv(cols, cw)) * cw; };
     int64_t most = need(16, 4 * cus);
     if (hd <= 128 && cols > 64) most = std::max(most, need(128, 2 * cus));
-    if (hd == 128 && cols > 64) most = std::max(most, need(256, cus));
     return most * (hd + 2) * (int64_t)sizeof(float);
 }
 int64_t sv_own_ws(int64_t seqs, int64_t nq, int64_t nkv, int64_t hd) {
@@ -132,16 +154,16 @@ int sv_shared(A8 P, A8 O, int64_t seqs, hipStream_t s) {
         fp = sv_prefix_form(P.cols, P.nkv, HD, span);
     }
     a8_take(P, fp);
-    if (P.chunks > 0) {
-        const int rc = a8_launch<HD, A8_FLAT | A8_PART>(P, fp, 1, s);
-        if (rc) return rc;
-    }
-    hipLaunchKernelGGL((k_attn8<HD, A8_PART>), dim3((unsigned)(O.nkv * O.ncb), (unsigned)seqs, (unsigned)O.chunks), dim3(256), 0, s, O);
+    const int64_t prefixes = (int64_t)P.nkv * P.ncb * P.chunks, own = (int64_t)O.nkv * O.ncb * seqs * O.chunks;
+    const dim3 grid((unsigned)(prefixes + own)), block(256);
+    if (fp.cw == 16) hipLaunchKernelGGL((k_attn8_shared<HD, 16>), grid, block, 0, s, P, O, (int)prefixes, (int)seqs);
+    if constexpr (HD <= 128)
+        if (fp.cw == 128) hipLaunchKernelGGL((k_attn8_shared<HD, 128>), grid, block, 0, s, P, O, (int)prefixes, (int)seqs);
     AETH_LAUNCH_CHECK();
     const int64_t cols = (int64_t)O.nkv * O.G;
     constexpr int GR = 1024 / HD;
-    if (P.chunks + O.chunks <= 8) hipLaunchKernelGGL((k_attn8_join<HD, 1>), dim3((unsigned)aeth_cdiv(cols, GR), (unsigned)seqs), dim3(256), 0, s, P, fp.cw, O);
-    else hipLaunchKernelGGL((k_attn8_join<HD, GR>), dim3((unsigned)cols, (unsigned)seqs), dim3(256), 0, s, P, fp.cw, O);
+    if (P.chunks + O.chunks <= 8) hipLaunchKernelGGL((k_attn8_join<HD, 1>), dim3((unsigned)aeth_cdiv(cols, GR), (unsigned)seqs), block, 0, s, P, fp.cw, O);
+    else hipLaunchKernelGGL((k_attn8_join<HD, GR>), dim3((unsigned)cols, (unsigned)seqs), block, 0, s, P, fp.cw, O);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }
@@ -153,176 +175,307 @@ struct Weigh {
     float* weights;
     int64_t max_seq;
     float* part;         // k_kv8_weigh in several chunks of columns: [chunks][nkv][keys]
-    int chunks;
-    int64_t keys;        // of a row of part: a multiple of 256
+    int chunks, per;     // of `per` blocks of columns, as many as the keys' columns have
+    int first, full;     // the first group of keys that some column sees; so many from there have all chunks
+    int64_t keys;        // of a row of part, from that group on: whole groups
+    int wgs;             // workgroups a head
 };
 
-// From the scores of up to a few hundred columns: 1024 keys a workgroup
-__global__ void __launch_bounds__(256) k_kv8_weigh_scores(A8 A, Weigh W) {
-    constexpr int CB = 64;
-    __shared__ float2 col[CB];  // maximum, 1 / sum
-    const int tid = threadIdx.x, h = blockIdx.y, seq = blockIdx.z;
-    const int len = a8_len(A, seq), t0 = blockIdx.x * 1024;
+// The maximum and 1 / sum of a column: as the attention left it, or from its chunks' parts (every lane of the wave calls it, and
+// every lane has the result)
+template <int HD>
+__device__ __forceinline__ float2 sv_column(const A8& A, int len, int seq, int h, int x) {
+    const int64_t unit = (int64_t)seq * A.nkv + h;
+    if (A.chunks == 1) return *(const float2*)(A.stat + 2 * (unit * A.cols + x));
+    int beg, end;
+    a8_tiles(A, len, x / 16 * 16, 16, beg, end);
+    const int live = max(1, (end - beg + A.tpc - 1) / A.tpc), lane = threadIdx.x & 63;
+    const int64_t step = 16 * (HD + 2);
+    const float* st = A.ws + (unit * A.ncb + x / 16) * A.chunks * step + 16 * HD + 2 * (x % 16);
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    for (int k = lane; k < live; k += 64) {
+        const float2 more = *(const float2*)(st + k * step);
+        const float m = fmaxf(ml.x, more.x);
+        ml.y = (ml.x == -INFINITY ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - m)) + (more.x == -INFINITY ? 0.0f : more.y * __builtin_amdgcn_exp2f(more.x - m));
+        ml.x = m;
+    }
+    const float M = aeth_wave_max(ml.x);
+    const float S = aeth_wave_sum(ml.x == -INFINITY ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - M));
+    return make_float2(M, 1.0f / S);
+}
+
+// From the scores: workgroup (256 keys, KV head), the columns 32 at a time, their statistics first
+template <int HD>
+__device__ __forceinline__ void sv_weigh_scores(const A8& A, const Weigh& W, int bx, int seq, float2 (&col)[32]) {
+    const int tid = threadIdx.x, h = bx % A.nkv, t0 = bx / A.nkv * 256, t = t0 + tid;
+    const int len = a8_len(A, seq);
     if (t0 >= len) return;  // (uniform)
-    const int64_t unit = (int64_t)seq * A.nkv + h, row = 64 * (int64_t)A.score_tiles;
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c0 = 0; c0 < A.cols; c0 += CB) {
-        const int count = min(CB, A.cols - c0);
-        __syncthreads();
-        if (tid < count) {
-            const float2 ml = *(const float2*)(A.stat + 2 * (unit * A.cols + c0 + tid));
-            col[tid] = make_float2(ml.x, 1.0f / ml.y);
+    const int64_t unit = (int64_t)seq * A.nkv + h, row = 64 * (int64_t)A.score_tiles, at = unit * W.max_seq + t;
+    const float* src = A.scores + unit * A.cols * row + min(t, (int)row - 1);
+    const bool real = t < len;
+    float acc = real && W.prior ? W.prior[at] : 0.0f, sum = 0.0f;
+    for (int c0 = 0; c0 < A.cols; c0 += 32) {
+        const int count = min(32, A.cols - c0);
+        if (c0 > 0) __syncthreads();
+        for (int c = tid >> 6; c < count; c += 4) {
+            const float2 ml = sv_column<HD>(A, len, seq, h, c0 + c);
+            if ((tid & 63) == 0) col[c] = ml;
         }
         __syncthreads();
-        for (int c = 0; c < count; c++) {
-            const int hi = len - A.n + (c0 + c) / A.G + 1, lo = A.window > 0 ? hi - A.window : 0;  // (uniform)
-            const float* src = A.scores + (unit * A.cols + c0 + c) * row;
-            const float2 mi = col[c];
+        const int hi0 = len - A.n + 1;
+        for (int c1 = 0; c1 < count; c1 += 4) {
+            float s[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[j] = src[min(c0 + c1 + j, A.cols - 1) * row];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int t = t0 + tid + 256 * j;
-                if (t >= lo && t < hi) acc[j] = fmaf(__builtin_amdgcn_exp2f(src[t] - mi.x), mi.y, acc[j]);
+                const int x = c0 + c1 + j, hi = hi0 + x / A.G, lo = A.window > 0 ? hi - A.window : 0;  // (uniform)
+                const float2 ml = col[min(c1 + j, 31)];
+                if (x < A.cols && t >= lo && t < hi) sum = fmaf(__builtin_amdgcn_exp2f(s[j] - ml.x), ml.y, sum);
             }
         }
     }
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int64_t t = t0 + tid + 256 * j, at = unit * W.max_seq + t;
-        if (t < len) W.weights[at] = W.prior ? W.prior[at] + acc[j] : acc[j];
-    }
+    if (real) W.weights[at] = acc + sum;
 }
 
-// Many columns: a wave keeps 64 keys (one tile) as fp16 in registers, its workgroup 256, and goes through its columns 32 at a
-// time: their q as two fp16 parts from LDS (aeth_attn_kv8_dev.hpp: the same products as the attention's), the scores' exponentials summed
-// in registers over the blocks of columns and at the end over the lanes.
 template <int HD>
-__global__ void __launch_bounds__(256, 2) k_kv8_weigh(A8 A, Weigh W) {
-    constexpr int KS = HD / 16, KF = 1040, E = HD / 8;
+__global__ void __launch_bounds__(256) k_kv8_weigh_scores(A8 A, Weigh W) {
+    __shared__ float2 col[32];
+    sv_weigh_scores<HD>(A, W, blockIdx.x, blockIdx.y, col);
+}
+
+// The join of the attention's chunks (the first `joins` workgroups) and the weights, which only share what they read, in one launch
+template <int HD, bool SOME>
+__global__ void __launch_bounds__(256) k_kv8_join_weigh(A8 A, Weigh W, int joins) {
+    __shared__ __attribute__((aligned(16))) float sum[1024 / HD][HD];
+    __shared__ float2 col[32];
+    const int bx = blockIdx.x;
+    if (bx >= joins) sv_weigh_scores<HD>(A, W, bx - joins, blockIdx.y, col);
+    else if constexpr (SOME) a8_merge_some<HD, 0>(A, 16, bx, blockIdx.y);
+    else a8_merge_one<HD, 0>(A, 16, bx, blockIdx.y, sum);
+}
+
+// Keys of a workgroup of k_kv8_weigh: two halves of 32 a wave, or one where a half's codes take as many registers
+constexpr int sv_group(int hd) { return hd == 256 ? 256 : 512; }
+
+// The blocks of 32 columns that see a key of k0 .. k0 + keys - 1: from column x_beg on
+struct Seen {
+    int x_beg, x_end, blocks;
+};
+__host__ __device__ inline Seen sv_seen(int n, int G, int len, int window, int64_t k0, int keys) {
+    const int past = len - n;  // keys before the first query
+    const int64_t i0 = k0 > past ? k0 - past : 0;
+    int64_t i1 = n;
+    if (window > 0) {
+        const int64_t last = (k0 + keys < len ? k0 + keys : len) - 1 + (int64_t)window - past;
+        i1 = last < i1 ? last : i1;
+    }
+    if (i1 <= i0) return {0, 0, 0};
+    return {(int)(i0 * G), (int)(i1 * G), (int)(((i1 - i0) * G + 31) / 32)};
+}
+
+// The chunks of a group's columns
+__device__ __forceinline__ int sv_count(const A8& A, const Weigh& W, int group, int gk) {
+    return max(1, (sv_seen(A.n, A.G, A.max_len, A.window, gk * (int64_t)group, gk).blocks + W.per - 1) / W.per);
+}
+
+// Many columns: a wave keeps NT·32 keys as fp16 in registers, its workgroup of eight waves 512 (256), and goes through W.per blocks of 32
+// of the columns that see them: their q as two fp16 parts from LDS (the attention's own products, aeth_attn_kv8_dev.hpp), the exponentials
+// summed in registers over the blocks and at the end over the lanes.
+template <int HD>
+__global__ void __launch_bounds__(512, 2) k_kv8_weigh(A8 A, Weigh W) {
+    constexpr int GK = sv_group(HD), NT = GK / 256, KS = HD / 16, KF = 1040, E = HD / 16, EV = E < 8 ? E : 8;
     __shared__ __attribute__((aligned(16))) char qb[2][2 * KS * KF];
     __shared__ __attribute__((aligned(16))) float4 col[2][32];  // scale of a product, maximum, 1 / sum, the key behind the last one it sees
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = blockIdx.y, chunk = blockIdx.z, len = A.max_len, k0 = 256 * blockIdx.x;
-    const int last = (len - 1) >> 6, t = 4 * blockIdx.x + w, tl = min(t, last);
-    // the columns that see a key of the workgroup, those of this chunk
-    const int past = len - A.n;  // keys before the first query
-    const int i0 = max(0, k0 - past), i1 = A.window > 0 ? (int)min((int64_t)A.n, (int64_t)min(k0 + 256, len) + A.window - 1 - past) : A.n;
-    const int nb = i1 > i0 ? ((i1 - i0) * A.G + 31) / 32 : 0, per = (nb + W.chunks - 1) / W.chunks;
-    const int b0 = chunk * per, b1 = min(b0 + per, nb);
-    const int x_beg = i0 * A.G, x_end = i1 * A.G;
+    // Workgroups go to the eight dies in turn: a KV head stays on one where there are eight. There are none without work, which
+    // are not spread evenly and leave two on some CUs (with a third of them: 2000 tokens of 32 / 8 heads 106 µs).
+    const int h = blockIdx.x % A.nkv, len = A.max_len, past = len - A.n;
+    int group = W.first, chunk = blockIdx.x / A.nkv;
+    if (chunk < W.full * W.chunks) {
+        group += chunk / W.chunks;
+        chunk %= W.chunks;
+    } else {
+        group += W.full;
+        chunk -= W.full * W.chunks;
+        for (int count; chunk >= (count = sv_count(A, W, group, GK)); chunk -= count) group++;
+    }
+    const int k0 = GK * group + 32 * NT * w;  // the wave's first key
+    const Seen sees = sv_seen(A.n, A.G, len, A.window, GK * (int64_t)group, GK);
+    const int b0 = chunk * W.per, b1 = min(b0 + W.per, sees.blocks);
 
-    float acc[2][16];
+    float acc[NT][16];
 #pragma unroll
-    for (int T = 0; T < 2; T++)
+    for (int T = 0; T < NT; T++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[T][i] = 0.0f;
 
     if (b0 < b1) {  // (uniform)
-        // keys: lane (key l%32, half l/32) of fragment (T, ks) holds eight dimensions
-        const uint8_t* p = A.cache + ((int64_t)h * A.tiles + tl) * aeth_kv8_tile_bytes(HD);
-        a8_h8 kf[2][KS];
-        float sk[2];
-#pragma unroll
-        for (int T = 0; T < 2; T++) {
-            const int st = 32 * T + 8 * ((lane >> 2) & 3) + 4 * hf + (lane & 3);
-            const float ks = *(const float*)(p + 2 * KV8_TILE * HD + 4 * st), vs = *(const float*)(p + 2 * KV8_TILE * HD + 4 * (KV8_TILE + st));
-            sk[T] = fabsf(vs) < INFINITY ? ks : __uint_as_float(0x7FC00000u);
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const uint2 k = *(const uint2*)(p + (32 * T + c) * HD + 16 * s + 8 * hf);
-                const a8_h4 a = a8_half4(k.x), b = a8_half4(k.y);
-                kf[T][s] = (a8_h8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-            }
-        }
-        // a block of columns: eight threads take one
-        const int sc = tid >> 3, sj = tid & 7;
+        // a block of columns: 16 threads take one, E dimensions each
+        const int sc = tid >> 4, sj = tid & 15;
         float y[E];
-        float2 ml;
-        int qi = 0;
-        bool real = false;
-        auto fetch = [&](int b) {
-            const int x = x_beg + 32 * b + sc, xc = min(x, x_end - 1);
-            real = x < x_end;
-            qi = xc / A.G;
-            const float* src = A.q + (int64_t)qi * A.q_stride + (int64_t)(h * A.G + xc % A.G) * HD + E * sj;
+        float2 mi;
+        int hi;             // the key behind the last one it sees
+        // the column to fetch: its query and head, its q and statistics
+        int x = sees.x_beg + 32 * b0 + sc, qi = x / A.G, qg = x % A.G;
+        const int step_i = 32 / A.G, step_g = 32 % A.G;
+        const float* src = A.q + (int64_t)qi * A.q_stride + (int64_t)(h * A.G + qg) * HD + E * sj;
+        const int64_t step_src = step_i * A.q_stride + step_g * HD, wrap_src = A.q_stride - (int64_t)A.G * HD;
+        const float2* stat = (const float2*)A.stat + (int64_t)h * A.cols;
+        auto fetch = [&]() {
+            const bool real = x < sees.x_end;  // past the end: some column, masked
+            const float* p = real ? src : A.q + (int64_t)h * A.G * HD + E * sj;
 #pragma unroll
             for (int e = 0; e < E; e += 4) {
                 float4 v;
-                if (A.qvec) v = *(const float4*)(src + e);
-                else v = make_float4(src[e], src[e + 1], src[e + 2], src[e + 3]);
+                if (A.qvec) v = *(const float4*)(p + e);
+                else v = make_float4(p[e], p[e + 1], p[e + 2], p[e + 3]);
                 y[e] = v.x;
                 y[e + 1] = v.y;
                 y[e + 2] = v.z;
                 y[e + 3] = v.w;
             }
-            ml = *(const float2*)(A.stat + 2 * ((int64_t)h * A.cols + xc));
+            mi = stat[real ? x : 0];
+            hi = real ? past + qi + 1 : 0;
+            x += 32;
+            qi += step_i;
+            qg += step_g;
+            src += step_src;
+            if (qg >= A.G) {
+                qg -= A.G;
+                qi++;
+                src += wrap_src;
+            }
         };
         auto stage = [&](int buf) {
             uint32_t mb = 0;
 #pragma unroll
             for (int e = 0; e < E; e++) mb = max(mb, __float_as_uint(y[e]) & 0x7FFFFFFFu);
-            mb = kv8_umax<8>(mb);
+            mb = kv8_umax<16>(mb);
             const int e2 = a8_exponent(__uint_as_float(mb)) - 8;  // the largest below 2^15
-            const float f = a8_pow2(e2);
+            // a row that is NaN (its sum is; an infinity or NaN in q makes it so): products that are NaN, so that a masked key's can be left out
+            const bool nan = mi.y != mi.y;
+            const float f = nan ? mi.y : a8_pow2(e2);
 #pragma unroll
-            for (int e = 0; e < E; e += 8) {
-                a8_h8 hi, lo;
+            for (int e = 0; e < E; e += EV) {
+                typedef _Float16 part __attribute__((ext_vector_type(EV)));
+                part hi, lo;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
+                for (int i = 0; i < EV; i++) {
                     const float v = y[e + i] * f;
                     hi[i] = (_Float16)v;
                     lo[i] = (_Float16)(v - (float)hi[i]);
                 }
                 const int dim = E * sj + e;
-                char* dst = qb[buf] + (dim >> 4) * KF + (sc + 32 * (dim >> 3 & 1)) * 16;
-                *(a8_h8*)dst = hi;
-                *(a8_h8*)(dst + KS * KF) = lo;
+                char* dst = qb[buf] + (dim >> 4) * KF + (sc + 32 * (dim >> 3 & 1)) * 16 + 2 * (dim & 7);
+                *(part*)dst = hi;
+                *(part*)(dst + KS * KF) = lo;
             }
             if (sj == 0) {
-                // an infinity or NaN in q: every score NaN
-                const float qs = mb >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : a8_pow2(-e2) * (1.4426950408889634f / sqrtf((float)HD));
-                col[buf][sc] = make_float4(qs, ml.x, 1.0f / ml.y, __int_as_float(real ? past + qi + 1 : (int)0x80000000));
+                const float qs = a8_pow2(-e2) * (1.4426950408889634f / sqrtf((float)HD));
+                col[buf][sc] = make_float4(nan ? 1.0f : qs, nan ? 0.0f : mi.x, nan ? 1.0f : mi.y, __int_as_float(hi));
             }
         };
-        fetch(b0);
+        fetch();
+        // keys: lane (key l%32, half l/32) of fragment (T, ks) holds eight dimensions
+        const uint8_t* p = A.cache + ((int64_t)h * A.tiles + min(k0, len - 1) / KV8_TILE) * aeth_kv8_tile_bytes(HD);
+        a8_h8 kf[NT][KS];
+        float sk[NT];
+#pragma unroll
+        for (int T = 0; T < NT; T++) {
+            const int half = NT == 2 ? 32 * T : k0 & 32;  // of a tile
+            const int st = half + 8 * ((lane >> 2) & 3) + 4 * hf + (lane & 3);
+            const float ks = *(const float*)(p + 2 * KV8_TILE * HD + 4 * st), vs = *(const float*)(p + 2 * KV8_TILE * HD + 4 * (KV8_TILE + st));
+            sk[T] = fabsf(vs) < INFINITY ? ks : __uint_as_float(0x7FC00000u);
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const uint2 k = *(const uint2*)(p + (half + c) * HD + 16 * s + 8 * hf);
+                const a8_h4 a = a8_half4(k.x), b = a8_half4(k.y);
+                kf[T][s] = (a8_h8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+            }
+        }
+        // the first and last query of a block: every column of it sees the keys [all_lo, all_hi)
+        int x0 = sees.x_beg + 32 * b0, i_first = x0 / A.G, g_first = x0 % A.G;
+        a8_f16 s[NT];       // a block's scores, from one block to the next
+#pragma unroll
+        for (int T = 0; T < NT; T++) s[T] = (a8_f16){};
+        float4 cl = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        auto weigh = [&](float& a, float s, const float4& of) { a = fmaf(__builtin_amdgcn_exp2f(fmaf(s, of.x, -of.y)), of.z, a); };
+        // The next block's columns are staged, and those behind them fetched, by the first four waves before their products and by
+        // the others, one on each SIMD with them, behind: of two waves one has products for the matrix unit
+        auto ahead = [&](int b, int buf) {
+            if (b + 1 >= b1) return;  // (uniform)
+            stage(buf ^ 1);
+            if (b + 2 < b1) fetch();
+        };
+        stage(0);
+        if (b0 + 1 < b1) fetch();
+        __syncthreads();
         for (int b = b0; b < b1; b++) {
             const int buf = (b - b0) & 1;
-            stage(buf);
-            __syncthreads();  // (the other buffer's readers have passed the barrier before this one)
-            if (b + 1 < b1) fetch(b + 1);
-            const float4 cl = col[buf][c];
-            a8_f16 s[2] = {(a8_f16){}, (a8_f16){}};
+            if (w < 4) ahead(b, buf);
             const char* qp = qb[buf] + lane * 16;
+            const float4 of = cl;
+            cl = col[buf][c];
+            // The products of a block, and between them one by one the exponentials of the block before (before the first: of nothing,
+            // times 0): they run on different units, a product waits for the one before the last, and a wave issues in order
+            a8_f16 d[NT];
+            a8_h8 ql[2] = {*(const a8_h8*)(qp + KS * KF), *(const a8_h8*)(qp + (KS + 1) * KF)}, qh[2] = {*(const a8_h8*)qp, *(const a8_h8*)(qp + KF)};
+            a8_unroll<2 * KS * NT>([&](auto mm) {
+                constexpr int m = mm, T = m % NT, low = m / NT % 2 == 0, ks = m / (2 * NT);
+                constexpr int first = 8 * m / KS, count = 8 * (m + 1) / KS - first;
+                __builtin_amdgcn_sched_barrier(0);
+                a8_h8& q = low ? ql[ks & 1] : qh[ks & 1];
+                d[T] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[T][ks], q, low && ks == 0 ? (a8_f16){} : d[T], 0, 0, 0);
+                if constexpr (T == NT - 1 && ks + 2 < KS) q = *(const a8_h8*)(qp + ((low ? KS : 0) + ks + 2) * KF);
+                a8_unroll<count>([&](auto e) {
+                    constexpr int i = first + e;
+                    weigh(acc[i / 16][i % 16], s[i / 16][i % 16], of);
+                    asm volatile("" : "+v"(acc[i / 16][i % 16]));  // here, and not behind the next branch, where it is used
+                });
+            });
+            const int x1 = min(x0 + 31, sees.x_end - 1), i_last = i_first + (g_first + x1 - x0) / A.G;
+            const int all_hi = x0 + 32 > sees.x_end ? 0 : past + i_first + 1, all_lo = A.window > 0 ? past + i_last + 1 - A.window : 0;
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                const a8_h8 ql = *(const a8_h8*)(qp + (KS + ks) * KF), qh = *(const a8_h8*)(qp + ks * KF);
-                s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[0][ks], ql, s[0], 0, 0, 0);
-                s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[1][ks], ql, s[1], 0, 0, 0);
-                s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[0][ks], qh, s[0], 0, 0, 0);
-                s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[1][ks], qh, s[1], 0, 0, 0);
-            }
-            // every column of the block sees the keys [all_lo, all_hi)
-            const int x0 = x_beg + 32 * b, all_hi = x0 + 32 > x_end ? 0 : past + x0 / A.G + 1;
-            const int all_lo = A.window > 0 ? past + min(x0 + 31, x_end - 1) / A.G + 1 - A.window : 0;
-            const int hi = __float_as_int(cl.w), lo = A.window > 0 ? max(hi, 0) - A.window : 0;
-            const bool masked = 64 * t < all_lo || 64 * t + 64 > all_hi;  // (uniform)
-#pragma unroll
-            for (int T = 0; T < 2; T++)
+            for (int T = 0; T < NT; T++)
                 a8_unroll<16>([&](auto at) {
                     constexpr int i = at;
-                    float e = __builtin_amdgcn_exp2f(fmaf(s[T][i] * a8_row<i>(sk[T]), cl.x, -cl.y)) * cl.z;
-                    if (masked) {
-                        const int key = 64 * t + 32 * T + 8 * (i >> 2) + 4 * hf + (i & 3);
-                        e = key >= lo && key < hi ? e : 0.0f;
-                    }
-                    acc[T][i] += e;
+                    s[T][i] = d[T][i] * a8_row<i>(sk[T]);
                 });
+            if (k0 + 32 * NT > all_hi) {  // (uniform) some key is behind a column's last
+                const int hi = __float_as_int(cl.w) - k0 - 4 * hf;
+#pragma unroll
+                for (int T = 0; T < NT; T++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[T][i] = 32 * T + 8 * (i >> 2) + (i & 3) < hi ? s[T][i] : -INFINITY;
+            }
+            if (k0 < all_lo) {  // (uniform) some key is before a window
+                const int lo = max(__float_as_int(cl.w), 0) - A.window - k0 - 4 * hf;
+#pragma unroll
+                for (int T = 0; T < NT; T++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[T][i] = 32 * T + 8 * (i >> 2) + (i & 3) >= lo ? s[T][i] : -INFINITY;
+            }
+            if (w >= 4) ahead(b, buf);
+            __syncthreads();  // the next block's columns are there, this one's readers done
+            x0 += 32;
+            i_first += step_i;
+            g_first += step_g;
+            if (g_first >= A.G) {
+                g_first -= A.G;
+                i_first++;
+            }
         }
+#pragma unroll
+        for (int T = 0; T < NT; T++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) weigh(acc[T][i], s[T][i], cl);
     }
     // over the columns: the sum in every lane of a half, lane c keeps the one of register c
     float v = 0.0f;
 #pragma unroll
-    for (int T = 0; T < 2; T++)
+    for (int T = 0; T < NT; T++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             float a = acc[T][i];
@@ -334,33 +487,67 @@ __global__ void __launch_bounds__(256, 2) k_kv8_weigh(A8 A, Weigh W) {
             a = __uint_as_float(z[0]) + __uint_as_float(z[1]);
             v = c == 16 * T + i ? a : v;
         }
-    const int key = 64 * t + 32 * (c >> 4) + 8 * (c >> 2 & 3) + 4 * hf + (c & 3);
+    if (c >= 16 * NT) return;
+    const int key = k0 + 32 * (c >> 4) + 8 * (c >> 2 & 3) + 4 * hf + (c & 3);
     if (W.chunks > 1) {
-        W.part[((int64_t)chunk * A.nkv + h) * W.keys + key] = v;
+        W.part[((int64_t)chunk * A.nkv + h) * W.keys + key - GK * (int64_t)W.first] = v;
         return;
     }
     const int64_t at = h * W.max_seq + key;
     if (key < len) W.weights[at] = W.prior ? W.prior[at] + v : v;
 }
 
-// weights = prior + the chunks' sums
-__global__ void __launch_bounds__(256) k_kv8_weigh_sum(Weigh W, int64_t len, int nkv) {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int h = blockIdx.y;
-    if (t >= len) return;
+// weights = prior + the chunks' sums; groups of gk keys
+__global__ void __launch_bounds__(256) k_kv8_weigh_sum(A8 A, Weigh W, int gk) {
+    const int t0 = blockIdx.x * 256, t = t0 + threadIdx.x, h = blockIdx.y, group = t0 / gk;
+    int chunks = 0;
+    if (A.n > 0 && group >= W.first) chunks = sv_count(A, W, group, gk);  // (uniform)
+    if (t >= A.max_len) return;
     const int64_t at = h * W.max_seq + t;
+    const float* part = W.part + h * W.keys + t - gk * (int64_t)W.first;
     float v = 0.0f;
-    for (int z = 0; z < W.chunks; z++) v += W.part[((int64_t)z * nkv + h) * W.keys + t];
+#pragma unroll 4
+    for (int z = 0; z < chunks; z++) v += part[(int64_t)z * A.nkv * W.keys];
     W.weights[at] = W.prior ? W.prior[at] + v : v;
 }
 
 // columns whose scores are kept; more are formed again
 constexpr int64_t SCORES = 64;
-bool sv_scores(int64_t seqs, int64_t cols, bool batch) { return batch || cols <= SCORES; }
+bool sv_scores(int64_t cols, bool batch) { return batch || cols <= SCORES; }
 
-int64_t sv_chunks(int64_t cols, int64_t nkv, int64_t len) {
-    const int64_t units = nkv * aeth_cdiv(len, 256);
-    return std::max<int64_t>(1, std::min(aeth_cdiv(4 * (int64_t)aeth_num_cus(), units), aeth_cdiv(cols, 4 * 32)));
+// sums of at most this many groups of keys, in `units` groups of all heads
+int64_t sv_sums(int64_t units) { return 4 * (int64_t)aeth_num_cus() + units; }
+
+// Blocks of columns a workgroup takes. A workgroup fills a CU (eight waves of more than 128 registers) and costs about two
+// blocks beside its own (its keys, the sum over lanes), so: the least rounds·(per + 2) of one to four rounds of workgroups.
+void sv_chunks(Weigh& W, int64_t n, int64_t G, int64_t nkv, int64_t hd, int64_t len, int64_t window) {
+    const int64_t gk = sv_group((int)hd), cus = aeth_num_cus(), end = aeth_cdiv(len, gk), begin = window > 0 ? std::max<int64_t>(0, len - n + 1 - window) / gk : 0;
+    int64_t most = 1, all = 0;
+    auto blocks = [&](int64_t g) { return std::max<int64_t>(1, sv_seen((int)n, (int)G, (int)len, (int)window, gk * g, (int)gk).blocks); };
+    for (int64_t g = begin; g < end; g++) {
+        all += blocks(g);
+        most = std::max(most, blocks(g));
+    }
+    const int64_t units = (end - begin) * nkv, fewest = aeth_cdiv(most, sv_sums(units) / units);
+    int64_t best = most, least = INT64_MAX;
+    for (int64_t rounds = 1; rounds <= 4; rounds++)
+        for (int64_t more = 0; more < 3; more++) {
+            const int64_t per = std::min(std::max(fewest, aeth_cdiv(all * nkv, rounds * cus) + more), most);
+            int64_t wgs = 0;
+            for (int64_t g = begin; g < end; g++) wgs += aeth_cdiv(blocks(g), per);
+            const int64_t cost = aeth_cdiv(wgs * nkv, cus) * (per + 2);
+            if (cost < least) {
+                least = cost;
+                best = per;
+            }
+        }
+    W.per = (int)best;
+    W.chunks = (int)aeth_cdiv(most, best);
+    W.first = W.chunks > 1 ? (int)begin : 0;  // one chunk: every group, those that nothing sees for their prior
+    W.keys = (end - W.first) * gk;
+    W.full = window > 0 ? 0 : (int)(std::min<int64_t>(end, (len - n) / gk + 1));  // those that every query sees
+    W.wgs = 0;
+    for (int64_t g = W.first; g < end; g++) W.wgs += (int)aeth_cdiv(blocks(g), best);
 }
 
 // the workspace's parts, bytes from its start: the attention's own, columns' statistics, scores or sums by chunk
@@ -374,24 +561,35 @@ WeighWs sv_weigh_ws(int64_t seqs, int64_t n, int64_t nq, int64_t nkv, int64_t hd
     w.rest = w.stat + aeth_cdiv(seqs * nkv * cols * 8, 16) * 16;
     // a smaller call may keep scores where the largest does not
     const int64_t scores = seqs * nkv * std::min(cols, std::max(G, SCORES)) * aeth_cdiv(len, KV8_TILE) * KV8_TILE;
-    const int64_t units = nkv * aeth_cdiv(len, 256), sums = cols > SCORES ? (4 * (int64_t)aeth_num_cus() + units) * 256 : 0;
+    const int64_t gk = sv_group((int)hd), sums = cols > SCORES ? sv_sums(nkv * aeth_cdiv(len, gk)) * gk : 0;
     w.end = w.rest + std::max(scores, sums) * 4;
     return w;
 }
 
 template <int HD>
 int sv_weigh(A8 A, Weigh W, const Form& f, int64_t seqs, bool scores, hipStream_t s) {
-    const int rc = scores ? a8_launch<HD, A8_STAT | A8_SCORE>(A, f, seqs, s) : a8_launch<HD, A8_STAT>(A, f, seqs, s);
-    if (rc) return rc;
     if (scores) {
-        hipLaunchKernelGGL(k_kv8_weigh_scores, dim3((unsigned)aeth_cdiv(A.max_len, 1024), (unsigned)A.nkv, (unsigned)seqs), dim3(256), 0, s, A, W);
+        const dim3 block(256);
+        const int64_t pieces = A.nkv * aeth_cdiv(A.max_len, 256), cols = (int64_t)A.nkv * A.cols;
+        hipLaunchKernelGGL((k_attn8<HD, A8_STAT | A8_SCORE>), dim3((unsigned)(A.nkv * A.ncb), (unsigned)seqs, (unsigned)A.chunks), block, 0, s, A);
+        AETH_LAUNCH_CHECK();
+        if (A.chunks == 1) {
+            hipLaunchKernelGGL(k_kv8_weigh_scores<HD>, dim3((unsigned)pieces, (unsigned)seqs), block, 0, s, A, W);
+        } else if (a8_merge_is_some(A, seqs)) {
+            const int64_t joins = aeth_cdiv(cols * (HD / 4), 256);
+            hipLaunchKernelGGL((k_kv8_join_weigh<HD, true>), dim3((unsigned)(joins + pieces), (unsigned)seqs), block, 0, s, A, W, (int)joins);
+        } else {
+            hipLaunchKernelGGL((k_kv8_join_weigh<HD, false>), dim3((unsigned)(cols + pieces), (unsigned)seqs), block, 0, s, A, W, (int)cols);
+        }
         AETH_LAUNCH_CHECK();
         return AETH_OK;
     }
-    hipLaunchKernelGGL(k_kv8_weigh<HD>, dim3((unsigned)aeth_cdiv(A.max_len, 256), (unsigned)A.nkv, (unsigned)W.chunks), dim3(256), 0, s, A, W);
+    const int rc = a8_launch<HD, A8_STAT>(A, f, seqs, s);
+    if (rc) return rc;
+    hipLaunchKernelGGL(k_kv8_weigh<HD>, dim3((unsigned)(A.nkv * W.wgs)), dim3(512), 0, s, A, W);
     AETH_LAUNCH_CHECK();
     if (W.chunks > 1) {
-        hipLaunchKernelGGL(k_kv8_weigh_sum, dim3((unsigned)aeth_cdiv(A.max_len, 256), (unsigned)A.nkv), dim3(256), 0, s, W, (int64_t)A.max_len, A.nkv);
+        hipLaunchKernelGGL(k_kv8_weigh_sum, dim3((unsigned)aeth_cdiv(A.max_len, 256), (unsigned)A.nkv), dim3(256), 0, s, A, W, sv_group(HD));
         AETH_LAUNCH_CHECK();
     }
     return AETH_OK;
@@ -404,7 +602,8 @@ int sv_attn_weights(const char* what, const float* q, int64_t q_stride, const vo
     if (n == 0) q = out = weights;  // no query, no row: either may be NULL
     int rc = aeth_attn_kv8_check(what, q, q_stride, cache, seqs, n, nq, nkv, hd, max_seq, max_len, window, out, ws);
     if (rc) return rc;
-    if (nkv > 65535) return aeth_set_error(AETH_EUNSUPPORTED, "%s: %lld KV heads", what, (long long)nkv);
+    if (nkv * aeth_cdiv(max_len, 256) + nq * n > (int64_t)1 << 23)  // workgroups of up to 512 threads within the grid's 2^32
+        return aeth_set_error(AETH_EUNSUPPORTED, "%s: %lld positions of %lld heads in one call", what, (long long)max_len, (long long)nkv);
     const WeighWs at = sv_weigh_ws(seqs, n, nq, nkv, hd, max_len);
     rc = aeth_attn_kv8_check_ws(what, ws, ws_bytes, at.end);
     if (!rc && lens) rc = aeth_attn_kv8_check_slices(what, seqs, stride, nkv, hd, max_seq);
@@ -413,20 +612,24 @@ int sv_attn_weights(const char* what, const float* q, int64_t q_stride, const vo
     if (prior && prior != weights && (uintptr_t)prior < (uintptr_t)weights + (uint64_t)bytes && (uintptr_t)weights < (uintptr_t)prior + (uint64_t)bytes)
         return aeth_set_error(AETH_EINVAL, "%s: the weights before and after overlap", what);
     if (seqs == 0 || max_len == 0) return AETH_OK;
-    Weigh W = {prior, weights, max_seq, (float*)((char*)ws + at.rest), 0, aeth_cdiv(max_len, 256) * 256};
+    Weigh W = {};
+    W.prior = prior;
+    W.weights = weights;
+    W.max_seq = max_seq;
+    W.part = (float*)((char*)ws + at.rest);
+    A8 A = a8_args(q, q_stride, cache, stride, lens, 0, n, nq, nkv, max_seq, max_len, window, out, ws);
     if (n == 0) {  // no query: the weights as they were
-        hipLaunchKernelGGL(k_kv8_weigh_sum, dim3((unsigned)aeth_cdiv(max_len, 256), (unsigned)nkv), dim3(256), 0, s, W, max_len, (int)nkv);
+        hipLaunchKernelGGL(k_kv8_weigh_sum, dim3((unsigned)aeth_cdiv(max_len, 256), (unsigned)nkv), dim3(256), 0, s, A, W, 256);
         AETH_LAUNCH_CHECK();
         return AETH_OK;
     }
-    A8 A = a8_args(q, q_stride, cache, stride, lens, 0, n, nq, nkv, max_seq, max_len, window, out, ws);
     const Form f = a8_form(seqs, n, A.G, nkv, hd, max_len, A.window, lens != nullptr);
     a8_take(A, f);
     A.stat = (float*)((char*)ws + at.stat);
-    const bool scores = sv_scores(seqs, A.cols, lens != nullptr);
-    A.scores = (float*)((char*)ws + at.rest);
+    const bool scores = sv_scores(A.cols, lens != nullptr);
+    A.scores = W.part;
     A.score_tiles = (int)aeth_cdiv(max_len, KV8_TILE);
-    W.chunks = scores ? 1 : (int)sv_chunks(A.cols, nkv, max_len);
+    if (!scores) sv_chunks(W, n, A.G, nkv, hd, max_len, A.window);
     if (hd == 64) return sv_weigh<64>(A, W, f, seqs, scores, s);
     if (hd == 128) return sv_weigh<128>(A, W, f, seqs, scores, s);
     return sv_weigh<256>(A, W, f, seqs, scores, s);

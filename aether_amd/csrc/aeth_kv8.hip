@@ -386,10 +386,8 @@ __device__ __forceinline__ float qk_sum(float v) {
 }
 
 // hd / 8 lanes a head, four pairs a lane; rows, weights and tables 16-byte aligned
-// Several axes (AXES): pair j's row of the tables is its axis' position of the token, so the four pairs of a lane take their
-// entries one by one. (The table's rows of a token serve all its heads from the cache.)
-template <int HD, bool AXES>
-__device__ __forceinline__ void qk_norm_rope_v(const QkArgs& A, const QkAxes& X) {
+template <int HD>
+__global__ void __launch_bounds__(256) k_qk_norm_rope_v(QkArgs A) {
     constexpr int L = HD / 8, HALF = HD / 2;
     const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / L, all = (uint32_t)A.n * A.heads;  // at most 2^25 units
     const uint32_t u = min(unit, all - 1), row = u / (uint32_t)A.heads;  // past the end: loaded, not stored (whole waves stay active)
@@ -397,18 +395,8 @@ __device__ __forceinline__ void qk_norm_rope_v(const QkArgs& A, const QkAxes& X)
     const int h = (int)(u - row * A.heads), e = 4 * (threadIdx.x % L);
     const float* src = A.x + i * A.x_stride + (int64_t)h * HD + e;
     float4 a = *(const float4*)src, b = *(const float4*)(src + HALF);
-    float4 sn, cs;
-    if constexpr (AXES) {
-        const uint32_t axes = X.axis[e / 4];
-        int64_t at[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) at[j] = qk_row(A, X, i, axes >> (8 * j) & 0xFFu) * HALF + e + j;
-        sn = make_float4(A.sin_t[at[0]], A.sin_t[at[1]], A.sin_t[at[2]], A.sin_t[at[3]]);
-        cs = make_float4(A.cos_t[at[0]], A.cos_t[at[1]], A.cos_t[at[2]], A.cos_t[at[3]]);
-    } else {
-        const int64_t p = qk_row(A, i);
-        sn = *(const float4*)(A.sin_t + p * HALF + e), cs = *(const float4*)(A.cos_t + p * HALF + e);
-    }
+    const int64_t p = qk_row(A, i);
+    const float4 sn = *(const float4*)(A.sin_t + p * HALF + e), cs = *(const float4*)(A.cos_t + p * HALF + e);
     const float* w = h < A.nq ? A.qw : A.kw;
     if (A.qw || A.kw) {  // (uniform)
         const float4 wa = w ? *(const float4*)(w + e) : make_float4(1, 1, 1, 1), wb = w ? *(const float4*)(w + e + HALF) : wa;
@@ -425,10 +413,51 @@ __device__ __forceinline__ void qk_norm_rope_v(const QkArgs& A, const QkAxes& X)
     __builtin_nontemporal_store((kv8_f4){b.x, b.y, b.z, b.w}, (kv8_f4*)(dst + HALF));
 }
 
-template <int HD>
-__global__ void __launch_bounds__(256) k_qk_norm_rope_v(QkArgs A) { qk_norm_rope_v<HD, false>(A, {}); }
-template <int HD>
-__global__ void __launch_bounds__(256) k_qk_norm_rope_axes_v(QkArgs A, QkAxes X) { qk_norm_rope_v<HD, true>(A, X); }
+// Σx² of four, rounded as it is in k_qk_norm_rope_v: where the axes agree both give the same bits
+__device__ __forceinline__ float qk_squares(float4 a) { return fmaf(a.x, a.x, a.y * a.y) + fmaf(a.z, a.z, a.w * a.w); }
+
+// Several axes: the four pairs of a lane take their table entries one by one, each from the row of its axis' position, and
+// serve HEADS heads of the token.
+template <int HD, int HEADS>
+__global__ void __launch_bounds__(256) k_qk_norm_rope_axes_v(QkArgs A, QkAxes X) {
+    constexpr int L = HD / 8, HALF = HD / 2;
+    const uint32_t groups = ((uint32_t)A.heads + HEADS - 1) / HEADS;  // of a row
+    const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / L, all = (uint32_t)A.n * groups;  // at most 2^25 units
+    const uint32_t u = min(unit, all - 1), row = u / groups;  // past the end: loaded, not stored (whole waves stay active)
+    const int64_t i = row;
+    const int h0 = (int)(u - row * groups) * HEADS, e = 4 * (threadIdx.x % L);
+    const float* src = A.x + i * A.x_stride + e;
+    float4 a[HEADS], b[HEADS];
+#pragma unroll
+    for (int j = 0; j < HEADS; j++) {
+        const float* p = src + (int64_t)min(h0 + j, A.heads - 1) * HD;
+        a[j] = *(const float4*)p;
+        b[j] = *(const float4*)(p + HALF);
+    }
+    const uint32_t axes = X.axis[e / 4];
+    int64_t at[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) at[j] = qk_row(A, X, i, axes >> (8 * j) & 0xFFu) * HALF + e + j;
+    const float4 sn = make_float4(A.sin_t[at[0]], A.sin_t[at[1]], A.sin_t[at[2]], A.sin_t[at[3]]);
+    const float4 cs = make_float4(A.cos_t[at[0]], A.cos_t[at[1]], A.cos_t[at[2]], A.cos_t[at[3]]);
+#pragma unroll
+    for (int j = 0; j < HEADS; j++) {
+        const int h = min(h0 + j, A.heads - 1);
+        const float* w = h < A.nq ? A.qw : A.kw;
+        if (A.qw || A.kw) {  // (uniform)
+            const float4 wa = w ? *(const float4*)(w + e) : make_float4(1, 1, 1, 1), wb = w ? *(const float4*)(w + e + HALF) : wa;
+            const float ss = qk_sum<L>(qk_squares(a[j]) + qk_squares(b[j]));
+            const float rms = w ? sqrtf(ss / (float)HD + A.eps) : 1.0f;
+            a[j] = make_float4(a[j].x / rms * wa.x, a[j].y / rms * wa.y, a[j].z / rms * wa.z, a[j].w / rms * wa.w);
+            b[j] = make_float4(b[j].x / rms * wb.x, b[j].y / rms * wb.y, b[j].z / rms * wb.z, b[j].w / rms * wb.w);
+        }
+        kv8_rotate(a[j], b[j], sn, cs);
+        if (unit >= all || h0 + j >= A.heads) continue;
+        float* dst = A.out + i * A.out_stride + (int64_t)h * HD + e;
+        __builtin_nontemporal_store((kv8_f4){a[j].x, a[j].y, a[j].z, a[j].w}, (kv8_f4*)dst);
+        __builtin_nontemporal_store((kv8_f4){b[j].x, b[j].y, b[j].z, b[j].w}, (kv8_f4*)(dst + HALF));
+    }
+}
 
 // any even hd, any alignment: a wave a head, lanes over the pairs (read again for the rotation: the row is in cache)
 template <bool AXES>
@@ -463,6 +492,13 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(QkArgs A) { qk_norm_rope<f
 __global__ void __launch_bounds__(256) k_qk_norm_rope_axes(QkArgs A, QkAxes X) { qk_norm_rope<true>(A, X); }
 }  // namespace
 
+template <int HD>
+static void qk_launch_axes(const QkArgs& A, const QkAxes& X, hipStream_t s) {
+    auto grid = [&](int64_t heads) { return dim3((unsigned)aeth_cdiv(A.n * aeth_cdiv(A.heads, heads) * (HD / 8), 256)); };
+    if (grid(4).x >= 4u * (unsigned)aeth_num_cus()) hipLaunchKernelGGL((k_qk_norm_rope_axes_v<HD, 4>), grid(4), dim3(256), 0, s, A, X);
+    else hipLaunchKernelGGL((k_qk_norm_rope_axes_v<HD, 1>), grid(1), dim3(256), 0, s, A, X);
+}
+
 // X: several axes (nullptr: one)
 static int qk_launch(const QkArgs& A, const QkAxes* X, hipStream_t s) {
     if (A.n <= 0 || A.heads <= 0) return AETH_OK;
@@ -473,9 +509,9 @@ static int qk_launch(const QkArgs& A, const QkAxes* X, hipStream_t s) {
     if (al16 && (hd == 64 || hd == 128 || hd == 256)) {
         const dim3 grid((unsigned)aeth_cdiv(A.n * A.heads * (hd / 8), 256));
         if (X) {
-            if (hd == 64) hipLaunchKernelGGL(k_qk_norm_rope_axes_v<64>, grid, block, 0, s, A, *X);
-            else if (hd == 128) hipLaunchKernelGGL(k_qk_norm_rope_axes_v<128>, grid, block, 0, s, A, *X);
-            else hipLaunchKernelGGL(k_qk_norm_rope_axes_v<256>, grid, block, 0, s, A, *X);
+            if (hd == 64) qk_launch_axes<64>(A, *X, s);
+            else if (hd == 128) qk_launch_axes<128>(A, *X, s);
+            else qk_launch_axes<256>(A, *X, s);
         } else {
             if (hd == 64) hipLaunchKernelGGL(k_qk_norm_rope_v<64>, grid, block, 0, s, A);
             else if (hd == 128) hipLaunchKernelGGL(k_qk_norm_rope_v<128>, grid, block, 0, s, A);

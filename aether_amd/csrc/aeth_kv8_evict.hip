@@ -18,6 +18,17 @@
 
 namespace {
 
+// sums of the values of a wave's lanes up to and with each
+__device__ __forceinline__ uint32_t ev_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8: within rows of 16
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);  // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
 struct EvictArgs {
     const uint8_t* cache;  // slice of the first sequence
     int64_t seq_bytes;
@@ -44,139 +55,156 @@ __device__ __forceinline__ int64_t ev_len(const EvictArgs& A, int seq) {
     return A.lens ? min(max((int64_t)A.lens[seq], (int64_t)0), A.max_len) : A.max_len;
 }
 
-// weights as whole numbers in their order
+// Weights as whole numbers in their order: NaN 1, -Inf 0x007FFFFF, +Inf 0xFF800000. What stays in any case has EV_STAYS, no slot 0,
+// so that the kept ones are the `keep` largest.
+constexpr uint32_t EV_STAYS = 0xFFFFFFFFu;
 __device__ __forceinline__ uint32_t ev_key(float w) {
-    uint32_t f = __float_as_uint(w);
-    f = f == 0x80000000u ? 0 : f;
-    if ((f & 0x7FFFFFFFu) > 0x7F800000u) return 0;
-    return f & 0x80000000u ? ~f : f | 0x80000000u;
+    const float y = w + 0.0f;  // -0 + 0 is 0
+    const uint32_t f = __float_as_uint(y);
+    return y != y ? 1u : f ^ ((uint32_t)((int)f >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ uint32_t ev_rank(uint64_t lanes) {  // of them those before this lane
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
 }
 
-constexpr int SEL = 1024;  // threads of a selection
+constexpr int SEL = 1024, PER = 32;  // threads of a selection, weights a thread holds
 
-// exclusive prefix sums of two counts below 2^16 each over the workgroup, packed in one word, and their totals
-__device__ __forceinline__ uint32_t ev_scan(uint32_t v, uint32_t (*part)[SEL / 64], int round, uint32_t& total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    uint32_t x = v;
+// f(0) .. f(J - 1) and on to a multiple of 8, eight at a time (a jump over each of the others would fetch its code)
+template <class F>
+__device__ __forceinline__ void ev_each(int J, F&& f) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t y = __shfl_up(x, d, 64);
-        x += lane >= d ? y : 0;
-    }
-    if (lane == 63) part[round & 1][w] = x;
-    __syncthreads();  // (the other buffer's readers have passed the barrier before this one)
-    uint32_t before = 0;
-    total = 0;
+    for (int g = 0; g < PER; g += 8) {
+        if (g >= J) break;  // (uniform)
 #pragma unroll
-    for (int i = 0; i < SEL / 64; i++) {
-        const uint32_t y = part[round & 1][i];
-        before += i < w ? y : 0;
-        total += y;
+        for (int j = 0; j < 8; j++) f(g + j);
     }
-    return before + x - v;
 }
 
-// One workgroup a head: the key of the last token chosen by three passes over its bits (11, 11, 10) with counts in LDS,
-// then one pass that numbers the kept slots in order.
+// One workgroup a head. Its waves hold 32768 weights and their keys in registers, a wave 64·J consecutive ones (lane l, register j:
+// 64·j + l of them), so that a rank among them is a count of bits. The key of the last token kept is found by up to three passes over the
+// keys' bits (11, 11, 10) with counts in LDS, the kept slots numbered in a last one; a head of more tokens reads its weights again in each
+// pass. What bounds it is instructions, on one CU a head: hence one word that says all of a token.
 __global__ void __launch_bounds__(SEL) k_kv8_select(EvictArgs A) {
-    __shared__ uint32_t hist[2048];
-    __shared__ uint32_t part[2][SEL / 64];
-    __shared__ uint32_t found[2];
-    const int tid = threadIdx.x, h = blockIdx.x, seq = blockIdx.y;
-    const int64_t len = ev_len(A, seq), unit = (int64_t)seq * A.nkv + h;
+    __shared__ __attribute__((aligned(16))) uint32_t hist[2048][4];  // a copy for every fourth lane: weights fill few bins, and lanes of one wait for each other
+    __shared__ uint32_t part[2][SEL / 64], sums[2][SEL / 64];
+    __shared__ uint32_t found[3];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = blockIdx.x, seq = blockIdx.y;
+    const int len = (int)ev_len(A, seq);
+    const int64_t unit = (int64_t)seq * A.nkv + h;
     const float* w = A.weights + unit * A.max_seq;
     int* list = A.list + unit * A.list_stride;
     float* kw = A.kept_weights + unit * A.most;
-    const int64_t rows = min(len, A.keep);
-    if (tid == 0) A.rows[unit] = (int)rows;
+    if (tid == 0) A.rows[unit] = (int)min((int64_t)len, A.keep);
     if (len <= A.keep) {  // (uniform) all stay
-        for (int64_t t = tid; t < len; t += SEL) {
-            list[t] = (int)t;
+        for (int t = tid; t < len; t += SEL) {
+            list[t] = t;
             kw[t] = w[t];
         }
         return;
     }
-    const int64_t lo = A.first, hi = len - A.recent;  // the slots to choose from
-    uint32_t need = (uint32_t)(A.keep - A.first - A.recent), prefix = 0;
-    if (need > 0) {  // (uniform)
-        int done = 0;
-        for (int pass = 0; pass < 3; pass++) {
-            const int bits = pass < 2 ? 11 : 10, shift = 32 - done - bits;
-            for (int i = tid; i < 2048; i += SEL) hist[i] = 0;
-            __syncthreads();
-            for (int64_t t = lo + tid; t < hi; t += SEL) {
-                const uint32_t k = ev_key(w[t]);
-                if (done == 0 || k >> (32 - done) == prefix) atomicAdd(&hist[k >> shift & ((1u << bits) - 1)], 1u);
+    if (A.keep == 0) return;  // (uniform)
+    const int lo = (int)A.first, hi = len - (int)A.recent;  // the slots to choose from
+    float v[PER];
+    uint32_t key[PER];
+    int J = 0, first = 0;  // registers in use, the lane's slot in register 0
+    auto load = [&](int base) {
+        const int n = min(SEL * PER, len - base);
+        J = (n + SEL - 1) / SEL;
+        first = base + 64 * J * wv + lane;
+        const int from = base + 64 * J * wv, end = min(len, from + 64 * J);
+        ev_each(J, [&](int j) { v[j] = w[(uint32_t)min(first + 64 * j, len - 1)]; });
+        ev_each(J, [&](int j) {
+            key[j] = ev_key(v[j]);
+            if (from + 64 * j < lo || from + 64 * j + 64 > min(hi, end)) {  // (uniform)
+                const int t = first + 64 * j;
+                key[j] = t >= end ? 0u : t < lo || t >= hi ? EV_STAYS : key[j];
             }
-            __syncthreads();
-            // the bin in which the need-th from the top lies: counts above each pair of bins
-            const int b = 2046 - 2 * tid;  // thread 0: the highest two
-            const uint32_t c1 = hist[b + 1], c0 = hist[b];
-            // counts may pass 2^16: a scan of whole words
-            uint32_t x = c0 + c1;
-            const int lane = tid & 63, wv = tid >> 6;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint32_t y = __shfl_up(x, d, 64);
-                x += lane >= d ? y : 0;
-            }
-            if (lane == 63) part[0][wv] = x;
-            __syncthreads();
-            uint32_t above = x - c0 - c1;
-            for (int i = 0; i < wv; i++) above += part[0][i];
-            if (above < need && need <= above + c1) {
-                found[0] = b + 1;
-                found[1] = above;
-            } else if (above + c1 < need && need <= above + c1 + c0) {
-                found[0] = b;
-                found[1] = above + c1;
-            }
-            __syncthreads();
-            prefix = prefix << bits | found[0];
-            need -= found[1];
-            done += bits;
+        });
+    };
+    const bool whole = len <= SEL * PER;
+    uint32_t need = (uint32_t)A.keep, last = 0, prefix = 0;  // keys above `last` are taken, and `need` equal to it
+    uint32_t equals = 0, sures = 0;                           // of them passed so far
+    int done = 0, bits = 11, round = 0;                      // bits of the last one's key that are known, and that a pass adds
+    for (int pass = 0;; pass++) {
+        if (bits > 0) {
+            for (int i = tid; i < 2048; i += SEL) *(uint4*)hist[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
         }
-    }
-    // prefix: the key of the last one chosen; `need` of its equals, from the lowest slot on. need 0 from the start: none
-    const bool some = A.keep > A.first + A.recent;
-    uint32_t equals = 0;
-    int64_t at = 0;  // equal keys passed and slots listed so far
-    int round = 0;
-    for (int64_t t0 = 0; t0 < len; t0 += 4 * SEL, round++) {
-        uint32_t key[4];
-        float wt[4];
-        bool sure[4], equal[4];
-        uint32_t n_eq = 0, n_sure = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int64_t t = t0 + 4 * tid + j;
-            wt[j] = t < len ? w[t] : 0.0f;
-            key[j] = ev_key(wt[j]);
-            const bool ends = t < len && (t < lo || t >= hi), mid = t >= lo && t < hi;
-            sure[j] = ends || (mid && some && key[j] > prefix);
-            equal[j] = mid && some && key[j] == prefix;
-            n_eq += equal[j];
-            n_sure += sure[j];
-        }
-        uint32_t total;
-        const uint32_t before = ev_scan(n_sure << 16 | n_eq, part, round, total);
-        // equals taken before a slot: those passed, up to `need`
-        uint32_t eq = equals + (before & 0xFFFFu);
-        int64_t pos = at + (before >> 16) + min(eq, need) - min(equals, need);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const bool take = sure[j] || (equal[j] && eq < need);
-            eq += equal[j];
-            if (take) {
-                list[pos] = (int)(t0 + 4 * tid + j);
-                kw[pos] = wt[j];
-                pos++;
+        for (int base = 0; base < len; base += SEL * PER) {
+            if (pass == 0 || !whole) load(base);
+            if (bits > 0) {  // (uniform) count
+                const int shift = 32 - done - bits;
+                const uint32_t low = bits < 32 - shift ? prefix << bits : 0;  // (nothing known: 0)
+                uint32_t* mine = &hist[0][lane & 3];
+                ev_each(J, [&](int j) {
+                    const uint32_t bin = (key[j] >> shift) - low;
+                    if (bin < 1u << bits) atomicAdd(mine + 4 * bin, 1u);
+                });
+                continue;
             }
+            uint32_t ns = 0, ne = 0;  // (uniform) the wave's
+            ev_each(J, [&](int j) {
+                ns += (uint32_t)__popcll(__ballot(key[j] > last));
+                ne += (uint32_t)__popcll(__ballot(key[j] == last));
+            });
+            if (lane == 0) {
+                part[round][wv] = ns;
+                sums[round][wv] = ne;
+            }
+            __syncthreads();  // (the other buffers' readers have passed the barrier before this one)
+            uint32_t s0 = sures, e0 = equals;
+#pragma unroll
+            for (int i = 0; i < SEL / 64; i++) {
+                const uint32_t a = part[round][i], b = sums[round][i];
+                s0 += i < wv ? a : 0;
+                e0 += i < wv ? b : 0;
+                sures += a;
+                equals += b;
+            }
+            round ^= 1;
+            ev_each(J, [&](int j) {
+                const bool sure = key[j] > last, equal = key[j] == last;
+                const uint64_t ms = __ballot(sure), me = __ballot(equal);
+                const uint32_t e = e0 + ev_rank(me), at = s0 + ev_rank(ms) + min(e, need);
+                if (sure || (equal && e < need)) {
+                    list[at] = first + 64 * j;
+                    kw[at] = v[j];
+                }
+                s0 += (uint32_t)__popcll(ms);
+                e0 += (uint32_t)__popcll(me);
+            });
         }
-        const uint32_t all = equals + (total & 0xFFFFu);
-        at += (total >> 16) + min(all, need) - min(equals, need);
-        equals = all;
+        if (bits == 0) return;
+        __syncthreads();
+        // the bin in which the need-th from the top lies: counts above each pair of bins
+        const int b = 2046 - 2 * tid;  // thread 0: the highest two
+        const uint4 h1 = *(const uint4*)hist[b + 1], h0 = *(const uint4*)hist[b];
+        const uint32_t c1 = h1.x + h1.y + h1.z + h1.w, c0 = h0.x + h0.y + h0.z + h0.w, x = ev_scan(c0 + c1);
+        if (lane == 63) part[0][wv] = x;
+        __syncthreads();
+        uint32_t above = x - c0 - c1;
+#pragma unroll
+        for (int i = 0; i < SEL / 64; i++) above += i < wv ? part[0][i] : 0;
+        if (above < need && need <= above + c1) {
+            found[0] = b + 1;
+            found[1] = above;
+            found[2] = c1;
+        } else if (above + c1 < need && need <= above + c1 + c0) {
+            found[0] = b;
+            found[1] = above + c1;
+            found[2] = c0;
+        }
+        __syncthreads();
+        prefix = prefix << bits | found[0];
+        need -= found[1];
+        done += bits;
+        last = prefix;
+        bits = done == 22 ? 10 : done == 32 ? 0 : 11;
+        if (found[2] == need) {  // (uniform) the whole bin; its lowest key is above 0: fewer stay than there are
+            last = (prefix << (32 - done)) - 1;  // (done 32: a shift by 0)
+            need = 0;
+            bits = 0;
+        }
     }
 }
 
