@@ -213,7 +213,14 @@ __device__ __forceinline__ void sv_weigh_scores(const A8& A, const Weigh& W, int
     const int64_t unit = (int64_t)seq * A.nkv + h, row = 64 * (int64_t)A.score_tiles, at = unit * W.max_seq + t;
     const float* src = A.scores + unit * A.cols * row + min(t, (int)row - 1);
     const bool real = t < len;
-    float acc = real && W.prior ? W.prior[at] : 0.0f, sum = 0.0f;
+    float s[4];  // four columns' scores, asked for before what their sums wait for
+    auto fetch = [&](int x) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[j] = src[min(x + j, A.cols - 1) * row];
+    };
+    fetch(0);
+    const float prior = real && W.prior ? W.prior[at] : 0.0f;
+    float sum = 0.0f;
     for (int c0 = 0; c0 < A.cols; c0 += 32) {
         const int count = min(32, A.cols - c0);
         if (c0 > 0) __syncthreads();
@@ -224,18 +231,16 @@ __device__ __forceinline__ void sv_weigh_scores(const A8& A, const Weigh& W, int
         __syncthreads();
         const int hi0 = len - A.n + 1;
         for (int c1 = 0; c1 < count; c1 += 4) {
-            float s[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) s[j] = src[min(c0 + c1 + j, A.cols - 1) * row];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int x = c0 + c1 + j, hi = hi0 + x / A.G, lo = A.window > 0 ? hi - A.window : 0;  // (uniform)
                 const float2 ml = col[min(c1 + j, 31)];
                 if (x < A.cols && t >= lo && t < hi) sum = fmaf(__builtin_amdgcn_exp2f(s[j] - ml.x), ml.y, sum);
             }
+            if (c0 + c1 + 4 < A.cols) fetch(c0 + c1 + 4);
         }
     }
-    if (real) W.weights[at] = acc + sum;
+    if (real) W.weights[at] = prior + sum;
 }
 
 template <int HD>
@@ -395,8 +400,13 @@ __global__ void __launch_bounds__(512, 2) k_kv8_weigh(A8 A, Weigh W) {
                 kf[T][s] = (a8_h8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
             }
         }
+        // Some column of the blocks [w0, w1) sees a key of the wave. (At a prompt's diagonal half of the waves see none, and the others have
+        // the SIMD to themselves.)
+        const int64_t d0 = (int64_t)(k0 - past) * A.G - sees.x_beg, d1 = (int64_t)(k0 - past + 32 * NT - 1 + A.window) * A.G - sees.x_beg;
+        const int w0 = (int)min(max(d0 >> 5, (int64_t)b0), (int64_t)b1);
+        const int w1 = A.window > 0 ? (int)min(max((d1 + 31) >> 5, (int64_t)w0), (int64_t)b1) : b1;
         // the first and last query of a block: every column of it sees the keys [all_lo, all_hi)
-        int x0 = sees.x_beg + 32 * b0, i_first = x0 / A.G, g_first = x0 % A.G;
+        int x0 = sees.x_beg + 32 * w0, i_first = x0 / A.G, g_first = x0 % A.G;
         a8_f16 s[NT];       // a block's scores, from one block to the next
 #pragma unroll
         for (int T = 0; T < NT; T++) s[T] = (a8_f16){};
@@ -412,7 +422,15 @@ __global__ void __launch_bounds__(512, 2) k_kv8_weigh(A8 A, Weigh W) {
         stage(0);
         if (b0 + 1 < b1) fetch();
         __syncthreads();
-        for (int b = b0; b < b1; b++) {
+        int b = b0;
+        auto pass = [&](int end) {
+            for (; b < end; b++) {
+                ahead(b, (b - b0) & 1);
+                __syncthreads();
+            }
+        };
+        pass(w0);
+        for (; b < w1; b++) {
             const int buf = (b - b0) & 1;
             if (w < 4) ahead(b, buf);
             const char* qp = qb[buf] + lane * 16;
@@ -471,6 +489,7 @@ __global__ void __launch_bounds__(512, 2) k_kv8_weigh(A8 A, Weigh W) {
         for (int T = 0; T < NT; T++)
 #pragma unroll
             for (int i = 0; i < 16; i++) weigh(acc[T][i], s[T][i], cl);
+        pass(b1);
     }
     // over the columns: the sum in every lane of a half, lane c keeps the one of register c
     float v = 0.0f;

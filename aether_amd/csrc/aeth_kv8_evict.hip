@@ -42,7 +42,7 @@ struct EvictArgs {
     float* dst_weights;    // [seqs][nkv][dst_seq]; nullptr: not moved
     int* dst_lens;         // [seqs]; nullptr: not written
     // between the steps: tokens kept [seqs][nkv]; their slots and weights [seqs][nkv][keep]
-    int* rows;
+    int* rows;             // (the lengths may be overwritten before the last step)
     int* list;
     int64_t list_stride;
     float* kept_weights;
@@ -69,14 +69,14 @@ __device__ __forceinline__ uint32_t ev_rank(uint64_t lanes) {  // of them those 
 
 constexpr int SEL = 1024, PER = 32;  // threads of a selection, weights a thread holds
 
-// f(0) .. f(J - 1) and on to a multiple of 8, eight at a time (a jump over each of the others would fetch its code)
+// f(0) .. f(J - 1) and on to a multiple of 4, four at a time (a jump over each of the others would fetch its code)
 template <class F>
 __device__ __forceinline__ void ev_each(int J, F&& f) {
 #pragma unroll
-    for (int g = 0; g < PER; g += 8) {
+    for (int g = 0; g < PER; g += 4) {
         if (g >= J) break;  // (uniform)
 #pragma unroll
-        for (int j = 0; j < 8; j++) f(g + j);
+        for (int j = 0; j < 4; j++) f(g + j);
     }
 }
 
@@ -108,11 +108,12 @@ __global__ void __launch_bounds__(SEL) k_kv8_select(EvictArgs A) {
     uint32_t key[PER];
     int J = 0, first = 0;  // registers in use, the lane's slot in register 0
     auto load = [&](int base) {
-        const int n = min(SEL * PER, len - base);
-        J = (n + SEL - 1) / SEL;
+        J = (min(SEL * PER, len - base) + SEL - 1) / SEL;
         first = base + 64 * J * wv + lane;
-        const int from = base + 64 * J * wv, end = min(len, from + 64 * J);
         ev_each(J, [&](int j) { v[j] = w[(uint32_t)min(first + 64 * j, len - 1)]; });
+    };
+    auto keys = [&]() {
+        const int from = first - lane, end = min(len, from + 64 * J);
         ev_each(J, [&](int j) {
             key[j] = ev_key(v[j]);
             if (from + 64 * j < lo || from + 64 * j + 64 > min(hi, end)) {  // (uniform)
@@ -126,12 +127,13 @@ __global__ void __launch_bounds__(SEL) k_kv8_select(EvictArgs A) {
     uint32_t equals = 0, sures = 0;                           // of them passed so far
     int done = 0, bits = 11, round = 0;                      // bits of the last one's key that are known, and that a pass adds
     for (int pass = 0;; pass++) {
-        if (bits > 0) {
-            for (int i = tid; i < 2048; i += SEL) *(uint4*)hist[i] = make_uint4(0, 0, 0, 0);
-            __syncthreads();
-        }
         for (int base = 0; base < len; base += SEL * PER) {
             if (pass == 0 || !whole) load(base);
+            if (bits > 0 && base == 0) {  // beside the loads
+                for (int i = tid; i < 2048; i += SEL) *(uint4*)hist[i] = make_uint4(0, 0, 0, 0);
+                __syncthreads();
+            }
+            if (pass == 0 || !whole) keys();
             if (bits > 0) {  // (uniform) count
                 const int shift = 32 - done - bits;
                 const uint32_t low = bits < 32 - shift ? prefix << bits : 0;  // (nothing known: 0)
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(256) k_kv8_gather(EvictArgs A, uint8_t* dst, i
     __shared__ int from[KV8_TILE];
     const int tile = blockIdx.x, h = blockIdx.y, seq = blockIdx.z;
     const int64_t unit = (int64_t)seq * A.nkv + h;
-    const int64_t rows = A.rows[unit];
+    const int64_t rows = A.lens ? A.rows[unit] : A.most;
     if (tile >= A.gather_blocks) {  // (uniform)
         ev_weights(A, unit, rows, tile - A.gather_blocks);
         return;
@@ -290,7 +292,7 @@ __global__ void __launch_bounds__(256) k_kv8_put_back(EvictArgs A, const uint8_t
     __shared__ int from[KV8_TILE];
     constexpr int64_t TB = aeth_kv8_tile_bytes(HD);
     const int tile = blockIdx.x, h = blockIdx.y, seq = blockIdx.z;
-    const int64_t unit = (int64_t)seq * A.nkv + h, rows = A.rows[unit], t0 = (int64_t)tile * KV8_TILE;
+    const int64_t unit = (int64_t)seq * A.nkv + h, rows = A.lens ? A.rows[unit] : A.most, t0 = (int64_t)tile * KV8_TILE;
     const int n = (int)min((int64_t)KV8_TILE, rows - t0);
     if (n <= 0) return;  // (uniform)
     const int* list = A.list + unit * A.list_stride + t0;
