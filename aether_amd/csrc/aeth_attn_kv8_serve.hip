@@ -8,7 +8,7 @@
 // their parts in the workspace and k_attn8_join joins them.
 //
 // The weights that tokens receive. weights[t] = prior[t] + Σ_x 2^(s_x(t) - m_x) / l_x over the columns x that see t. m_x and l_x are
-// known behind the attention. Up to 64 columns its workgroups also leave their scores, 4 bytes a column and key where a
+// known behind the attention. Of few columns (SCORES) its workgroups also leave their scores, 4 bytes a column and key where a
 // key's codes are 2·hd + 8 (k_kv8_weigh_scores); of more the scores are formed once more from the keys (k_kv8_weigh), where they are summed
 // over columns in registers: no score reaches memory. Every sum has a fixed order.
 #include "aeth_attn_kv8_dev.hpp"
@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(512, 2) k_kv8_weigh(A8 A, Weigh W) {
                     for (int i = 0; i < 16; i++) s[T][i] = 32 * T + 8 * (i >> 2) + (i & 3) < hi ? s[T][i] : -INFINITY;
             }
             if (k0 < all_lo) {  // (uniform) some key is before a window
-                const int lo = max(__float_as_int(cl.w), 0) - A.window - k0 - 4 * hf;
+                const int lo = max(__float_as_int(cl.w) - k0 - 4 * hf, -64) - A.window;  // (a column that sees no key here is masked above)
 #pragma unroll
                 for (int T = 0; T < NT; T++)
 #pragma unroll
@@ -530,8 +530,10 @@ __global__ void __launch_bounds__(256) k_kv8_weigh_sum(A8 A, Weigh W, int gk) {
     W.weights[at] = W.prior ? W.prior[at] + v : v;
 }
 
-// columns whose scores are kept; more are formed again
-constexpr int64_t SCORES = 64;
+// Columns whose scores are kept; more are formed again. 32 / 8 heads of 128, 20000 tokens, µs with kept / formed scores: 28 columns (7 queries)
+// 32.3 / 38.8, 40 41.0 / 45.2, 48 44.2 / 44.7, 56 49.9 / 46.8, 64 54.0 / 47.1; 2000 tokens: 48 22.3 / 23.5, 64 26.7 / 23.5. A batch, of one query
+// a sequence, keeps them however many query heads a KV head has.
+constexpr int64_t SCORES = 48;
 bool sv_scores(int64_t cols, bool batch) { return batch || cols <= SCORES; }
 
 // sums of at most this many groups of keys, in `units` groups of all heads
@@ -678,6 +680,8 @@ extern "C" AETH_API int aeth_attn_kv8_shared(const float* d_q, int64_t q_stride,
     if (!rc) rc = aeth_attn_kv8_check_slices(what, n_seqs, layer_stride, kv_heads, head_dim, max_seq);
     if (!rc && prefix_len > KV8_MAX_SEQ - max_len)
         rc = aeth_set_error(AETH_EINVAL, "%s: %lld tokens behind %lld", what, (long long)max_len, (long long)prefix_len);
+    if (!rc && n_seqs * kv_heads * aeth_cdiv(n_heads / kv_heads, 16) > (int64_t)1 << 22)  // workgroups of 256 threads within the grid's 2^32
+        rc = aeth_set_error(AETH_EUNSUPPORTED, "%s: %lld sequences of %lld heads in one call", what, (long long)n_seqs, (long long)n_heads);
     if (rc || n_seqs == 0) return rc;
     const int64_t own = sv_own_ws(n_seqs, n_heads, kv_heads, head_dim);
     rc = aeth_attn_kv8_check_ws(what, d_ws, ws_bytes, own + (prefix_len > 0 ? sv_prefix_ws(n_seqs, n_heads, kv_heads, head_dim) : 0));
@@ -696,6 +700,12 @@ extern "C" AETH_API int aeth_attn_kv8_shared(const float* d_q, int64_t q_stride,
 extern "C" AETH_API int64_t aeth_attn_kv8_weights_ws_bytes(int64_t n_seqs, int64_t n, int64_t n_heads, int64_t kv_heads, int64_t head_dim,
                                                            int64_t max_len) {
     if (aeth_attn_kv8_ws_bytes(n_seqs, n, n_heads, kv_heads, head_dim, max_len) < 0) {
+        aeth_set_error(AETH_EINVAL, "aeth_attn_kv8_weights_ws_bytes: bad shape");
+        return -1;
+    }
+    int64_t all;  // the scores of the largest, as sv_weigh_ws has them
+    if (!aeth_mul_ok(n_seqs * kv_heads, std::min(n * (n_heads / kv_heads), std::max(n_heads / kv_heads, SCORES)), &all) ||
+        !aeth_mul_ok(all, max_len + KV8_TILE, &all) || all > (int64_t)1 << 58) {
         aeth_set_error(AETH_EINVAL, "aeth_attn_kv8_weights_ws_bytes: bad shape");
         return -1;
     }

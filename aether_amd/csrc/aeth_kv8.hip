@@ -440,12 +440,20 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_axes_v(QkArgs A, QkAxes X)
     for (int j = 0; j < 4; j++) at[j] = qk_row(A, X, i, axes >> (8 * j) & 0xFFu) * HALF + e + j;
     const float4 sn = make_float4(A.sin_t[at[0]], A.sin_t[at[1]], A.sin_t[at[2]], A.sin_t[at[3]]);
     const float4 cs = make_float4(A.cos_t[at[0]], A.cos_t[at[1]], A.cos_t[at[2]], A.cos_t[at[3]]);
+    // the weights of the first head's kind, which nearly always serve the others too
+    const float* w0 = h0 < A.nq ? A.qw : A.kw;
+    const float4 one = make_float4(1, 1, 1, 1), wa0 = w0 ? *(const float4*)(w0 + e) : one, wb0 = w0 ? *(const float4*)(w0 + e + HALF) : one;
 #pragma unroll
     for (int j = 0; j < HEADS; j++) {
         const int h = min(h0 + j, A.heads - 1);
-        const float* w = h < A.nq ? A.qw : A.kw;
         if (A.qw || A.kw) {  // (uniform)
-            const float4 wa = w ? *(const float4*)(w + e) : make_float4(1, 1, 1, 1), wb = w ? *(const float4*)(w + e + HALF) : wa;
+            const float* w = w0;
+            float4 wa = wa0, wb = wb0;
+            if (h0 < A.nq && h >= A.nq) {
+                w = A.kw;
+                wa = w ? *(const float4*)(w + e) : one;
+                wb = w ? *(const float4*)(w + e + HALF) : one;
+            }
             const float ss = qk_sum<L>(qk_squares(a[j]) + qk_squares(b[j]));
             const float rms = w ? sqrtf(ss / (float)HD + A.eps) : 1.0f;
             a[j] = make_float4(a[j].x / rms * wa.x, a[j].y / rms * wa.y, a[j].z / rms * wa.z, a[j].w / rms * wa.w);

@@ -3,7 +3,7 @@
 // Of a head's len tokens `keep` stay: the first `first`, the last `recent`, and of the others the
 // keep - first - recent of largest weight, the lower slot before the higher where weights are equal
 // (NaN is below every number, -0 equals 0). They keep their order, their codes and their scales: a kept
-// token stands for the same values as before. Three steps: the list of kept slots by head (k_kv8_select),
+// token stands for the same values as before. Three steps: the list of kept slots by head (k_kv8_select; k_kv8_count, k_kv8_number),
 // the tokens gathered into the destination's tiles (k_kv8_gather), and, where the destination is the source, into
 // tiles of the workspace and from there back (k_kv8_put_back): a tile may then be read by many workgroups
 // before another has written it, with no order between them.
@@ -67,10 +67,16 @@ __device__ __forceinline__ uint32_t ev_rank(uint64_t lanes) {  // of them those 
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
 }
 
-constexpr int SEL = 1024, PER = 32;  // threads of a selection, weights a thread holds
+constexpr int SEL = 1024;             // threads of a selection
+constexpr int NEAR = 32, FAR = 8;     // weights a thread holds: of a head in one workgroup, in many
+
+struct EvictLds {
+    __attribute__((aligned(16))) uint32_t hist[2048][4];  // a copy for every fourth lane: weights fill few bins, and lanes of one wait for each other
+    uint32_t part[2][SEL / 64], sums[2][SEL / 64], found[3];
+};
 
 // f(0) .. f(J - 1) and on to a multiple of 4, four at a time (a jump over each of the others would fetch its code)
-template <class F>
+template <int PER, class F>
 __device__ __forceinline__ void ev_each(int J, F&& f) {
 #pragma unroll
     for (int g = 0; g < PER; g += 4) {
@@ -80,133 +86,272 @@ __device__ __forceinline__ void ev_each(int J, F&& f) {
     }
 }
 
-// One workgroup a head. Its waves hold 32768 weights and their keys in registers, a wave 64·J consecutive ones (lane l, register j:
-// 64·j + l of them), so that a rank among them is a count of bits. The key of the last token kept is found by up to three passes over the
-// keys' bits (11, 11, 10) with counts in LDS, the kept slots numbered in a last one; a head of more tokens reads its weights again in each
-// pass. What bounds it is instructions, on one CU a head: hence one word that says all of a token.
+// The weights of a piece of a head and their keys in a workgroup's registers: a wave has 64·J consecutive ones, lane l and register j
+// 64·j + l of them, so that a rank among them is a count of bits.
+template <int PER>
+struct EvictHeld {
+    float v[PER];
+    uint32_t key[PER];
+    int J, first;  // registers in use, the lane's slot in register 0
+    __device__ __forceinline__ void load(const float* w, int base, int end) {  // slots from base on, below end
+        J = (min(SEL * PER, end - base) + SEL - 1) / SEL;
+        first = base + 64 * J * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + (threadIdx.x & 63);
+        ev_each<PER>(J, [&](int j) { v[j] = w[(uint32_t)min(first + 64 * j, end - 1)]; });
+    }
+    __device__ __forceinline__ void keys(int lo, int hi, int end) {  // [lo, hi): the slots to choose from
+        const int from = first - (threadIdx.x & 63), stop = min(end, from + 64 * J);
+        ev_each<PER>(J, [&](int j) {
+            key[j] = ev_key(v[j]);
+            if (from + 64 * j < lo || from + 64 * j + 64 > min(hi, stop)) {  // (uniform)
+                const int t = first + 64 * j;
+                key[j] = t >= stop ? 0u : t < lo || t >= hi ? EV_STAYS : key[j];
+            }
+        });
+    }
+};
+
+// What is known of the last key that stays: its first `done` bits, and how many to take of the keys that have them. `bits` more in the next pass; 0:
+// keys above `last` stay, and `need` of those equal to it.
+struct EvictState {
+    uint32_t prefix, need, last;
+    int done, bits;
+};
+__device__ __forceinline__ EvictState ev_start(int64_t keep) { return {0, (uint32_t)keep, 0, 0, 11}; }
+
+__device__ __forceinline__ void ev_clear(EvictLds& L) {
+    for (int i = threadIdx.x; i < 2048; i += SEL) *(uint4*)L.hist[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+}
+// Counts keys that begin as is known by their next bits. (No slot's key counts too where a workgroup has all of a head: it is the lowest, and fewer
+// stay than there are slots.)
+template <int PER>
+__device__ __forceinline__ void ev_count(const EvictState& S, const EvictHeld<PER>& H, EvictLds& L) {
+    const int shift = 32 - S.done - S.bits;
+    const uint32_t low = S.done > 0 ? S.prefix << S.bits : 0;
+    uint32_t* mine = &L.hist[0][threadIdx.x & 3];
+    ev_each<PER>(H.J, [&](int j) {
+        const uint32_t bin = (H.key[j] >> shift) - low;
+        if (bin < 1u << S.bits && (PER == NEAR || H.key[j] != 0)) atomicAdd(mine + 4 * bin, 1u);
+    });
+}
+// the counts c1 of bin b + 1 and c0 of b = 2046 - 2·thread, of which one holds the need-th from the top: the pass done
+__device__ __forceinline__ EvictState ev_find(EvictState S, uint32_t c1, uint32_t c0, EvictLds& L) {
+    const int tid = threadIdx.x, wv = tid >> 6, b = 2046 - 2 * tid;
+    const uint32_t x = ev_scan(c0 + c1);
+    if ((tid & 63) == 63) L.part[0][wv] = x;
+    __syncthreads();
+    uint32_t above = x - c0 - c1;
+#pragma unroll
+    for (int i = 0; i < SEL / 64; i++) above += i < wv ? L.part[0][i] : 0;
+    if (above < S.need && S.need <= above + c1) {
+        L.found[0] = b + 1;
+        L.found[1] = above;
+        L.found[2] = c1;
+    } else if (above + c1 < S.need && S.need <= above + c1 + c0) {
+        L.found[0] = b;
+        L.found[1] = above + c1;
+        L.found[2] = c0;
+    }
+    __syncthreads();
+    S.prefix = S.prefix << S.bits | L.found[0];
+    S.need -= L.found[1];
+    S.done += S.bits;
+    S.last = S.prefix;
+    S.bits = S.done == 22 ? 10 : S.done == 32 ? 0 : 11;
+    if (L.found[2] == S.need) {  // (uniform) the whole bin; its lowest key is above 0: fewer stay than there are
+        S.last = (S.prefix << (32 - S.done)) - 1;  // (done 32: a shift by 0)
+        S.need = 0;
+        S.bits = 0;
+    }
+    return S;
+}
+
+// Lists those of a piece that stay, behind `sures` above the last key and `equals` equal to it, and adds its own to them
+template <int PER>
+__device__ __forceinline__ void ev_number(const EvictState& S, const EvictHeld<PER>& H, EvictLds& L, int round, uint32_t& sures, uint32_t& equals, int* list,
+                                          float* kw) {
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t ns = 0, ne = 0;  // (uniform) the wave's
+    ev_each<PER>(H.J, [&](int j) {
+        ns += (uint32_t)__popcll(__ballot(H.key[j] > S.last));
+        ne += (uint32_t)__popcll(__ballot(H.key[j] == S.last));
+    });
+    if ((threadIdx.x & 63) == 0) {
+        L.part[round][wv] = ns;
+        L.sums[round][wv] = ne;
+    }
+    __syncthreads();  // (the other round's readers have passed the barrier before this one)
+    uint32_t s0 = sures, e0 = equals;
+#pragma unroll
+    for (int i = 0; i < SEL / 64; i++) {
+        const uint32_t a = L.part[round][i], b = L.sums[round][i];
+        s0 += i < wv ? a : 0;
+        e0 += i < wv ? b : 0;
+        sures += a;
+        equals += b;
+    }
+    ev_each<PER>(H.J, [&](int j) {
+        const bool sure = H.key[j] > S.last, equal = H.key[j] == S.last;
+        const uint64_t ms = __ballot(sure), me = __ballot(equal);
+        const uint32_t e = e0 + ev_rank(me), at = s0 + ev_rank(ms) + min(e, S.need);
+        if (sure || (equal && e < S.need)) {
+            list[at] = H.first + 64 * j;
+            kw[at] = H.v[j];
+        }
+        s0 += (uint32_t)__popcll(ms);
+        e0 += (uint32_t)__popcll(me);
+    });
+}
+
+// One workgroup a head of up to 32768 tokens. The last key that stays is found by up to three passes over the keys' bits (11, 11, 10) with
+// counts in LDS (two, but for weights that are equal or nearly), the slots that stay numbered in a last one. What bounds it is instructions, on one
+// CU a head: hence one word that says all of a token. 8 heads of 2500 tokens 8.5 µs, of 30000 18.
 __global__ void __launch_bounds__(SEL) k_kv8_select(EvictArgs A) {
-    __shared__ __attribute__((aligned(16))) uint32_t hist[2048][4];  // a copy for every fourth lane: weights fill few bins, and lanes of one wait for each other
-    __shared__ uint32_t part[2][SEL / 64], sums[2][SEL / 64];
-    __shared__ uint32_t found[3];
-    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = blockIdx.x, seq = blockIdx.y;
-    const int len = (int)ev_len(A, seq);
-    const int64_t unit = (int64_t)seq * A.nkv + h;
+    __shared__ EvictLds lds;
+    const int seq = blockIdx.y, len = (int)ev_len(A, seq);
+    const int64_t unit = (int64_t)seq * A.nkv + blockIdx.x;
     const float* w = A.weights + unit * A.max_seq;
     int* list = A.list + unit * A.list_stride;
     float* kw = A.kept_weights + unit * A.most;
-    if (tid == 0) A.rows[unit] = (int)min((int64_t)len, A.keep);
+    if (threadIdx.x == 0) A.rows[unit] = (int)min((int64_t)len, A.keep);
     if (len <= A.keep) {  // (uniform) all stay
-        for (int t = tid; t < len; t += SEL) {
+        for (int t = threadIdx.x; t < len; t += SEL) {
             list[t] = t;
             kw[t] = w[t];
         }
         return;
     }
     if (A.keep == 0) return;  // (uniform)
-    const int lo = (int)A.first, hi = len - (int)A.recent;  // the slots to choose from
-    float v[PER];
-    uint32_t key[PER];
-    int J = 0, first = 0;  // registers in use, the lane's slot in register 0
-    auto load = [&](int base) {
-        J = (min(SEL * PER, len - base) + SEL - 1) / SEL;
-        first = base + 64 * J * wv + lane;
-        ev_each(J, [&](int j) { v[j] = w[(uint32_t)min(first + 64 * j, len - 1)]; });
-    };
-    auto keys = [&]() {
-        const int from = first - lane, end = min(len, from + 64 * J);
-        ev_each(J, [&](int j) {
-            key[j] = ev_key(v[j]);
-            if (from + 64 * j < lo || from + 64 * j + 64 > min(hi, end)) {  // (uniform)
-                const int t = first + 64 * j;
-                key[j] = t >= end ? 0u : t < lo || t >= hi ? EV_STAYS : key[j];
-            }
-        });
-    };
-    const bool whole = len <= SEL * PER;
-    uint32_t need = (uint32_t)A.keep, last = 0, prefix = 0;  // keys above `last` are taken, and `need` equal to it
-    uint32_t equals = 0, sures = 0;                           // of them passed so far
-    int done = 0, bits = 11, round = 0;                      // bits of the last one's key that are known, and that a pass adds
-    for (int pass = 0;; pass++) {
-        for (int base = 0; base < len; base += SEL * PER) {
-            if (pass == 0 || !whole) load(base);
-            if (bits > 0 && base == 0) {  // beside the loads
-                for (int i = tid; i < 2048; i += SEL) *(uint4*)hist[i] = make_uint4(0, 0, 0, 0);
-                __syncthreads();
-            }
-            if (pass == 0 || !whole) keys();
-            if (bits > 0) {  // (uniform) count
-                const int shift = 32 - done - bits;
-                const uint32_t low = bits < 32 - shift ? prefix << bits : 0;  // (nothing known: 0)
-                uint32_t* mine = &hist[0][lane & 3];
-                ev_each(J, [&](int j) {
-                    const uint32_t bin = (key[j] >> shift) - low;
-                    if (bin < 1u << bits) atomicAdd(mine + 4 * bin, 1u);
-                });
-                continue;
-            }
-            uint32_t ns = 0, ne = 0;  // (uniform) the wave's
-            ev_each(J, [&](int j) {
-                ns += (uint32_t)__popcll(__ballot(key[j] > last));
-                ne += (uint32_t)__popcll(__ballot(key[j] == last));
-            });
-            if (lane == 0) {
-                part[round][wv] = ns;
-                sums[round][wv] = ne;
-            }
-            __syncthreads();  // (the other buffers' readers have passed the barrier before this one)
-            uint32_t s0 = sures, e0 = equals;
+    EvictHeld<NEAR> H;
+    EvictState S = ev_start(A.keep);
+    H.load(w, 0, len);
+    ev_clear(lds);
+    H.keys((int)A.first, len - (int)A.recent, len);
+    while (S.bits > 0) {
+        if (S.done > 0) ev_clear(lds);
+        ev_count(S, H, lds);
+        __syncthreads();
+        const int b = 2046 - 2 * threadIdx.x;
+        const uint4 h1 = *(const uint4*)lds.hist[b + 1], h0 = *(const uint4*)lds.hist[b];
+        S = ev_find(S, h1.x + h1.y + h1.z + h1.w, h0.x + h0.y + h0.z + h0.w, lds);
+    }
+    uint32_t sures = 0, equals = 0;
+    ev_number(S, H, lds, 0, sures, equals, list, kw);
+}
+
+// More tokens: many workgroups a head, a chunk of its slots each, and a launch for each pass. The workgroups of a pass leave their counts in memory,
+// those of the next one add all of them up and go on from there, each for itself; the last launch knows from the counts how many stay before its chunk.
+// 8 heads of 131000 tokens: one workgroup a head, which reads its weights again in each pass, 107 µs.
+struct EvictFar {
+    uint32_t* hist;   // [3 passes][units][chunks][2048]
+    uint32_t* state;  // [2][units][4]: behind the first pass, the second
+    int64_t units;
+    int chunk, chunks;  // slots of a chunk, a multiple of 8192; chunks of max_len slots
+};
+__device__ __forceinline__ const uint32_t* ev_counts(const EvictFar& F, int pass, int64_t unit, int c) {
+    return F.hist + ((pass * F.units + unit) * F.chunks + c) * 2048;
+}
+__device__ __forceinline__ EvictState ev_resolve(const EvictState& S, const EvictFar& F, int pass, int64_t unit, int live, EvictLds& L) {
+    uint32_t c1 = 0, c0 = 0;
+#pragma unroll 4
+    for (int c = 0; c < live; c++) {
+        const uint2 n = *(const uint2*)(ev_counts(F, pass, unit, c) + 2046 - 2 * threadIdx.x);
+        c0 += n.x;
+        c1 += n.y;
+    }
+    return ev_find(S, c1, c0, L);
+}
+__device__ __forceinline__ void ev_keep_state(const EvictFar& F, int pass, int64_t unit, const EvictState& S) {
+    if (blockIdx.x != 0 || threadIdx.x != 0) return;
+    *(uint4*)(F.state + (pass * F.units + unit) * 4) = make_uint4(S.prefix, S.need, S.last, (uint32_t)(S.done << 8 | S.bits));
+}
+__device__ __forceinline__ EvictState ev_state(const EvictFar& F, int pass, int64_t unit) {
+    const uint4 s = *(const uint4*)(F.state + (pass * F.units + unit) * 4);
+    return {s.x, s.y, s.z, (int)(s.w >> 8), (int)(s.w & 255)};
+}
+
+template <int PASS>
+__global__ void __launch_bounds__(SEL) k_kv8_count(EvictArgs A, EvictFar F) {
+    __shared__ EvictLds lds;
+    const int seq = blockIdx.z, len = (int)ev_len(A, seq), s0 = (int)blockIdx.x * F.chunk, s1 = min(s0 + F.chunk, len), live = (len + F.chunk - 1) / F.chunk;
+    if (s0 >= len || len <= A.keep || A.keep == 0) return;  // (uniform)
+    const int64_t unit = (int64_t)seq * A.nkv + blockIdx.y;
+    EvictState S = ev_start(A.keep);
+    if constexpr (PASS == 1) S = ev_resolve(S, F, 0, unit, live, lds);
+    if constexpr (PASS == 2) {
+        S = ev_state(F, 0, unit);
+        if (S.bits > 0) S = ev_resolve(S, F, 1, unit, live, lds);  // (uniform)
+    }
+    if constexpr (PASS > 0) ev_keep_state(F, PASS - 1, unit, S);
+    if (S.bits == 0) return;  // (uniform)
+    EvictHeld<FAR> H;
+    ev_clear(lds);
+    for (int base = s0; base < s1; base += SEL * FAR) {
+        H.load(A.weights + unit * A.max_seq, base, s1);
+        H.keys((int)A.first, len - (int)A.recent, s1);
+        ev_count(S, H, lds);
+    }
+    __syncthreads();
+    uint32_t* out = F.hist + ((PASS * F.units + unit) * F.chunks + blockIdx.x) * 2048;
+    for (int i = threadIdx.x; i < 2048; i += SEL) {
+        const uint4 n = *(const uint4*)lds.hist[i];
+        out[i] = n.x + n.y + n.z + n.w;
+    }
+}
+
+__global__ void __launch_bounds__(SEL) k_kv8_number(EvictArgs A, EvictFar F) {
+    __shared__ EvictLds lds;
+    const int seq = blockIdx.z, len = (int)ev_len(A, seq), s0 = (int)blockIdx.x * F.chunk, s1 = min(s0 + F.chunk, len), live = (len + F.chunk - 1) / F.chunk;
+    const int tid = threadIdx.x;
+    const int64_t unit = (int64_t)seq * A.nkv + blockIdx.y;
+    const float* w = A.weights + unit * A.max_seq;
+    int* list = A.list + unit * A.list_stride;
+    float* kw = A.kept_weights + unit * A.most;
+    if (blockIdx.x == 0 && tid == 0) A.rows[unit] = (int)min((int64_t)len, A.keep);
+    if (len <= A.keep) {  // (uniform) all stay
+        for (int t = s0 + tid; t < s1; t += SEL) {
+            list[t] = t;
+            kw[t] = w[t];
+        }
+        return;
+    }
+    if (s0 >= len || A.keep == 0) return;  // (uniform)
+    EvictState S = ev_state(F, 1, unit);
+    if (S.bits > 0) S = ev_resolve(S, F, 2, unit, live, lds);  // (uniform)
+    // before the chunk: keys of a higher bin in some pass, and of the last pass' own bin where all of it stays, or the equal ones
+    uint32_t sures = 0, equals = 0;
+    for (int pass = 0; pass < 3; pass++) {
+        const int known = pass < 2 ? 11 * (pass + 1) : 32;
+        if (known > S.done) break;  // (uniform)
+        const uint32_t bin = S.prefix >> (S.done - known) & (pass < 2 ? 2047u : 1023u);
+        const bool ends = known == S.done;
+        for (int c = 0; c < (int)blockIdx.x; c++) {
+            const uint2 n = *(const uint2*)(ev_counts(F, pass, unit, c) + 2 * tid);
+            const uint32_t b = 2 * tid;
+            sures += (b > bin || (ends && S.need == 0 && b == bin) ? n.x : 0) + (b + 1 > bin || (ends && S.need == 0 && b + 1 == bin) ? n.y : 0);
+            if (ends && S.need > 0) equals += b == bin ? n.x : b + 1 == bin ? n.y : 0;
+        }
+    }
+    sures = ev_scan(sures);
+    equals = ev_scan(equals);
+    __syncthreads();  // (ev_resolve's readers)
+    if ((tid & 63) == 63) {
+        lds.part[1][tid >> 6] = sures;
+        lds.sums[1][tid >> 6] = equals;
+    }
+    __syncthreads();
+    sures = equals = 0;
 #pragma unroll
-            for (int i = 0; i < SEL / 64; i++) {
-                const uint32_t a = part[round][i], b = sums[round][i];
-                s0 += i < wv ? a : 0;
-                e0 += i < wv ? b : 0;
-                sures += a;
-                equals += b;
-            }
-            round ^= 1;
-            ev_each(J, [&](int j) {
-                const bool sure = key[j] > last, equal = key[j] == last;
-                const uint64_t ms = __ballot(sure), me = __ballot(equal);
-                const uint32_t e = e0 + ev_rank(me), at = s0 + ev_rank(ms) + min(e, need);
-                if (sure || (equal && e < need)) {
-                    list[at] = first + 64 * j;
-                    kw[at] = v[j];
-                }
-                s0 += (uint32_t)__popcll(ms);
-                e0 += (uint32_t)__popcll(me);
-            });
-        }
-        if (bits == 0) return;
-        __syncthreads();
-        // the bin in which the need-th from the top lies: counts above each pair of bins
-        const int b = 2046 - 2 * tid;  // thread 0: the highest two
-        const uint4 h1 = *(const uint4*)hist[b + 1], h0 = *(const uint4*)hist[b];
-        const uint32_t c1 = h1.x + h1.y + h1.z + h1.w, c0 = h0.x + h0.y + h0.z + h0.w, x = ev_scan(c0 + c1);
-        if (lane == 63) part[0][wv] = x;
-        __syncthreads();
-        uint32_t above = x - c0 - c1;
-#pragma unroll
-        for (int i = 0; i < SEL / 64; i++) above += i < wv ? part[0][i] : 0;
-        if (above < need && need <= above + c1) {
-            found[0] = b + 1;
-            found[1] = above;
-            found[2] = c1;
-        } else if (above + c1 < need && need <= above + c1 + c0) {
-            found[0] = b;
-            found[1] = above + c1;
-            found[2] = c0;
-        }
-        __syncthreads();
-        prefix = prefix << bits | found[0];
-        need -= found[1];
-        done += bits;
-        last = prefix;
-        bits = done == 22 ? 10 : done == 32 ? 0 : 11;
-        if (found[2] == need) {  // (uniform) the whole bin; its lowest key is above 0: fewer stay than there are
-            last = (prefix << (32 - done)) - 1;  // (done 32: a shift by 0)
-            need = 0;
-            bits = 0;
-        }
+    for (int i = 0; i < SEL / 64; i++) {
+        sures += lds.part[1][i];
+        equals += lds.sums[1][i];
+    }
+    EvictHeld<FAR> H;
+    int round = 0;  // (the first writes part[0])
+    for (int base = s0; base < s1; base += SEL * FAR, round ^= 1) {
+        H.load(w, base, s1);
+        H.keys((int)A.first, len - (int)A.recent, s1);
+        ev_number(S, H, lds, round, sures, equals, list, kw);
     }
 }
 
@@ -308,26 +453,41 @@ __global__ void __launch_bounds__(256) k_kv8_put_back(EvictArgs A, const uint8_t
     ev_tile<HD>(dst, src, from, n);
 }
 
+// A head of many tokens is counted in at most 64 chunks
+constexpr int64_t FAR_CHUNK = SEL * FAR, FAR_CHUNKS = 64;
+bool ev_far(int64_t max_len) { return max_len > SEL * NEAR; }
+
 // the workspace's parts, each 16-byte aligned: bytes from its start
 struct EvictWs {
-    int64_t list, weights, stage, end;
+    int64_t list, weights, state, hist, stage, end;
 };
-bool ev_ws(int64_t seqs, int64_t nkv, int64_t hd, int64_t most, bool in_place, EvictWs& W) {
-    const int64_t units = seqs * nkv;  // below 2^32
+bool ev_ws(int64_t seqs, int64_t nkv, int64_t hd, int64_t max_len, int64_t keep, bool in_place, EvictWs& W) {
+    const int64_t units = seqs * nkv, most = std::min(keep, max_len);  // units below 2^32
+    const int64_t chunks = ev_far(max_len) ? std::min(FAR_CHUNKS, aeth_cdiv(max_len, FAR_CHUNK)) : 0;
     int64_t all, tiles;
     if (!aeth_mul_ok(units, most, &all) || !aeth_mul_ok(units * aeth_cdiv(most, KV8_TILE), aeth_kv8_tile_bytes((int)hd), &tiles) ||
         all > (int64_t)1 << 58 || tiles > (int64_t)1 << 60)
         return false;
     W.list = aeth_cdiv(4 * units, 16) * 16;
     W.weights = W.list + aeth_cdiv(4 * all, 16) * 16;
-    W.stage = W.weights + aeth_cdiv(4 * all, 16) * 16;
+    W.state = W.weights + aeth_cdiv(4 * all, 16) * 16;
+    W.hist = W.state + (chunks > 0 ? 32 * units : 0);
+    W.stage = W.hist + 3 * units * chunks * 2048 * 4;
     W.end = W.stage + (in_place ? tiles : 0);
     return true;
 }
 
 template <int HD>
-int ev_launch(EvictArgs A, int64_t seqs, uint8_t* stage, hipStream_t s) {
-    hipLaunchKernelGGL(k_kv8_select, dim3((unsigned)A.nkv, (unsigned)seqs), dim3(SEL), 0, s, A);
+int ev_launch(EvictArgs A, EvictFar F, int64_t seqs, uint8_t* stage, hipStream_t s) {
+    if (ev_far(A.max_len)) {
+        const dim3 grid((unsigned)F.chunks, (unsigned)A.nkv, (unsigned)seqs), block(SEL);
+        hipLaunchKernelGGL(k_kv8_count<0>, grid, block, 0, s, A, F);
+        hipLaunchKernelGGL(k_kv8_count<1>, grid, block, 0, s, A, F);
+        hipLaunchKernelGGL(k_kv8_count<2>, grid, block, 0, s, A, F);
+        hipLaunchKernelGGL(k_kv8_number, grid, block, 0, s, A, F);
+    } else {
+        hipLaunchKernelGGL(k_kv8_select, dim3((unsigned)A.nkv, (unsigned)seqs), dim3(SEL), 0, s, A);
+    }
     AETH_LAUNCH_CHECK();
     const int64_t weight_blocks = A.dst_weights ? aeth_cdiv(A.dst_seq, 2048) : 0;
     const int64_t head = (int64_t)A.gather_blocks * aeth_kv8_tile_bytes(HD);
@@ -360,10 +520,10 @@ int evict(const char* what, const void* cache, int64_t stride, const float* weig
         std::min(keep, max_len) > dst_seq)
         return aeth_set_error(AETH_EINVAL, "%s: %lld of %lld tokens kept (the first %lld and last %lld) in slices of %lld and %lld", what, (long long)keep,
                               (long long)max_len, (long long)first, (long long)recent, (long long)max_seq, (long long)dst_seq);
-    int64_t all, dst_all, w_all, dw_all;
+    int64_t all, dst_all, w_all, dw_all, k_all = 0;
     if (seqs < 0 || seqs > 65535 || stride < 0 || dst_stride < 0 || ((stride | dst_stride) & 15) || (seqs > 1 && (stride < bytes || dst_stride < dst_bytes)) ||
         !aeth_mul_ok(seqs, std::max(stride, bytes), &all) || !aeth_mul_ok(seqs, std::max(dst_stride, dst_bytes), &dst_all) ||
-        !aeth_mul_ok(seqs * nkv, max_seq, &w_all) || !aeth_mul_ok(seqs * nkv, dst_seq, &dw_all) || w_all > INT64_MAX / 4 || dw_all > INT64_MAX / 4)
+        (kept && !aeth_mul_ok(seqs * nkv, keep, &k_all)) || k_all > INT64_MAX / 4 || !aeth_mul_ok(seqs * nkv, max_seq, &w_all) || !aeth_mul_ok(seqs * nkv, dst_seq, &dw_all) || w_all > INT64_MAX / 4 || dw_all > INT64_MAX / 4)
         return aeth_set_error(AETH_EINVAL, "%s: %lld sequences %lld and %lld bytes apart", what, (long long)seqs, (long long)stride, (long long)dst_stride);
     const bool in_place = dst == cache;
     if (in_place ? dst_seq != max_seq || (seqs > 1 && dst_stride != stride) : !apart(cache, all, dst, dst_all))
@@ -375,7 +535,7 @@ int evict(const char* what, const void* cache, int64_t stride, const float* weig
     if (aeth_cdiv(most, KV8_TILE) + aeth_cdiv(dst_seq, 2048) > (int64_t)1 << 23)
         return aeth_set_error(AETH_EUNSUPPORTED, "%s: %lld tokens kept in one call", what, (long long)keep);
     EvictWs W;
-    if (!ev_ws(seqs, nkv, hd, most, in_place, W)) return aeth_set_error(AETH_EINVAL, "%s: bad shape", what);
+    if (!ev_ws(seqs, nkv, hd, max_len, keep, in_place, W)) return aeth_set_error(AETH_EINVAL, "%s: bad shape", what);
     if (seqs == 0) return AETH_OK;
     if (!ws || ws_bytes < W.end)
         return aeth_set_error(AETH_EINVAL, "%s: a workspace of %lld bytes (%lld given)", what, (long long)W.end, (long long)(ws ? ws_bytes : 0));
@@ -405,9 +565,15 @@ int evict(const char* what, const void* cache, int64_t stride, const float* weig
     A.gather_blocks = (int)std::max<int64_t>(1, aeth_cdiv(most, KV8_TILE));
     A.in_place = in_place;
     uint8_t* stage = in_place ? (uint8_t*)ws + W.stage : nullptr;
-    if (hd == 64) return ev_launch<64>(A, seqs, stage, s);
-    if (hd == 128) return ev_launch<128>(A, seqs, stage, s);
-    return ev_launch<256>(A, seqs, stage, s);
+    EvictFar F = {};
+    F.hist = (uint32_t*)((char*)ws + W.hist);
+    F.state = (uint32_t*)((char*)ws + W.state);
+    F.units = seqs * nkv;
+    F.chunk = (int)(aeth_cdiv(max_len, FAR_CHUNKS * FAR_CHUNK) * FAR_CHUNK);
+    F.chunks = (int)(max_len > 0 ? aeth_cdiv(max_len, F.chunk) : 0);
+    if (hd == 64) return ev_launch<64>(A, F, seqs, stage, s);
+    if (hd == 128) return ev_launch<128>(A, F, seqs, stage, s);
+    return ev_launch<256>(A, F, seqs, stage, s);
 }
 
 }  // namespace
@@ -415,7 +581,7 @@ int evict(const char* what, const void* cache, int64_t stride, const float* weig
 extern "C" AETH_API int64_t aeth_kv8_evict_ws_bytes(int64_t n_seqs, int64_t kv_heads, int64_t head_dim, int64_t max_len, int64_t keep, int in_place) {
     EvictWs W;
     if (n_seqs < 0 || n_seqs > 65535 || max_len < 0 || max_len > KV8_MAX_SEQ || keep < 0 || aeth_kv8_layer_bytes(kv_heads, head_dim, 1) < 0 ||
-        !ev_ws(n_seqs, kv_heads, head_dim, std::min(keep, max_len), in_place != 0, W)) {
+        !ev_ws(n_seqs, kv_heads, head_dim, max_len, keep, in_place != 0, W)) {
         aeth_set_error(AETH_EINVAL, "aeth_kv8_evict_ws_bytes: bad shape");
         return -1;
     }

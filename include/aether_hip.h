@@ -371,8 +371,8 @@ AETH_API int aeth_attn_kv8_shared(const float* d_q, int64_t q_stride, const void
                                   int64_t n_seqs, int64_t n_heads, int64_t kv_heads, int64_t head_dim, int64_t max_seq,
                                   int64_t max_len, int64_t window, float* d_out, void* d_ws, int64_t ws_bytes, void* stream);
 /* Bytes of workspace for the two calls below, in the terms of aeth_attn_kv8_ws_bytes. For
- * up to 64 queries times query heads of a KV head it holds their scores: 4 bytes for
- * each of them, position and KV head. */
+ * up to 48 queries times query heads of a KV head (and in a batch) it holds their scores: 4
+ * bytes for each of them, position and KV head. */
 AETH_API int64_t aeth_attn_kv8_weights_ws_bytes(int64_t n_seqs, int64_t n, int64_t n_heads, int64_t kv_heads,
                                                 int64_t head_dim, int64_t max_len);
 /* aeth_attn_kv8, and the attention weight that each token receives added up: for slots

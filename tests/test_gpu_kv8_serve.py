@@ -421,6 +421,25 @@ def test_evict_batch(gpu, hd, in_place):
         check_evicted(torch, src[0], was[0], before[0], dst[0], dst_weights[0], kept[0], nkv, hd, max_seq, 700, keep, first, recent, dst_seq)
 
 
+@pytest.mark.parametrize("keep,first,recent", [(3000, 4, 100), (0, 0, 0), (500, 200, 300), (40000, 0, 0), (1, 0, 0)])
+def test_evict_batch_of_many_tokens(gpu, keep, first, recent):
+    """Lengths at the borders of what one workgroup holds and of the chunks of many, next to short ones; new lengths in the old ones' place."""
+    torch = gpu
+    nkv, hd, max_seq = 1, 64, 70000
+    lens = [70000, 0, 32768, 32769, 100, 40960, 40961, keep, keep + 1]
+    b = len(lens)
+    layers = some_layer(torch, 1, b * nkv, hd, max_seq).reshape((b,) + R.layer_shape(nkv, hd, max_seq))
+    weights = uneven(torch, keep, b, nkv, max_seq)
+    weights[5] = 0.25  # all equal
+    weights[0, 0, 5000:] = 1.0 + 2.0 ** -20 * torch.rand(65000, generator=torch.Generator().manual_seed(2)).cuda()  # alike in their first bits
+    src, was, d_lens = layers.clone(), weights.clone(), ints(torch, lens)
+    kept = torch.full((b, nkv, max(keep, 1)), -7, dtype=torch.int32, device="cuda")
+    evict_batch(torch, layers, weights, d_lens, nkv, hd, max_seq, max_seq, keep, first, recent, layers, max_seq, weights, d_lens, kept)
+    assert d_lens.tolist() == [min(l, keep) for l in lens]
+    for i, seq in enumerate(lens):
+        check_evicted(torch, src[i], was[i], src[i], layers[i], weights[i], kept[i] if keep else None, nkv, hd, max_seq, seq, keep, first, recent, max_seq)
+
+
 def test_evict_captured(gpu):
     torch = gpu
     nkv, hd, max_seq, keep, b = 2, 128, 500, 100, 4

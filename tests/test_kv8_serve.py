@@ -24,6 +24,11 @@ def test_shared_refuses(change, rc):
     assert "aeth_attn_kv8_shared" in A.last_error()
 
 
+def test_shared_refuses_more_than_a_grid():
+    change = dict(seqs=60000, nq=128, nkv=128, qs=2 ** 14, hd=64, ms=64, ml=64, stride=128 * 64 * 136)
+    assert call("aeth_attn_kv8_shared", SHARED, change) == -4
+
+
 def test_shared_nothing_to_do():
     assert call("aeth_attn_kv8_shared", SHARED, dict(seqs=0)) == 0
     assert call("aeth_attn_kv8_shared", SHARED, dict(seqs=0, prefix=None, pl=0, ps=0)) == 0
@@ -49,6 +54,11 @@ def test_batch_weights_refuse(change, rc):
     assert "aeth_attn_kv8_weights_batch" in A.last_error()
 
 
+def test_weights_refuse_more_than_a_grid():
+    change = dict(nq=64, nkv=64, qs=2 ** 14, hd=64, n=1, seq=2 ** 26, ms=2 ** 26, wsb=2 ** 62)
+    assert call("aeth_attn_kv8_weights", WEIGHTS, change) == -4
+
+
 def test_weights_nothing_to_do():
     assert call("aeth_attn_kv8_weights", WEIGHTS, dict(n=0, seq=0)) == 0
     assert call("aeth_attn_kv8_weights", WEIGHTS, dict(n=0, seq=0, q=None, out=None)) == 0
@@ -68,15 +78,16 @@ def test_workspaces():
                 smaller = list(args)
                 smaller[i] = less
                 assert 0 <= ws(*smaller) <= most, smaller
-    # scores of at most 64 columns cost more than the sums of many
+    # scores of few columns cost more than the sums of many
     for length in (100, 5000, 100000):
-        for n in (1, 15, 16, 17, 64, 500):
+        for n in (1, 11, 12, 13, 15, 16, 17, 64, 500):
             assert L.aeth_attn_kv8_weights_ws_bytes(1, n, 32, 8, 128, length) <= L.aeth_attn_kv8_weights_ws_bytes(1, n + 1, 32, 8, 128, length)
     for bad in ((-1, 32, 8, 128, 10, 10), (3, 30, 8, 128, 10, 10), (3, 32, 8, 96, 10, 10), (3, 32, 8, 128, -1, 10), (3, 32, 8, 128, 10, -1),
                 (3, 32, 8, 128, 2 ** 31, 10)):
         assert L.aeth_attn_kv8_shared_ws_bytes(*bad) == -1, bad
     for bad in ((-1, 1, 32, 8, 128, 64), (1, -1, 32, 8, 128, 64), (1, 1, 30, 8, 128, 64), (1, 1, 32, 8, 96, 64), (1, 1, 32, 8, 128, -1)):
         assert L.aeth_attn_kv8_weights_ws_bytes(*bad) == -1, bad
+    assert L.aeth_attn_kv8_weights_ws_bytes(65535, 2 ** 24, 4096, 4096, 64, 2 ** 30) == -1  # past 64 bits
     for bad in ((-1, 8, 128, 10, 5, 0), (70000, 8, 128, 10, 5, 0), (1, 0, 128, 10, 5, 0), (1, 8, 100, 10, 5, 0), (1, 8, 128, -1, 5, 0), (1, 8, 128, 10, -1, 0),
                 (1, 8, 128, 2 ** 31, 5, 0)):
         assert L.aeth_kv8_evict_ws_bytes(*bad) == -1, bad
@@ -103,7 +114,7 @@ def test_evict_refuses(change, rc):
 
 
 @pytest.mark.parametrize("change,rc", CUTS + [
-    (dict(layers=None), -1), (dict(lens=None), -1), (dict(lens=P + 1), -1), (dict(dl=P + 2), -1), (dict(seqs=-1), -1), (dict(seqs=70000), -1), (dict(ml=-1), -1),
+    (dict(keep=2 ** 62), -1), (dict(layers=None), -1), (dict(lens=None), -1), (dict(lens=P + 1), -1), (dict(dl=P + 2), -1), (dict(seqs=-1), -1), (dict(seqs=70000), -1), (dict(ml=-1), -1),
     (dict(ml=4097), -1), (dict(stride=64 * BYTES - 16), -1), (dict(stride=64 * BYTES + 8), -1), (dict(stride=2 ** 62), -1), (dict(dstride=16 * BYTES - 16), -1),
     (dict(dstride=-16), -1), (dict(dst=P + 64 * BYTES), -1), (dict(dst=P, ds=4096, dstride=65 * BYTES), -1),
     (dict(seqs=60000, nkv=60000, stride=60000 * 64 * 64 * 264, dstride=60000 * 16 * 64 * 264, dst=1 << 62), -1)])
