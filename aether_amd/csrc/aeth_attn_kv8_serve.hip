@@ -204,23 +204,31 @@ __device__ __forceinline__ float2 sv_column(const A8& A, int len, int seq, int h
     return make_float2(M, 1.0f / S);
 }
 
-// From the scores: workgroup (256 keys, KV head), the columns 32 at a time, their statistics first
-template <int HD>
+// From the scores: workgroup (256·KT keys, KV head), the columns 32 at a time, their statistics first
+template <int HD, int KT>
 __device__ __forceinline__ void sv_weigh_scores(const A8& A, const Weigh& W, int bx, int seq, float2 (&col)[32]) {
-    const int tid = threadIdx.x, h = bx % A.nkv, t0 = bx / A.nkv * 256, t = t0 + tid;
+    const int tid = threadIdx.x, h = bx % A.nkv, t0 = bx / A.nkv * (256 * KT);
     const int len = a8_len(A, seq);
     if (t0 >= len) return;  // (uniform)
-    const int64_t unit = (int64_t)seq * A.nkv + h, row = 64 * (int64_t)A.score_tiles, at = unit * W.max_seq + t;
-    const float* src = A.scores + unit * A.cols * row + min(t, (int)row - 1);
-    const bool real = t < len;
-    float s[4];  // four columns' scores, asked for before what their sums wait for
+    const int64_t unit = (int64_t)seq * A.nkv + h, row = 64 * (int64_t)A.score_tiles;
+    const float* src = A.scores + unit * A.cols * row;
+    int t[KT];
+#pragma unroll
+    for (int k = 0; k < KT; k++) t[k] = t0 + tid + 256 * k;
+    float s[4][KT];  // four columns' scores, asked for before what their sums wait for
     auto fetch = [&](int x) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) s[j] = src[min(x + j, A.cols - 1) * row];
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int k = 0; k < KT; k++) s[j][k] = src[min(x + j, A.cols - 1) * row + min(t[k], (int)row - 1)];
     };
     fetch(0);
-    const float prior = real && W.prior ? W.prior[at] : 0.0f;
-    float sum = 0.0f;
+    float prior[KT], sum[KT];
+#pragma unroll
+    for (int k = 0; k < KT; k++) {
+        prior[k] = t[k] < len && W.prior ? W.prior[unit * W.max_seq + t[k]] : 0.0f;
+        sum[k] = 0.0f;
+    }
     for (int c0 = 0; c0 < A.cols; c0 += 32) {
         const int count = min(32, A.cols - c0);
         if (c0 > 0) __syncthreads();
@@ -233,29 +241,33 @@ __device__ __forceinline__ void sv_weigh_scores(const A8& A, const Weigh& W, int
         for (int c1 = 0; c1 < count; c1 += 4) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int x = c0 + c1 + j, hi = hi0 + x / A.G, lo = A.window > 0 ? hi - A.window : 0;  // (uniform)
+                const int x = c0 + c1 + j, hi = A.n > 1 ? hi0 + x / A.G : hi0, lo = A.window > 0 ? hi - A.window : 0;  // (uniform)
                 const float2 ml = col[min(c1 + j, 31)];
-                if (x < A.cols && t >= lo && t < hi) sum = fmaf(__builtin_amdgcn_exp2f(s[j] - ml.x), ml.y, sum);
+#pragma unroll
+                for (int k = 0; k < KT; k++)
+                    if (x < A.cols && t[k] >= lo && t[k] < hi) sum[k] = fmaf(__builtin_amdgcn_exp2f(s[j][k] - ml.x), ml.y, sum[k]);
             }
             if (c0 + c1 + 4 < A.cols) fetch(c0 + c1 + 4);
         }
     }
-    if (real) W.weights[at] = prior + sum;
+#pragma unroll
+    for (int k = 0; k < KT; k++)
+        if (t[k] < len) W.weights[unit * W.max_seq + t[k]] = prior[k] + sum[k];
 }
 
-template <int HD>
+template <int HD, int KT>
 __global__ void __launch_bounds__(256) k_kv8_weigh_scores(A8 A, Weigh W) {
     __shared__ float2 col[32];
-    sv_weigh_scores<HD>(A, W, blockIdx.x, blockIdx.y, col);
+    sv_weigh_scores<HD, KT>(A, W, blockIdx.x, blockIdx.y, col);
 }
 
 // The join of the attention's chunks (the first `joins` workgroups) and the weights, which only share what they read, in one launch
-template <int HD, bool SOME>
+template <int HD, bool SOME, int KT>
 __global__ void __launch_bounds__(256) k_kv8_join_weigh(A8 A, Weigh W, int joins) {
     __shared__ __attribute__((aligned(16))) float sum[1024 / HD][HD];
     __shared__ float2 col[32];
     const int bx = blockIdx.x;
-    if (bx >= joins) sv_weigh_scores<HD>(A, W, bx - joins, blockIdx.y, col);
+    if (bx >= joins) sv_weigh_scores<HD, KT>(A, W, bx - joins, blockIdx.y, col);
     else if constexpr (SOME) a8_merge_some<HD, 0>(A, 16, bx, blockIdx.y);
     else a8_merge_one<HD, 0>(A, 16, bx, blockIdx.y, sum);
 }
@@ -587,21 +599,24 @@ WeighWs sv_weigh_ws(int64_t seqs, int64_t n, int64_t nq, int64_t nkv, int64_t hd
     return w;
 }
 
+template <int HD, int KT>
+void sv_weigh_kept(const A8& A, const Weigh& W, int64_t seqs, hipStream_t s) {
+    const dim3 block(256);
+    const int64_t pieces = A.nkv * aeth_cdiv(A.max_len, 256 * KT), cols = (int64_t)A.nkv * A.cols, joins = aeth_cdiv(cols * (HD / 4), 256);
+    auto grid = [&](int64_t n) { return dim3((unsigned)n, (unsigned)seqs); };
+    if (A.chunks == 1) hipLaunchKernelGGL((k_kv8_weigh_scores<HD, KT>), grid(pieces), block, 0, s, A, W);
+    else if (a8_merge_is_some(A, seqs)) hipLaunchKernelGGL((k_kv8_join_weigh<HD, true, KT>), grid(joins + pieces), block, 0, s, A, W, (int)joins);
+    else hipLaunchKernelGGL((k_kv8_join_weigh<HD, false, KT>), grid(cols + pieces), block, 0, s, A, W, (int)cols);
+}
+
 template <int HD>
 int sv_weigh(A8 A, Weigh W, const Form& f, int64_t seqs, bool scores, hipStream_t s) {
     if (scores) {
-        const dim3 block(256);
-        const int64_t pieces = A.nkv * aeth_cdiv(A.max_len, 256), cols = (int64_t)A.nkv * A.cols;
-        hipLaunchKernelGGL((k_attn8<HD, A8_STAT | A8_SCORE>), dim3((unsigned)(A.nkv * A.ncb), (unsigned)seqs, (unsigned)A.chunks), block, 0, s, A);
+        hipLaunchKernelGGL((k_attn8<HD, A8_STAT | A8_SCORE>), dim3((unsigned)(A.nkv * A.ncb), (unsigned)seqs, (unsigned)A.chunks), dim3(256), 0, s, A);
         AETH_LAUNCH_CHECK();
-        if (A.chunks == 1) {
-            hipLaunchKernelGGL(k_kv8_weigh_scores<HD>, dim3((unsigned)pieces, (unsigned)seqs), block, 0, s, A, W);
-        } else if (a8_merge_is_some(A, seqs)) {
-            const int64_t joins = aeth_cdiv(cols * (HD / 4), 256);
-            hipLaunchKernelGGL((k_kv8_join_weigh<HD, true>), dim3((unsigned)(joins + pieces), (unsigned)seqs), block, 0, s, A, W, (int)joins);
-        } else {
-            hipLaunchKernelGGL((k_kv8_join_weigh<HD, false>), dim3((unsigned)(cols + pieces), (unsigned)seqs), block, 0, s, A, W, (int)cols);
-        }
+        // four keys a thread where one each makes more workgroups than the CUs hold at once
+        if (A.nkv * aeth_cdiv(A.max_len, 256) * seqs > 8 * (int64_t)aeth_num_cus()) sv_weigh_kept<HD, 4>(A, W, seqs, s);
+        else sv_weigh_kept<HD, 1>(A, W, seqs, s);
         AETH_LAUNCH_CHECK();
         return AETH_OK;
     }

@@ -229,7 +229,8 @@ def test_weights_long(gpu, hd, n, seq, nkv, g):
 
 @pytest.mark.parametrize("hd,nkv,g,lens,max_seq,max_len,window", [
     (128, 2, 4, [1, 0, 64, 65, 300], 310, 300, 0), (64, 1, 8, [5, 700, 1, 699], 700, 700, 0), (128, 2, 3, [50, 400, 129], 410, 400, 60),
-    (256, 1, 20, [70, 3], 80, 70, 0), (128, 8, 4, [100 + 61 * i for i in range(24)], 1600, 1503, 0), (64, 1, 70, [90, 200], 200, 200, 0)])
+    (256, 1, 20, [70, 3], 80, 70, 0), (128, 8, 4, [100 + 61 * i for i in range(24)], 1600, 1503, 0), (64, 1, 70, [90, 200], 200, 200, 0),
+    (64, 16, 2, [(37 * i) % 301 for i in range(65)], 310, 300, 0), (128, 16, 3, [5000, 1, 700, 4999, 0, 2048, 3333], 5001, 5000, 700)])
 def test_weights_batch(gpu, hd, nkv, g, lens, max_seq, max_len, window):
     torch = gpu
     b = len(lens)
