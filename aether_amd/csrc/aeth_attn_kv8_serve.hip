@@ -42,64 +42,101 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8_shared(A8 P, A
     }
 }
 
-// Joins a column's parts of the prefix (P, blocks of cw columns) and of its own tokens (O, of 16): HD/4 lanes of four dimensions, GR of such
-// groups take every GR-th part.
-template <int HD, int GR>
-__global__ void __launch_bounds__(256) k_attn8_join(A8 P, int cw, A8 O) {
-    constexpr int L = HD / 4, CW = 256 / (L * GR);  // columns a workgroup
-    __shared__ __attribute__((aligned(16))) float sum[GR > 1 ? GR : 1][GR > 1 ? HD : 4];
-    const int tid = threadIdx.x, d = 4 * (tid % L), grp = tid / L % GR, seq = blockIdx.y;
-    const int unit = blockIdx.x * CW + tid / (L * GR);
-    if (unit >= O.nkv * O.G) return;  // (uniform where GR > 1)
-    const int h = unit / O.G, g = unit % O.G;
+// A column's parts: of the prefix (P, in blocks of cw columns), then of its own tokens (O, of 16). Part k: its maximum and sum, its value from dimension d on
+template <int HD>
+struct Parts {
+    const float *p, *o;
+    int64_t step_p, step_o;
+    int of_p, stat_p, value_p, stat_o, value_o;  // parts of the prefix; offsets in a part
+    __device__ __forceinline__ Parts(const A8& P, int cw, const A8& O, int seq, int unit, int d) {
+        const int h = unit / O.G, g = unit % O.G, x = seq * O.G + g;
+        step_p = (int64_t)cw * (HD + 2);
+        step_o = 16 * (HD + 2);
+        p = P.ws + (int64_t)(h * P.ncb + x / cw) * P.chunks * step_p;
+        o = O.ws + (int64_t)((seq * O.nkv + h) * O.ncb + g / 16) * O.chunks * step_o;
+        of_p = P.chunks;
+        stat_p = cw * HD + 2 * (x % cw);
+        value_p = x % cw * HD + d;
+        stat_o = 16 * HD + 2 * (g % 16);
+        value_o = g % 16 * HD + d;
+    }
+    __device__ __forceinline__ float2 stat(int k) const { return *(const float2*)(k < of_p ? p + k * step_p + stat_p : o + (k - of_p) * step_o + stat_o); }
+    __device__ __forceinline__ a8_f4 value(int k) const { return *(const a8_f4*)(k < of_p ? p + k * step_p + value_p : o + (k - of_p) * step_o + value_o); }
+};
+// parts with something in them: all of the prefix's, the first of a sequence's own
+__device__ __forceinline__ int sv_live(const A8& P, const A8& O, int seq, int g) {
     int beg, end;
     a8_tiles(O, a8_len(O, seq), g / 16 * 16, 16, beg, end);
-    const int live_o = max(1, (end - beg + O.tpc - 1) / O.tpc);
-    a8_tiles<A8_FLAT>(P, 0, 0, 0, beg, end);
-    const int live_p = (end - beg + P.tpc - 1) / P.tpc, live = live_p + live_o;
-    const int x = seq * O.G + g;
-    const int64_t step_p = (int64_t)cw * (HD + 2), step_o = 16 * (HD + 2);
-    const float* part_p = P.ws + (int64_t)(h * P.ncb + x / cw) * P.chunks * step_p;
-    const float* part_o = O.ws + (int64_t)((seq * O.nkv + h) * O.ncb + g / 16) * O.chunks * step_o;
-    const int cp = x % cw, co = g % 16;
-    auto stat = [&](int k) { return *(const float2*)(k < live_p ? part_p + k * step_p + cw * HD + 2 * cp : part_o + (k - live_p) * step_o + 16 * HD + 2 * co); };
-    auto value = [&](int k) { return *(const a8_f4*)(k < live_p ? part_p + k * step_p + cp * HD + d : part_o + (k - live_p) * step_o + co * HD + d); };
+    return P.chunks + max(1, (end - beg + O.tpc - 1) / O.tpc);
+}
+
+// Joins many parts: a workgroup a column, HD/4 lanes of four dimensions for every 1024/HD-th part
+template <int HD>
+__global__ void __launch_bounds__(256) k_attn8_join(A8 P, int cw, A8 O) {
+    constexpr int L = HD / 4, GR = 256 / L;
+    __shared__ __attribute__((aligned(16))) float sum[GR][HD];
+    const int tid = threadIdx.x, lane = tid & 63, d = 4 * (tid % L), grp = tid / L, seq = blockIdx.y, unit = blockIdx.x;
+    const int live = sv_live(P, O, seq, unit % O.G);
+    const Parts<HD> part(P, cw, O, seq, unit, d);
     float M = -INFINITY, S = 0.0f;
-    if constexpr (GR > 1) {
-        const int lane = tid & 63;
-        for (int k = lane; k < live; k += 64) M = fmaxf(M, stat(k).x);
-        M = aeth_wave_max(M);
-        for (int k = lane; k < live; k += 64) {
-            const float2 ml = stat(k);
-            S += (ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M)) * ml.y;
-        }
-        S = aeth_wave_sum(S);
-    } else {
-#pragma unroll 4
-        for (int k = 0; k < live; k++) M = fmaxf(M, stat(k).x);
+    for (int k = lane; k < live; k += 64) M = fmaxf(M, part.stat(k).x);
+    M = aeth_wave_max(M);
+    for (int k = lane; k < live; k += 64) {
+        const float2 ml = part.stat(k);
+        S += (ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M)) * ml.y;
     }
+    S = aeth_wave_sum(S);
     a8_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int k = grp; k < live; k += GR) {
-        const float2 ml = stat(k);
-        const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
-        acc += value(k) * w;
-        if (GR == 1) S += w * ml.y;
+        const float m = part.stat(k).x;
+        acc += part.value(k) * (m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M));
     }
-    float* dst = O.out + (int64_t)seq * ((int64_t)O.nq * HD) + (int64_t)unit * HD;
-    if constexpr (GR > 1) {
-        *(a8_f4*)&sum[grp][d] = acc;
-        __syncthreads();
-        if (tid >= HD) return;
-        float y = 0.0f;
+    *(a8_f4*)&sum[grp][d] = acc;
+    __syncthreads();
+    if (tid >= HD) return;
+    float y = 0.0f;
 #pragma unroll
-        for (int i = 0; i < GR; i++) y += sum[i][tid];
-        dst[tid] = S == 0.0f ? 0.0f : y * (1.0f / S);
-    } else {
-        acc = S == 0.0f ? (a8_f4){0.0f, 0.0f, 0.0f, 0.0f} : acc * (1.0f / S);
-        if (O.ovec) *(a8_f4*)(dst + d) = acc;
-        else dst[d] = acc[0], dst[d + 1] = acc[1], dst[d + 2] = acc[2], dst[d + 3] = acc[3];
-    }
+    for (int i = 0; i < GR; i++) y += sum[i][tid];
+    O.out[(int64_t)seq * ((int64_t)O.nq * HD) + (int64_t)unit * HD + tid] = S == 0.0f ? 0.0f : y * (1.0f / S);
+}
+
+// ... and at most 8: HD/4 lanes a column, its parts all in flight at once, those without content too (they are left out behind the length,
+// which is still on its way: 2 sequences of 32 heads 5.0 µs where their number was waited for)
+constexpr int JOIN_FEW = 8;
+template <int HD>
+__global__ void __launch_bounds__(256) k_attn8_join_few(A8 P, int cw, A8 O) {
+    constexpr int L = HD / 4;
+    const int unit = (blockIdx.x * 256 + threadIdx.x) / L, d = 4 * (threadIdx.x % L), seq = blockIdx.y, all = P.chunks + O.chunks;
+    if (unit >= O.nkv * O.G) return;
+    const Parts<HD> part(P, cw, O, seq, unit, d);
+    float2 ml[JOIN_FEW];
+    a8_f4 v[JOIN_FEW];
+#pragma unroll
+    for (int k = 0; k < JOIN_FEW; k++)
+        if (k < all) {  // (uniform)
+            ml[k] = part.stat(k);
+            v[k] = part.value(k);
+        }
+    const int live = sv_live(P, O, seq, unit % O.G);
+    float M = -INFINITY, S = 0.0f;
+#pragma unroll
+    for (int k = 0; k < JOIN_FEW; k++)
+        if (k < all) M = k < live ? fmaxf(M, ml[k].x) : M;
+    a8_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < JOIN_FEW; k++)
+        if (k < all) {
+            const bool in = k < live && ml[k].x != -INFINITY;
+            const float w = __builtin_amdgcn_exp2f(ml[k].x - M);
+            S += in ? w * ml[k].y : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] += in ? v[k][e] * w : 0.0f;
+        }
+    acc = S == 0.0f ? (a8_f4){0.0f, 0.0f, 0.0f, 0.0f} : acc * (1.0f / S);
+    float* dst = O.out + (int64_t)seq * ((int64_t)O.nq * HD) + (int64_t)unit * HD + d;
+    if (O.ovec) *(a8_f4*)dst = acc;
+    else dst[0] = acc[0], dst[1] = acc[1], dst[2] = acc[2], dst[3] = acc[3];
 }
 
 // The prefix's form, 16 or 128 columns: a8_form's reckoning for columns that all see `span` tiles
@@ -161,9 +198,9 @@ int sv_shared(A8 P, A8 O, int64_t seqs, hipStream_t s) {
         if (fp.cw == 128) hipLaunchKernelGGL((k_attn8_shared<HD, 128>), grid, block, 0, s, P, O, (int)prefixes, (int)seqs);
     AETH_LAUNCH_CHECK();
     const int64_t cols = (int64_t)O.nkv * O.G;
-    constexpr int GR = 1024 / HD;
-    if (P.chunks + O.chunks <= 8) hipLaunchKernelGGL((k_attn8_join<HD, 1>), dim3((unsigned)aeth_cdiv(cols, GR), (unsigned)seqs), block, 0, s, P, fp.cw, O);
-    else hipLaunchKernelGGL((k_attn8_join<HD, GR>), dim3((unsigned)cols, (unsigned)seqs), block, 0, s, P, fp.cw, O);
+    if (P.chunks + O.chunks <= JOIN_FEW)
+        hipLaunchKernelGGL(k_attn8_join_few<HD>, dim3((unsigned)aeth_cdiv(cols, 1024 / HD), (unsigned)seqs), block, 0, s, P, fp.cw, O);
+    else hipLaunchKernelGGL(k_attn8_join<HD>, dim3((unsigned)cols, (unsigned)seqs), block, 0, s, P, fp.cw, O);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }
