@@ -19,7 +19,9 @@ namespace {
 
 // Both attentions in one launch, each a share of the workgroups: the prefix's products keep the matrix units busy, the sequences' own
 // tokens the memory. The first `prefixes` workgroups take the prefix in columns of cw (16, or 128 in the form for many), the others a sequence
-// each (its chunks after one another: the first ones, which every sequence has, first).
+// each (its chunks after one another: the first ones, which every sequence has, first). 32 / 8 heads of 128: 2 sequences behind 1000 tokens
+// 7.1 µs (in two launches 6.8 and 5.7), 160 of up to 500 tokens behind 20000 134 (138 and 25): what bounds that is the prefix's products, 0.40
+// PFLOP/s of the formula, 0.80 of the matrix units', as in aeth_attn_kv8's long prompts. 160 copies of the prefix in a batch's own caches take 1101.
 template <int HD, int CW>
 __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8_shared(A8 P, A8 O, int prefixes, int seqs) {
     constexpr int MAX = CW == 128 ? std::max((int)sizeof(float[4][16][HD + 4]), 2 * (HD / 8) * A8_KF) : (int)sizeof(float[4][16][HD + 4]);
@@ -70,7 +72,7 @@ __device__ __forceinline__ int sv_live(const A8& P, const A8& O, int seq, int g)
     return P.chunks + max(1, (end - beg + O.tpc - 1) / O.tpc);
 }
 
-// Joins many parts: a workgroup a column, HD/4 lanes of four dimensions for every 1024/HD-th part
+// Joins many parts (9 parts of 48 sequences' 32 heads of 64: 5.0 µs): a workgroup a column, HD/4 lanes of four dimensions for every 1024/HD-th part
 template <int HD>
 __global__ void __launch_bounds__(256) k_attn8_join(A8 P, int cw, A8 O) {
     constexpr int L = HD / 4, GR = 256 / L;
@@ -102,7 +104,7 @@ __global__ void __launch_bounds__(256) k_attn8_join(A8 P, int cw, A8 O) {
 }
 
 // ... and at most 8: HD/4 lanes a column, its parts all in flight at once, those without content too (they are left out behind the length,
-// which is still on its way: 2 sequences of 32 heads 5.0 µs where their number was waited for)
+// which is still on its way: 2 sequences of 32 heads 3.4 µs, 5.0 where their number was waited for; 160 6.2, 21 MB)
 constexpr int JOIN_FEW = 8;
 template <int HD>
 __global__ void __launch_bounds__(256) k_attn8_join_few(A8 P, int cw, A8 O) {
@@ -139,8 +141,13 @@ __global__ void __launch_bounds__(256) k_attn8_join_few(A8 P, int cw, A8 O) {
     else dst[0] = acc[0], dst[1] = acc[1], dst[2] = acc[2], dst[3] = acc[3];
 }
 
-// The prefix's form, 16 or 128 columns: a8_form's reckoning for columns that all see `span` tiles
-Form sv_prefix_form(int64_t cols, int64_t nkv, int64_t hd, int64_t span) {
+// The prefix's form, 16 or 128 columns: a8_form's reckoning for columns that all see `span` tiles, `own` chunks of the sequences' own tokens beside
+// them; chunks of 128 columns take any length, as even as they can be, and one more than the CUs hold at once is counted by half. 32 / 8 heads of
+// 128, µs with the form taken (the best of 13 tried): 1000 sequences behind 2000 tokens 175, 128 columns in 1 chunk (175); 256 behind 6000 101, 16
+// in 1 (88, 128 in 4); 160 behind 20000 141, 128 in 6 (139, 12; 7 chunks take 162); 64 behind 3000 21.5, 16 in 2 (21.8); 48 behind 4001 32, 16 in 6
+// (29, 4); 32 behind 8000 22.3, 16 in 4 (23.0); 17 behind 20000 32, 16 in 6 (32). The 256-column form, whose workgroup fills a CU, has no room for
+// the sequences' own beside it.
+Form sv_prefix_form(int64_t cols, int64_t nkv, int64_t hd, int64_t span, int64_t own) {
     const int64_t cus = aeth_num_cus();
     const Form small = a8_split(16, nkv * aeth_cdiv(cols, 16), span, 2 * cus, 4);
     if (hd > 128 || cols <= 64) return small;
@@ -150,16 +157,20 @@ Form sv_prefix_form(int64_t cols, int64_t nkv, int64_t hd, int64_t span) {
     for (int64_t cw : {16, 128}) {
         const int64_t units = nkv * aeth_cdiv(cols, cw);
         const double tiles = (double)units * (double)span;
-        for (int64_t target : {(int64_t)0, cus, 2 * cus, 4 * cus}) {
-            if (target > (cw == 16 ? 4 : 2) * cus) continue;
-            const Form f = a8_split(cw, units, span, std::max<int64_t>(1, target), cw == 16 ? 4 : 8);
+        const int64_t limit = (cw == 16 ? 4 : 2) * cus;
+        for (int64_t target : {(int64_t)0, cus, 2 * cus, limit, cus / units * units, std::min(limit, units * std::max<int64_t>(1, JOIN_FEW - own))}) {
+            Form f = a8_split(cw, units, span, std::max<int64_t>(1, target), cw == 16 ? 4 : 8);
+            if (cw == 128) {
+                f.tpc = (int)aeth_cdiv(span, f.chunks);
+                f.chunks = (int)aeth_cdiv(span, f.tpc);
+            }
             const int64_t wgs = units * f.chunks;
             const double w = tiles / c, tpc = (double)std::min<int64_t>(f.tpc, span);
             const double u = (double)aeth_cdiv(wgs, cus), q = u * (tiles / (double)wgs);
-            double t = cw == 128   ? (hd == 128 ? std::max(8.0 + 2.3 * tpc, 22.0 + 1.96 * w) : std::max(7.0 + 1.53 * tpc, 15.0 + 1.25 * w))
+            double t = cw == 128   ? (hd == 128 ? std::max(8.0 + 2.3 * tpc, 22.0 + 0.98 * (w + q)) : std::max(7.0 + 1.53 * tpc, 15.0 + 0.625 * (w + q)))
                        : hd == 128 ? std::max(5.5 + 0.45 * tpc, 6.0 + 0.33 * q + 4.5 * std::ceil(u / 3.0))
                                    : std::max(5.0 + 0.3 * tpc, 5.0 + 0.185 * q + 2.8 * std::ceil(u / 4.0));
-            t += (cw == 16 ? 2e-6 : 1e-6) * (double)(nkv * cols * f.chunks) * (double)(hd + 2);
+            t += 3e-6 * (double)(nkv * cols * f.chunks) * (double)(hd + 2) + (f.chunks + own > JOIN_FEW ? 2.5 : 0.0);
             if (t < least) {
                 least = t;
                 best = f;
@@ -188,7 +199,7 @@ int sv_shared(A8 P, A8 O, int64_t seqs, hipStream_t s) {
     Form fp = {16, 0, 4};
     if (P.max_len > 0) {
         const int64_t span = aeth_cdiv(P.max_len, KV8_TILE) - (P.window > 0 ? std::max(0, P.max_len - P.window) / KV8_TILE : 0);
-        fp = sv_prefix_form(P.cols, P.nkv, HD, span);
+        fp = sv_prefix_form(P.cols, P.nkv, HD, span, O.chunks);
     }
     a8_take(P, fp);
     const int64_t prefixes = (int64_t)P.nkv * P.ncb * P.chunks, own = (int64_t)O.nkv * O.ncb * seqs * O.chunks;
@@ -241,7 +252,8 @@ __device__ __forceinline__ float2 sv_column(const A8& A, int len, int seq, int h
     return make_float2(M, 1.0f / S);
 }
 
-// From the scores: workgroup (256·KT keys, KV head), the columns 32 at a time, their statistics first
+// From the scores: workgroup (256·KT keys, KV head), the columns 32 at a time, their statistics first. Latency bounds it: a length, chunks'
+// statistics, the sum.
 template <int HD, int KT>
 __device__ __forceinline__ void sv_weigh_scores(const A8& A, const Weigh& W, int bx, int seq, float2 (&col)[32]) {
     const int tid = threadIdx.x, h = bx % A.nkv, t0 = bx / A.nkv * (256 * KT);
@@ -298,7 +310,8 @@ __global__ void __launch_bounds__(256) k_kv8_weigh_scores(A8 A, Weigh W) {
     sv_weigh_scores<HD, KT>(A, W, blockIdx.x, blockIdx.y, col);
 }
 
-// The join of the attention's chunks (the first `joins` workgroups) and the weights, which only share what they read, in one launch
+// The join of the attention's chunks (the first `joins` workgroups) and the weights, which only share what they read, in one launch. 32 / 8
+// heads: a token over 2049 3.5 µs (a launch each: 3.3 and 7.8), 32 sequences of up to 4096 7.5 (4.6 and 10.1; 9.1 with one key a thread).
 template <int HD, bool SOME, int KT>
 __global__ void __launch_bounds__(256) k_kv8_join_weigh(A8 A, Weigh W, int joins) {
     __shared__ __attribute__((aligned(16))) float sum[1024 / HD][HD];
@@ -335,7 +348,10 @@ __device__ __forceinline__ int sv_count(const A8& A, const Weigh& W, int group, 
 
 // Many columns: a wave keeps NT·32 keys as fp16 in registers, its workgroup of eight waves 512 (256), and goes through W.per blocks of 32
 // of the columns that see them: their q as two fp16 parts from LDS (the attention's own products, aeth_attn_kv8_dev.hpp), the exponentials
-// summed in registers over the blocks and at the end over the lanes.
+// summed in registers over the blocks and at the end over the lanes. 32 / 8 heads of 128, a 2000-token prompt: 55 µs, 0.30 PFLOP/s of the formula
+// (QKᵀ once), 0.60 of the matrix units'. A block takes 4170 cycles, its products 2050 of them on each matrix unit and 3370 of instructions
+// beside them: an exponential and three more for each of 64 keys and 32 columns a lane pair, and making q's parts. The clock falls to 1.9 GHz.
+// The first block comes 9000 cycles late (the keys).
 template <int HD>
 __global__ void __launch_bounds__(512, 2) k_kv8_weigh(A8 A, Weigh W) {
     constexpr int GK = sv_group(HD), NT = GK / 256, KS = HD / 16, KF = 1040, E = HD / 16, EV = E < 8 ? E : 8;
@@ -565,7 +581,7 @@ __global__ void __launch_bounds__(512, 2) k_kv8_weigh(A8 A, Weigh W) {
     if (key < len) W.weights[at] = W.prior ? W.prior[at] + v : v;
 }
 
-// weights = prior + the chunks' sums; groups of gk keys
+// weights = prior + the chunks' sums; groups of gk keys (2000 keys of 8 heads in up to 12 chunks 5.2 µs)
 __global__ void __launch_bounds__(256) k_kv8_weigh_sum(A8 A, Weigh W, int gk) {
     const int t0 = blockIdx.x * 256, t = t0 + threadIdx.x, h = blockIdx.y, group = t0 / gk;
     int chunks = 0;

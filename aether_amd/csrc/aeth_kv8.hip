@@ -417,7 +417,8 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_v(QkArgs A) {
 __device__ __forceinline__ float qk_squares(float4 a) { return fmaf(a.x, a.x, a.y * a.y) + fmaf(a.z, a.z, a.w * a.w); }
 
 // Several axes: the four pairs of a lane take their table entries one by one, each from the row of its axis' position, and
-// serve HEADS heads of the token.
+// serve HEADS heads of the token: four, where that leaves each CU four workgroups, else one. 4000 rows of 32 + 8 heads of 128 by three axes 27 µs
+// (6.1 TB/s; with inputs not in the caches 34); one head a thread 50, two, three, eight in turn 38, 36, 39 against those 34.
 template <int HD, int HEADS>
 __global__ void __launch_bounds__(256) k_qk_norm_rope_axes_v(QkArgs A, QkAxes X) {
     constexpr int L = HD / 8, HALF = HD / 2;

@@ -205,7 +205,8 @@ __device__ __forceinline__ void ev_number(const EvictState& S, const EvictHeld<P
 
 // One workgroup a head of up to 32768 tokens. The last key that stays is found by up to three passes over the keys' bits (11, 11, 10) with
 // counts in LDS (two, but for weights that are equal or nearly), the slots that stay numbered in a last one. What bounds it is instructions, on one
-// CU a head: hence one word that says all of a token. 8 heads of 2500 tokens 8.5 µs, of 30000 18.
+// CU a head: hence one word that says all of a token. 8 heads of 2500 tokens 7.0 µs, of 30000 19 (40 with weights read again in each pass
+// and a scan over threads); 24 sequences' 4 heads of up to 4001 7.6.
 __global__ void __launch_bounds__(SEL) k_kv8_select(EvictArgs A) {
     __shared__ EvictLds lds;
     const int seq = blockIdx.y, len = (int)ev_len(A, seq);
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(SEL) k_kv8_select(EvictArgs A) {
 
 // More tokens: many workgroups a head, a chunk of its slots each, and a launch for each pass. The workgroups of a pass leave their counts in memory,
 // those of the next one add all of them up and go on from there, each for itself; the last launch knows from the counts how many stay before its chunk.
-// 8 heads of 131000 tokens: one workgroup a head, which reads its weights again in each pass, 107 µs.
+// 8 heads of 131000 tokens: 5 + 7 + 8 + 15 µs; one workgroup a head, which reads its weights again in each pass, 112.
 struct EvictFar {
     uint32_t* hist;   // [3 passes][units][chunks][2048]
     uint32_t* state;  // [2][units][4]: behind the first pass, the second
@@ -408,7 +409,9 @@ __device__ __forceinline__ void ev_weights(const EvictArgs& A, int64_t unit, int
     for (int64_t t = t0 + threadIdx.x; t < t1; t += 256) dst[t] = t < rows ? src[t] : 0.0f;
 }
 
-// blocks: the tiles of kept tokens of a head, then pieces of its weights
+// blocks: the tiles of kept tokens of a head, then pieces of its weights. Memory bounds it where much is kept: half of 64 sequences' 4096 tokens
+// of 8 heads of 128 155 µs, 4.5 TB/s of what it touches (all rows of V, kept rows of K, both written); 2048 of 2500 tokens 7.5, the way from the
+// list to the bytes. A lane takes bytes of four tokens that are a word of the destination: neighbours mostly share a source line.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_gather(EvictArgs A, uint8_t* dst, int64_t dst_seq_bytes, int64_t dst_head_bytes) {
     __shared__ int from[KV8_TILE];
@@ -431,7 +434,7 @@ __global__ void __launch_bounds__(256) k_kv8_gather(EvictArgs A, uint8_t* dst, i
                 A.cache + seq * A.seq_bytes + (int64_t)h * A.tiles * aeth_kv8_tile_bytes(HD), from, n);
 }
 
-// in place: the gathered tiles from the workspace
+// in place: the gathered tiles from the workspace (the 64 sequences' 96 µs: 5.8 TB/s)
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_put_back(EvictArgs A, const uint8_t* stage, int64_t stage_seq_bytes, int64_t stage_head_bytes) {
     __shared__ int from[KV8_TILE];
@@ -523,7 +526,8 @@ int evict(const char* what, const void* cache, int64_t stride, const float* weig
     int64_t all, dst_all, w_all, dw_all, k_all = 0;
     if (seqs < 0 || seqs > 65535 || stride < 0 || dst_stride < 0 || ((stride | dst_stride) & 15) || (seqs > 1 && (stride < bytes || dst_stride < dst_bytes)) ||
         !aeth_mul_ok(seqs, std::max(stride, bytes), &all) || !aeth_mul_ok(seqs, std::max(dst_stride, dst_bytes), &dst_all) ||
-        (kept && !aeth_mul_ok(seqs * nkv, keep, &k_all)) || k_all > INT64_MAX / 4 || !aeth_mul_ok(seqs * nkv, max_seq, &w_all) || !aeth_mul_ok(seqs * nkv, dst_seq, &dw_all) || w_all > INT64_MAX / 4 || dw_all > INT64_MAX / 4)
+        (kept && !aeth_mul_ok(seqs * nkv, keep, &k_all)) || !aeth_mul_ok(seqs * nkv, max_seq, &w_all) || !aeth_mul_ok(seqs * nkv, dst_seq, &dw_all) ||
+        k_all > INT64_MAX / 4 || w_all > INT64_MAX / 4 || dw_all > INT64_MAX / 4)
         return aeth_set_error(AETH_EINVAL, "%s: %lld sequences %lld and %lld bytes apart", what, (long long)seqs, (long long)stride, (long long)dst_stride);
     const bool in_place = dst == cache;
     if (in_place ? dst_seq != max_seq || (seqs > 1 && dst_stride != stride) : !apart(cache, all, dst, dst_all))
