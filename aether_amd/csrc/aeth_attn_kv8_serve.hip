@@ -608,9 +608,11 @@ int64_t sv_sums(int64_t units) { return 4 * (int64_t)aeth_num_cus() + units; }
 // blocks beside its own (its keys, the sum over lanes), so: the least rounds·(per + 2) of one to four rounds of workgroups.
 void sv_chunks(Weigh& W, int64_t n, int64_t G, int64_t nkv, int64_t hd, int64_t len, int64_t window) {
     const int64_t gk = sv_group((int)hd), cus = aeth_num_cus(), end = aeth_cdiv(len, gk), begin = window > 0 ? std::max<int64_t>(0, len - n + 1 - window) / gk : 0;
-    int64_t most = 1, all = 0;
     auto blocks = [&](int64_t g) { return std::max<int64_t>(1, sv_seen((int)n, (int)G, (int)len, (int)window, gk * g, (int)gk).blocks); };
-    for (int64_t g = begin; g < end; g++) {
+    // the groups before `some` are seen by every query; the others, as many as the queries and a window reach, are counted one by one
+    const int64_t some = window > 0 ? begin : std::min<int64_t>(end, (len - n) / gk + 1);
+    int64_t most = some > begin ? blocks(begin) : 1, all = (some - begin) * most;
+    for (int64_t g = some; g < end; g++) {
         all += blocks(g);
         most = std::max(most, blocks(g));
     }
@@ -619,8 +621,8 @@ void sv_chunks(Weigh& W, int64_t n, int64_t G, int64_t nkv, int64_t hd, int64_t 
     for (int64_t rounds = 1; rounds <= 4; rounds++)
         for (int64_t more = 0; more < 3; more++) {
             const int64_t per = std::min(std::max(fewest, aeth_cdiv(all * nkv, rounds * cus) + more), most);
-            int64_t wgs = 0;
-            for (int64_t g = begin; g < end; g++) wgs += aeth_cdiv(blocks(g), per);
+            int64_t wgs = (some - begin) * aeth_cdiv(most, per);
+            for (int64_t g = some; g < end; g++) wgs += aeth_cdiv(blocks(g), per);
             const int64_t cost = aeth_cdiv(wgs * nkv, cus) * (per + 2);
             if (cost < least) {
                 least = cost;
@@ -631,9 +633,9 @@ void sv_chunks(Weigh& W, int64_t n, int64_t G, int64_t nkv, int64_t hd, int64_t 
     W.chunks = (int)aeth_cdiv(most, best);
     W.first = W.chunks > 1 ? (int)begin : 0;  // one chunk: every group, those that nothing sees for their prior
     W.keys = (end - W.first) * gk;
-    W.full = window > 0 ? 0 : (int)(std::min<int64_t>(end, (len - n) / gk + 1));  // those that every query sees
-    W.wgs = 0;
-    for (int64_t g = W.first; g < end; g++) W.wgs += (int)aeth_cdiv(blocks(g), best);
+    W.full = (int)(W.chunks == 1 ? end : some - begin);  // (begin > 0 with a window only)
+    W.wgs = W.full * W.chunks;
+    for (int64_t g = W.first + W.full; g < end; g++) W.wgs += (int)aeth_cdiv(blocks(g), best);
 }
 
 // the workspace's parts, bytes from its start: the attention's own, columns' statistics, scores or sums by chunk

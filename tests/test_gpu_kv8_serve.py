@@ -74,6 +74,22 @@ def test_shared_prefix_long(gpu, hd, seqs, nkv, g, prefix_len):
     within(torch, got, *S.shared(q, prefix, prefix_len, prefix_len, layers, lens, nkv, hd, 320, 0))
 
 
+@pytest.mark.parametrize("hd,seqs,nkv,g,prefix_len,window", [
+    (128, 100, 2, 4, 5000, 3001), (128, 100, 2, 4, 5000, 150), (64, 90, 4, 4, 4001, 2000), (128, 40, 8, 8, 3500, 3333), (256, 40, 1, 4, 1500, 700)])
+def test_shared_prefix_long_with_a_window(gpu, hd, seqs, nkv, g, prefix_len, window):
+    """Sequences of one block whose windows begin in different tiles of the prefix, and those whose window leaves it; what no window reaches holds NaN scales."""
+    torch = gpu
+    lens = [(53 * b) % 301 for b in range(seqs)]
+    prefix = some_layer(torch, 1, nkv, hd, prefix_len)
+    layers = some_layers(torch, 9, seqs, nkv, hd, 320)
+    poison(torch, prefix, nkv, hd, prefix_len, range(0, prefix_len - window))
+    for b in range(seqs):
+        poison(torch, layers[b], nkv, hd, 320, range(lens[b], 320))
+    q = rand(torch, 2, seqs, nkv * g * hd)
+    got = shared(torch, q, prefix, prefix_len, prefix_len, layers, ints(torch, lens), nkv, hd, 320, 300, window)
+    within(torch, got, *S.shared(q, prefix, prefix_len, prefix_len, layers, lens, nkv, hd, 320, window))
+
+
 def poison(torch, layer, nkv, hd, max_seq, slots, part=2):
     """NaN as the scales of slots: part 0 of K, 1 of V, 2 of both."""
     view = layer.reshape(nkv, -1, 128 * hd + 512)
@@ -227,6 +243,24 @@ def test_weights_long(gpu, hd, n, seq, nkv, g):
     assert torch.equal(again[0], out) and torch.equal(again[1], w)
 
 
+@pytest.mark.parametrize("hd,n,seq,nkv,g,window", [
+    (128, 60, 9000, 2, 4, 900), (64, 60, 9000, 2, 1, 5), (256, 40, 6000, 1, 4, 1000), (128, 900, 5000, 2, 4, 1500), (64, 300, 7000, 1, 8, 6950),
+    (128, 700, 4200, 8, 4, 1)])
+def test_weights_of_a_long_cache_with_a_window(gpu, hd, n, seq, nkv, g, window):
+    """The columns of a group of keys in one chunk and in several; keys before every window, with NaN scales, keep their prior."""
+    torch = gpu
+    layer = some_layer(torch, n, nkv, hd, seq)
+    poison(torch, layer, nkv, hd, seq, range(0, max(0, seq - n + 1 - window)))
+    q = rand(torch, seq, n, nkv * g * hd)
+    prior = rand(torch, 5, nkv, seq).abs()
+    out, w = weigh(torch, q, layer, nkv, hd, seq, seq, window, prior)
+    o, ot, ww, wt = S.weights(q, layer, nkv, hd, seq, seq, window, prior)
+    within(torch, out, o, ot)
+    within(torch, w, ww, wt)
+    dark = max(0, seq - n + 1 - window)
+    assert torch.equal(w[:, :dark], prior[:, :dark])
+
+
 @pytest.mark.parametrize("hd,nkv,g,lens,max_seq,max_len,window", [
     (128, 2, 4, [1, 0, 64, 65, 300], 310, 300, 0), (64, 1, 8, [5, 700, 1, 699], 700, 700, 0), (128, 2, 3, [50, 400, 129], 410, 400, 60),
     (256, 1, 20, [70, 3], 80, 70, 0), (128, 8, 4, [100 + 61 * i for i in range(24)], 1600, 1503, 0), (64, 1, 70, [90, 200], 200, 200, 0),
@@ -245,6 +279,21 @@ def test_weights_batch(gpu, hd, nkv, g, lens, max_seq, max_len, window):
                 assert (out[i] == 0).all() and (w[i] == 7.0).all()
             else:
                 check_weights(torch, (out[i:i + 1], w[i]), want, nkv, seq)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n,seq,window", [(1, 700, 0), (3, 700, 100), (90, 700, 0), (90, 700, 33)])
+def test_weights_take_strides_and_any_alignment(gpu, hd, n, seq, window):
+    torch = gpu
+    nkv, g, max_seq = 2, 4, 701
+    layer = some_layer(torch, n, nkv, hd, max_seq)
+    wide = rand(torch, seq, n, nkv * g * hd + 7)
+    q = wide[:, 3:3 + nkv * g * hd]
+    out = torch.full((n * nkv * g * hd + 1,), math.nan, device="cuda")[1:].view(n, -1)
+    prior = rand(torch, 5, nkv * max_seq + 1).abs()[1:].view(nkv, max_seq)
+    into = torch.full((nkv * max_seq + 3,), 7.0, device="cuda")[3:].view(nkv, max_seq)
+    got = weigh(torch, q, layer, nkv, hd, max_seq, seq, window, prior, into, out=out)
+    check_weights(torch, got, S.weights(q.contiguous(), layer, nkv, hd, max_seq, seq, window, prior), nkv, seq)
 
 
 def test_weights_without_queries_are_the_prior(gpu):
