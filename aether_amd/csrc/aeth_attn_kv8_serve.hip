@@ -20,8 +20,8 @@ namespace {
 // Both attentions in one launch, each a share of the workgroups: the prefix's products keep the matrix units busy, the sequences' own
 // tokens the memory. The first `prefixes` workgroups take the prefix in columns of cw (16, or 128 in the form for many), the others a sequence
 // each (its chunks after one another: the first ones, which every sequence has, first). 32 / 8 heads of 128: 2 sequences behind 1000 tokens
-// 7.1 µs (in two launches 6.8 and 5.7), 160 of up to 500 tokens behind 20000 134 (138 and 25): what bounds that is the prefix's products, 0.40
-// PFLOP/s of the formula, 0.80 of the matrix units', as in aeth_attn_kv8's long prompts. 160 copies of the prefix in a batch's own caches take 1101.
+// 7.1 µs (in two launches 6.8 and 5.7), 160 of up to 500 tokens behind 20000 140 (138 and 25): what bounds that is the prefix's products, 0.38
+// PFLOP/s of the formula, 0.76 of the matrix units', as in aeth_attn_kv8's long prompts. 160 copies of the prefix in a batch's own caches take 1101.
 template <int HD, int CW>
 __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8_shared(A8 P, A8 O, int prefixes, int seqs) {
     constexpr int MAX = CW == 128 ? std::max((int)sizeof(float[4][16][HD + 4]), 2 * (HD / 8) * A8_KF) : (int)sizeof(float[4][16][HD + 4]);
