@@ -20,8 +20,8 @@ namespace {
 // Both attentions in one launch, each a share of the workgroups: the prefix's products keep the matrix units busy, the sequences' own
 // tokens the memory. The first `prefixes` workgroups take the prefix in columns of cw (16, or 128 in the form for many), the others a sequence
 // each (its chunks after one another: the first ones, which every sequence has, first). 32 / 8 heads of 128: 2 sequences behind 1000 tokens
-// 7.1 µs (in two launches 6.8 and 5.7), 160 of up to 500 tokens behind 20000 140 (138 and 25): what bounds that is the prefix's products, 0.38
-// PFLOP/s of the formula, 0.76 of the matrix units', as in aeth_attn_kv8's long prompts. 160 copies of the prefix in a batch's own caches take 1101.
+// 7.1 µs (in two launches 6.8 and 5.7), 160 of up to 500 tokens behind 20000 125 (138 and 25): what bounds that is the prefix's products, 0.42
+// PFLOP/s of the formula, 0.84 of the matrix units', as in aeth_attn_kv8's long prompts. 160 copies of the prefix in a batch's own caches take 1101.
 template <int HD, int CW>
 __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_attn8_shared(A8 P, A8 O, int prefixes, int seqs) {
     constexpr int MAX = CW == 128 ? std::max((int)sizeof(float[4][16][HD + 4]), 2 * (HD / 8) * A8_KF) : (int)sizeof(float[4][16][HD + 4]);
@@ -72,7 +72,7 @@ __device__ __forceinline__ int sv_live(const A8& P, const A8& O, int seq, int g)
     return P.chunks + max(1, (end - beg + O.tpc - 1) / O.tpc);
 }
 
-// Joins many parts (9 parts of 48 sequences' 32 heads of 64: 5.0 µs): a workgroup a column, HD/4 lanes of four dimensions for every 1024/HD-th part
+// Joins many parts (2 sequences behind 60000 tokens, 60 parts): a workgroup a column, HD/4 lanes of four dimensions for every 1024/HD-th part
 template <int HD>
 __global__ void __launch_bounds__(256) k_attn8_join(A8 P, int cw, A8 O) {
     constexpr int L = HD / 4, GR = 256 / L;
@@ -103,19 +103,20 @@ __global__ void __launch_bounds__(256) k_attn8_join(A8 P, int cw, A8 O) {
     O.out[(int64_t)seq * ((int64_t)O.nq * HD) + (int64_t)unit * HD + tid] = S == 0.0f ? 0.0f : y * (1.0f / S);
 }
 
-// ... and at most 8: HD/4 lanes a column, its parts all in flight at once, those without content too (they are left out behind the length,
-// which is still on its way: 2 sequences of 32 heads 3.4 µs, 5.0 where their number was waited for; 160 6.2, 21 MB)
-constexpr int JOIN_FEW = 8;
-template <int HD>
+// ... and at most MOST, 8 or 16: HD/4 lanes a column, its parts all in flight at once, those without content too (they are left out behind the length,
+// which is still on its way: 2 sequences of 32 heads 3.4 µs, 5.0 where their number was waited for; 160 of 13 parts 8.8, 13.1 with a workgroup a
+// column)
+constexpr int JOIN_FEW = 8, JOIN_MORE = 16;
+template <int HD, int MOST>
 __global__ void __launch_bounds__(256) k_attn8_join_few(A8 P, int cw, A8 O) {
     constexpr int L = HD / 4;
     const int unit = (blockIdx.x * 256 + threadIdx.x) / L, d = 4 * (threadIdx.x % L), seq = blockIdx.y, all = P.chunks + O.chunks;
     if (unit >= O.nkv * O.G) return;
     const Parts<HD> part(P, cw, O, seq, unit, d);
-    float2 ml[JOIN_FEW];
-    a8_f4 v[JOIN_FEW];
+    float2 ml[MOST];
+    a8_f4 v[MOST];
 #pragma unroll
-    for (int k = 0; k < JOIN_FEW; k++)
+    for (int k = 0; k < MOST; k++)
         if (k < all) {  // (uniform)
             ml[k] = part.stat(k);
             v[k] = part.value(k);
@@ -123,11 +124,11 @@ __global__ void __launch_bounds__(256) k_attn8_join_few(A8 P, int cw, A8 O) {
     const int live = sv_live(P, O, seq, unit % O.G);
     float M = -INFINITY, S = 0.0f;
 #pragma unroll
-    for (int k = 0; k < JOIN_FEW; k++)
+    for (int k = 0; k < MOST; k++)
         if (k < all) M = k < live ? fmaxf(M, ml[k].x) : M;
     a8_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < JOIN_FEW; k++)
+    for (int k = 0; k < MOST; k++)
         if (k < all) {
             const bool in = k < live && ml[k].x != -INFINITY;
             const float w = __builtin_amdgcn_exp2f(ml[k].x - M);
@@ -142,14 +143,15 @@ __global__ void __launch_bounds__(256) k_attn8_join_few(A8 P, int cw, A8 O) {
 }
 
 // The prefix's form, 16 or 128 columns: a8_form's reckoning for columns that all see `span` tiles, `own` chunks of the sequences' own tokens beside
-// them; chunks of 128 columns take any length, as even as they can be, and one more than the CUs hold at once is counted by half. 32 / 8 heads of
-// 128, µs with the form taken (the best of 13 tried): 1000 sequences behind 2000 tokens 175, 128 columns in 1 chunk (175); 256 behind 6000 101, 16
-// in 1 (88, 128 in 4); 160 behind 20000 141, 128 in 6 (139, 12; 7 chunks take 162); 64 behind 3000 21.5, 16 in 2 (21.8); 48 behind 4001 32, 16 in 6
-// (29, 4); 32 behind 8000 22.3, 16 in 4 (23.0); 17 behind 20000 32, 16 in 6 (32). The 256-column form, whose workgroup fills a CU, has no room for
-// the sequences' own beside it.
+// them; chunks of 128 columns take any length, as even as they can be, and what a part-filled round adds is counted by half. 32 / 8 heads of 128, µs
+// with the form taken (the best of 10 to 13 tried): 1000 sequences behind 2000 tokens 175, 128 columns in 1 chunk (175); 256 behind 6000 86, 128 in 4
+// (84); 200 behind 12000 117, 128 in 4 (113, 8); 160 behind 10000 78, 128 in 6 (78); 160 behind 20000 132, 128 in 12 (130; 6 chunks 137, 7 162);
+// 120 behind 20000 111, 128 in 8 (111); 64 behind 3000 21.5, 16 in 2 (21.5); 48 behind 4001 32, 16 in 2 (29, 4); 32 behind 8000 22.3, 16 in 4 (22.3);
+// 17 behind 20000 32, 16 in 6 (32). The 256-column form, whose workgroup fills a CU, has no room for the sequences' own beside it.
 Form sv_prefix_form(int64_t cols, int64_t nkv, int64_t hd, int64_t span, int64_t own) {
     const int64_t cus = aeth_num_cus();
-    const Form small = a8_split(16, nkv * aeth_cdiv(cols, 16), span, 2 * cus, 4);
+    // (at head_dim 256 a workgroup fills a CU: 32 sequences behind 8000 tokens of 16 / 4 heads in 8 chunks 33 µs, in 16 41)
+    const Form small = a8_split(16, nkv * aeth_cdiv(cols, 16), span, (hd == 256 ? 1 : 2) * cus, 4);
     if (hd > 128 || cols <= 64) return small;
     const double c = (double)cus;
     Form best = small;
@@ -158,7 +160,8 @@ Form sv_prefix_form(int64_t cols, int64_t nkv, int64_t hd, int64_t span, int64_t
         const int64_t units = nkv * aeth_cdiv(cols, cw);
         const double tiles = (double)units * (double)span;
         const int64_t limit = (cw == 16 ? 4 : 2) * cus;
-        for (int64_t target : {(int64_t)0, cus, 2 * cus, limit, cus / units * units, std::min(limit, units * std::max<int64_t>(1, JOIN_FEW - own))}) {
+        for (int64_t target : {(int64_t)0, cus, 2 * cus, limit, cus / units * units, (cw == 128 ? 2 * cus / units * units : cus),
+                               std::min(limit, units * std::max<int64_t>(1, JOIN_FEW - own))}) {
             Form f = a8_split(cw, units, span, std::max<int64_t>(1, target), cw == 16 ? 4 : 8);
             if (cw == 128) {
                 f.tpc = (int)aeth_cdiv(span, f.chunks);
@@ -170,7 +173,8 @@ Form sv_prefix_form(int64_t cols, int64_t nkv, int64_t hd, int64_t span, int64_t
             double t = cw == 128   ? (hd == 128 ? std::max(8.0 + 2.3 * tpc, 22.0 + 0.98 * (w + q)) : std::max(7.0 + 1.53 * tpc, 15.0 + 0.625 * (w + q)))
                        : hd == 128 ? std::max(5.5 + 0.45 * tpc, 6.0 + 0.33 * q + 4.5 * std::ceil(u / 3.0))
                                    : std::max(5.0 + 0.3 * tpc, 5.0 + 0.185 * q + 2.8 * std::ceil(u / 4.0));
-            t += 3e-6 * (double)(nkv * cols * f.chunks) * (double)(hd + 2) + (f.chunks + own > JOIN_FEW ? 2.5 : 0.0);
+            t += (cw == 128 && hd == 128 ? 1.5e-6 : 3e-6) * (double)(nkv * cols * f.chunks) * (double)(hd + 2);
+            if (f.chunks + own > (cw == 128 ? JOIN_MORE : JOIN_FEW)) t += 2.5;
             if (t < least) {
                 least = t;
                 best = f;
@@ -209,8 +213,10 @@ int sv_shared(A8 P, A8 O, int64_t seqs, hipStream_t s) {
         if (fp.cw == 128) hipLaunchKernelGGL((k_attn8_shared<HD, 128>), grid, block, 0, s, P, O, (int)prefixes, (int)seqs);
     AETH_LAUNCH_CHECK();
     const int64_t cols = (int64_t)O.nkv * O.G;
-    if (P.chunks + O.chunks <= JOIN_FEW)
-        hipLaunchKernelGGL(k_attn8_join_few<HD>, dim3((unsigned)aeth_cdiv(cols, 1024 / HD), (unsigned)seqs), block, 0, s, P, fp.cw, O);
+    const int parts = P.chunks + O.chunks;
+    const dim3 few((unsigned)aeth_cdiv(cols, 1024 / HD), (unsigned)seqs);
+    if (parts <= JOIN_FEW) hipLaunchKernelGGL((k_attn8_join_few<HD, JOIN_FEW>), few, block, 0, s, P, fp.cw, O);
+    else if (parts <= JOIN_MORE) hipLaunchKernelGGL((k_attn8_join_few<HD, JOIN_MORE>), few, block, 0, s, P, fp.cw, O);
     else hipLaunchKernelGGL(k_attn8_join<HD>, dim3((unsigned)cols, (unsigned)seqs), block, 0, s, P, fp.cw, O);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
