@@ -357,7 +357,7 @@ __device__ __forceinline__ int sv_count(const A8& A, const Weigh& W, int group, 
 // summed in registers over the blocks and at the end over the lanes. 32 / 8 heads of 128, a 2000-token prompt: 55 µs, 0.30 PFLOP/s of the formula
 // (QKᵀ once), 0.60 of the matrix units'. A block takes 4170 cycles, its products 2050 of them on each matrix unit and 3370 of instructions
 // beside them: an exponential and three more for each of 64 keys and 32 columns a lane pair, and making q's parts. The clock falls to 1.9 GHz.
-// The first block comes 9000 cycles late (the keys).
+// The first block comes some 6500 cycles late (the keys; 2500 more with loads of 8 bytes a lane).
 template <int HD>
 __global__ void __launch_bounds__(512, 2) k_kv8_weigh(A8 A, Weigh W) {
     constexpr int GK = sv_group(HD), NT = GK / 256, KS = HD / 16, KF = 1040, E = HD / 16, EV = E < 8 ? E : 8;
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(512, 2) k_kv8_weigh(A8 A, Weigh W) {
                     lo[i] = (_Float16)(v - (float)hi[i]);
                 }
                 const int dim = E * sj + e;
-                char* dst = qb[buf] + (dim >> 4) * KF + (sc + 32 * (dim >> 3 & 1)) * 16 + 2 * (dim & 7);
+                char* dst = qb[buf] + (2 * (dim >> 5) + (dim >> 3 & 1)) * KF + (sc + 32 * (dim >> 4 & 1)) * 16 + 2 * (dim & 7);  // as the keys' order
                 *(part*)dst = hi;
                 *(part*)(dst + KS * KF) = lo;
             }
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(512, 2) k_kv8_weigh(A8 A, Weigh W) {
             }
         };
         fetch();
-        // keys: lane (key l%32, half l/32) of fragment (T, ks) holds eight dimensions
+        // keys: lane (key l%32, half l/32) of fragments (T, 2·s) and (T, 2·s + 1) holds eight each of the dimensions 32·s + 16·half .. + 15
         const uint8_t* p = A.cache + ((int64_t)h * A.tiles + min(k0, len - 1) / KV8_TILE) * aeth_kv8_tile_bytes(HD);
         a8_h8 kf[NT][KS];
         float sk[NT];
@@ -465,10 +465,11 @@ __global__ void __launch_bounds__(512, 2) k_kv8_weigh(A8 A, Weigh W) {
             const float ks = *(const float*)(p + 2 * KV8_TILE * HD + 4 * st), vs = *(const float*)(p + 2 * KV8_TILE * HD + 4 * (KV8_TILE + st));
             sk[T] = fabsf(vs) < INFINITY ? ks : __uint_as_float(0x7FC00000u);
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const uint2 k = *(const uint2*)(p + (half + c) * HD + 16 * s + 8 * hf);
-                const a8_h4 a = a8_half4(k.x), b = a8_half4(k.y);
-                kf[T][s] = (a8_h8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+            for (int s = 0; s < KS / 2; s++) {
+                const uint4 k = *(const uint4*)(p + (half + c) * HD + 32 * s + 16 * hf);
+                const a8_h4 a = a8_half4(k.x), b = a8_half4(k.y), d = a8_half4(k.z), e = a8_half4(k.w);
+                kf[T][2 * s] = (a8_h8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                kf[T][2 * s + 1] = (a8_h8){d[0], d[1], d[2], d[3], e[0], e[1], e[2], e[3]};
             }
         }
         // Some column of the blocks [w0, w1) sees a key of the wave. (At a prompt's diagonal half of the waves see none, and the others have
