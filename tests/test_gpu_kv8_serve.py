@@ -59,9 +59,10 @@ def test_shared_prefix(gpu, hd, seqs, prefix_len, lens, nkv, g, window):
     within(torch, got, *S.shared(q, prefix, prefix_len, prefix_seq, layers, lens, nkv, hd, max_seq, window))
 
 
-@pytest.mark.parametrize("hd,seqs,nkv,g,prefix_len", [(128, 100, 2, 4, 5000), (128, 3, 1, 4, 20000), (64, 64, 1, 8, 6001), (128, 70, 8, 1, 2500)])
+@pytest.mark.parametrize("hd,seqs,nkv,g,prefix_len", [(128, 100, 2, 4, 5000), (128, 3, 1, 4, 20000), (64, 64, 1, 8, 6001), (128, 70, 8, 1, 2500), (128, 16, 8, 4, 3000),
+                                                           (64, 15, 4, 8, 3000), (256, 16, 4, 4, 2500), (128, 160, 8, 1, 4100)])
 def test_shared_prefix_long(gpu, hd, seqs, nkv, g, prefix_len):
-    """Many chunks of the prefix, blocks of 128 and 256 columns; the slots behind the prefix and the lengths hold NaN scales."""
+    """Many chunks of the prefix, up to 16 parts to join and more, blocks of 16 and 128 columns; the slots behind the prefix and the lengths hold NaN scales."""
     torch = gpu
     lens = [1 + (53 * b) % 300 for b in range(seqs)]
     prefix = some_layer(torch, 1, nkv, hd, prefix_len)
