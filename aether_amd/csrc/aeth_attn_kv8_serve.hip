@@ -130,8 +130,9 @@ __global__ void __launch_bounds__(256) k_attn8_join_few(A8 P, int cw, A8 O) {
 #pragma unroll
     for (int k = 0; k < MOST; k++)
         if (k < all) {
-            const bool in = k < live && ml[k].x != -INFINITY;
-            const float w = __builtin_amdgcn_exp2f(ml[k].x - M);
+            // (a part whose visible scores are all NaN has the maximum -Inf and the sum NaN, and 0·NaN keeps it; one that sees nothing adds 0·0)
+            const bool in = k < live;
+            const float w = ml[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - M);
             S += in ? w * ml[k].y : 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[e] += in ? v[k][e] * w : 0.0f;
