@@ -247,15 +247,17 @@ __device__ __forceinline__ float2 sv_column(const A8& A, int len, int seq, int h
     const int live = max(1, (end - beg + A.tpc - 1) / A.tpc), lane = threadIdx.x & 63;
     const int64_t step = 16 * (HD + 2);
     const float* st = A.ws + (unit * A.ncb + x / 16) * A.chunks * step + 16 * HD + 2 * (x % 16);
+    // (a part whose visible scores are all NaN has the maximum -Inf and the sum NaN: 0·NaN keeps it)
+    auto weight = [](float x, float m) { return x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m); };
     float2 ml = make_float2(-INFINITY, 0.0f);
     for (int k = lane; k < live; k += 64) {
         const float2 more = *(const float2*)(st + k * step);
         const float m = fmaxf(ml.x, more.x);
-        ml.y = (ml.x == -INFINITY ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - m)) + (more.x == -INFINITY ? 0.0f : more.y * __builtin_amdgcn_exp2f(more.x - m));
+        ml.y = ml.y * weight(ml.x, m) + more.y * weight(more.x, m);
         ml.x = m;
     }
     const float M = aeth_wave_max(ml.x);
-    const float S = aeth_wave_sum(ml.x == -INFINITY ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - M));
+    const float S = aeth_wave_sum(ml.y * weight(ml.x, M));
     return make_float2(M, 1.0f / S);
 }
 
