@@ -1,0 +1,70 @@
+"""The forms of the serving calls over the 8-bit cache that take many columns, at shapes that are reckoned to take them on
+256 CUs: a prefix in blocks of 128 columns; against 64 bits (tests/_kv8_serve.py)."""
+import math
+
+import pytest
+
+from tests import _kv8_serve as S
+from tests.test_gpu_kv8 import rand, some_layer, within
+from tests.test_gpu_kv8_serve import ints, shared, some_layers
+
+pytestmark = pytest.mark.gpu
+
+
+def no_numbers(torch, layer, hd, slots):
+    """NaN as the scales of a range of slots, in every head of a layer slice."""
+    for at in (128 * hd, 128 * hd + 256):
+        scales = layer[..., at:at + 256].contiguous().view(torch.float32)  # [heads][tiles][64]
+        scales.reshape(len(layer), -1)[:, slots.start:slots.stop] = math.nan
+        layer[..., at:at + 256] = scales.view(torch.uint8)
+
+
+def apart(torch, x):
+    """The same rows at an odd address and stride."""
+    buf = torch.zeros(x.shape[0] * (x.shape[1] + 3) + 1, device="cuda")
+    rows = torch.as_strided(buf, x.shape, (x.shape[1] + 3, 1), 1)
+    rows.copy_(x)
+    return rows
+
+
+# ── a shared prefix in blocks of 128 columns ──────────────────────────────
+
+# (head_dim, sequences, KV heads, query heads of each, prefix, window), with what is joined: parts of the prefix. Columns fill no whole number of
+# blocks but in the last two.
+BLOCKS = [(128, 17, 64, 32, 64, 0),      # 1
+          (128, 17, 8, 32, 6001, 0),     # 6
+          (64, 33, 4, 32, 12001, 0),     # 7
+          (128, 33, 2, 32, 12001, 0),    # 12
+          (64, 65, 2, 32, 20001, 0),     # 14
+          (128, 33, 4, 3, 80001, 0),     # 63, less than one block
+          (64, 100, 1, 8, 80001, 0),     # 35
+          (128, 17, 64, 32, 500, 250),   # 1, and windows that leave the prefix
+          (128, 17, 8, 32, 12001, 9001),  # 6
+          (64, 33, 4, 32, 20001, 12001),  # 7
+          (128, 17, 4, 32, 30001, 20001),  # 12
+          (64, 65, 2, 32, 30001, 20001),  # 14
+          (128, 160, 8, 4, 6000, 0),     # 6
+          (128, 160, 8, 4, 10000, 8000)]
+
+
+@pytest.mark.parametrize("hd,seqs,nkv,g,prefix_len,window", BLOCKS)
+def test_shared_prefix_in_blocks_of_128_columns(gpu, hd, seqs, nkv, g, prefix_len, window):
+    """Windows begin in different tiles of the prefix; what no window reaches and the slots behind the prefix and the lengths hold NaN scales."""
+    torch = gpu
+    own = 300
+    lens = [(53 * b) % (own + 1) for b in range(seqs)]
+    prefix, layers = some_layer(torch, 1, nkv, hd, prefix_len), some_layers(torch, 9, seqs, nkv, hd, own)
+    no_numbers(torch, prefix, hd, range(prefix_len, -(-prefix_len // 64) * 64))
+    if window:
+        no_numbers(torch, prefix, hd, range(0, prefix_len - window))
+    for b in range(seqs):
+        no_numbers(torch, layers[b], hd, range(lens[b], 320))
+    q = rand(torch, 2, seqs, nkv * g * hd)
+    got = shared(torch, q, prefix, prefix_len, prefix_len, layers, ints(torch, lens), nkv, hd, own, own, window)
+    assert not got.isnan().any()
+    pick = sorted({b * (seqs - 1) // 7 for b in range(8)})
+    want, bound = S.shared(q[pick].contiguous(), prefix, prefix_len, prefix_len, layers[pick], [lens[b] for b in pick], nkv, hd, own, window)
+    within(torch, got[pick], want, bound)
+    out = torch.full((q.numel() + 1,), math.nan, device="cuda")[1:].reshape(q.shape)
+    again = shared(torch, apart(torch, q), prefix, prefix_len, prefix_len, layers, ints(torch, lens), nkv, hd, own, own, window, out=out)
+    assert torch.equal(again, got)
