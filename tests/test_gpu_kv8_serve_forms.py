@@ -1,12 +1,13 @@
 """The forms of the serving calls over the 8-bit cache that take many columns, at shapes that are reckoned to take them on
-256 CUs: a prefix in blocks of 128 columns; against 64 bits (tests/_kv8_serve.py)."""
+256 CUs: a prefix in blocks of 128 columns, and the weights of tokens behind the attention in blocks of 128 and 256; against
+64 bits (tests/_kv8_serve.py)."""
 import math
 
 import pytest
 
 from tests import _kv8_serve as S
 from tests.test_gpu_kv8 import rand, some_layer, within
-from tests.test_gpu_kv8_serve import ints, shared, some_layers
+from tests.test_gpu_kv8_serve import ints, shared, some_layers, weigh
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +69,56 @@ def test_shared_prefix_in_blocks_of_128_columns(gpu, hd, seqs, nkv, g, prefix_le
     out = torch.full((q.numel() + 1,), math.nan, device="cuda")[1:].reshape(q.shape)
     again = shared(torch, apart(torch, q), prefix, prefix_len, prefix_len, layers, ints(torch, lens), nkv, hd, own, own, window, out=out)
     assert torch.equal(again, got)
+
+
+# ── token weights behind the attention in blocks of many columns ──────────
+
+# (head_dim, queries, tokens, KV heads, query heads of each, window), with the attention's columns of a block and chunks
+COLUMNS = [(128, 701, 701, 8, 8, 0),       # 128, 1
+           (128, 2000, 2000, 8, 4, 0),     # 128, 1
+           (128, 1000, 1000, 4, 8, 500),   # 128, 1
+           (128, 150, 8001, 16, 4, 0),     # 128, 4
+           (128, 70, 20001, 8, 8, 10000),  # 128, 7
+           (128, 300, 20001, 4, 1, 0),     # 128, 20
+           (128, 150, 150, 8, 32, 0),      # 256, 1
+           (128, 1000, 1500, 4, 16, 700),  # 256, 1
+           (128, 150, 2001, 4, 32, 0),     # 256, 4
+           (128, 70, 8001, 8, 8, 4000),    # 256, 8
+           (128, 40, 20001, 1, 64, 0),     # 256, 20
+           (128, 300, 8001, 4, 4, 4000),   # 256, 9
+           (64, 301, 301, 8, 32, 0),       # 128, 1
+           (64, 1000, 1500, 4, 16, 700),   # 128, 1
+           (64, 33, 4001, 8, 32, 0),       # 128, 4
+           (64, 70, 20001, 8, 8, 10000),   # 128, 7
+           (64, 700, 8001, 1, 4, 0),       # 128, 11
+           (64, 150, 40001, 2, 4, 20000)]  # 128, 20
+
+
+@pytest.mark.parametrize("hd,n,seq,nkv,g,window", COLUMNS)
+def test_weights_behind_blocks_of_many_columns(gpu, hd, n, seq, nkv, g, window):
+    """What no query sees holds NaN scales; then with a query that is NaN, at an odd address."""
+    torch = gpu
+    dark = max(0, seq - n + 1 - window) if window else 0
+    layer = some_layer(torch, n, nkv, hd, seq)
+    no_numbers(torch, layer, hd, range(seq, -(-seq // 64) * 64))
+    no_numbers(torch, layer, hd, range(0, dark))
+    q, prior = rand(torch, seq, n, nkv * g * hd), rand(torch, 5, nkv, seq).abs()
+    out, w = weigh(torch, q, layer, nkv, hd, seq, seq, window, prior)
+    o, ot, ww, wt = S.weights(q, layer, nkv, hd, seq, seq, window, prior)
+    within(torch, out, o, ot)
+    within(torch, w, ww, wt)
+    assert torch.equal(w[:, :dark], prior[:, :dark])
+    # a query head of the second KV head, or of the only one
+    i, head = n // 2, (g if nkv > 1 else 0) + g // 2
+    q[i, head * hd + 5] = math.nan
+    out, w = weigh(torch, apart(torch, q), layer, nkv, hd, seq, seq, window, prior)
+    fine = torch.ones((n, nkv * g), dtype=torch.bool, device="cuda")
+    fine[i, head] = False
+    at = fine.repeat_interleave(hd, 1)
+    assert out[~at].isnan().all()
+    within(torch, out[at], o[at], ot[at])
+    end = seq - n + i + 1
+    lit = torch.ones((nkv, seq), dtype=torch.bool, device="cuda")
+    lit[head // g, max(0, end - window) if window else 0:end] = False
+    assert w[~lit].isnan().all()
+    within(torch, w[lit], ww[lit], wt[lit])
