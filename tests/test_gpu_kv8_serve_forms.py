@@ -1,13 +1,14 @@
 """The forms of the serving calls over the 8-bit cache that take many columns, at shapes that are reckoned to take them on
-256 CUs: a prefix in blocks of 128 columns, and the weights of tokens behind the attention in blocks of 128 and 256; against
-64 bits (tests/_kv8_serve.py)."""
+256 CUs: a prefix in blocks of 128 columns, the weights of tokens behind the attention in blocks of 128 and 256, and
+four heads a thread of the rotation by several axes; against 64 bits (tests/_kv8.py, tests/_kv8_serve.py)."""
 import math
 
 import pytest
 
+import aether_amd as A
 from tests import _kv8_serve as S
-from tests.test_gpu_kv8 import rand, some_layer, within
-from tests.test_gpu_kv8_serve import ints, shared, some_layers, weigh
+from tests.test_gpu_kv8 import rand, some_layer, stream, within
+from tests.test_gpu_kv8_serve import axes_exact, axes_rope, ints, shared, some_layers, table, weigh
 
 pytestmark = pytest.mark.gpu
 
@@ -122,3 +123,33 @@ def test_weights_behind_blocks_of_many_columns(gpu, hd, n, seq, nkv, g, window):
     lit[head // g, max(0, end - window) if window else 0:end] = False
     assert w[~lit].isnan().all()
     within(torch, w[lit], ww[lit], wt[lit])
+
+
+# ── four heads a thread by several axes ───────────────────────────────────
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("nq,nk,norm", [(7, 3, "qk"), (7, 3, "q"), (7, 3, "k"), (7, 3, ""), (8, 4, "qk"), (1, 0, "q"), (0, 5, "k"), (2, 1, "qk")])
+def test_axes_of_many_rows(gpu, hd, nq, nk, norm, in_place):
+    """1024 workgroups and some more, the last one part-filled: heads in groups of four that hold both q's and k's, or end early."""
+    torch = gpu
+    n = 1024 * 256 // (-(-(nq + nk) // 4) * hd // 8) + 13
+    x = rand(torch, n, n, (nq + nk + 1) * hd)
+    qw, kw = (rand(torch, 7 + i, hd) if c in norm else None for i, c in enumerate("qk"))
+    g = torch.Generator().manual_seed(hd + nq)
+    pos = torch.randint(-3, 130, (3, n), generator=g, dtype=torch.int32).cuda()  # the table has 100 rows
+    pairs = torch.randint(0, 3, (hd // 2,), generator=g).tolist()
+    sin, cos = table(torch, 100, hd)
+    want, bound = axes_exact(x, nq, nk, hd, qw, kw, pos, pairs, sin, cos)
+    was = x.clone()
+    got = axes_rope(torch, x, nq, nk, hd, qw, kw, pos, pairs, sin, cos, out=x if in_place else None)
+    within(torch, got[:, :(nq + nk) * hd], want, bound)
+    assert torch.equal(x[:, (nq + nk) * hd:] if in_place else x, was[:, (nq + nk) * hd:] if in_place else was)
+    # axes that agree give the bits of one
+    same = pos[:1].expand(3, n).contiguous()
+    one = torch.empty((n, (nq + nk) * hd), device="cuda")
+    A.check(A.lib().aeth_qk_norm_rope(was.data_ptr(), was.shape[1], n, nq, nk, hd, qw.data_ptr() if qw is not None else None,
+                                      kw.data_ptr() if kw is not None else None, 1e-5, 0, same.data_ptr(), sin.data_ptr(), cos.data_ptr(), 100,
+                                      one.data_ptr(), one.shape[1], stream(torch)), "rope")
+    assert torch.equal(axes_rope(torch, was, nq, nk, hd, qw, kw, same, pairs, sin, cos), one)
