@@ -1,6 +1,6 @@
 """The forms of the serving calls over the 8-bit cache that take many columns, at shapes that are reckoned to take them on
-256 CUs: a prefix in blocks of 128 columns, the weights of tokens behind the attention in blocks of 128 and 256, and
-four heads a thread of the rotation by several axes; against 64 bits (tests/_kv8.py, tests/_kv8_serve.py)."""
+256 CUs: a prefix in blocks of 128 columns, the weights of tokens behind the attention in blocks of 128 and 256,
+four keys a thread of a batch's weights, and four heads a thread of the rotation by several axes; against 64 bits (tests/_kv8.py, tests/_kv8_serve.py)."""
 import math
 
 import pytest
@@ -8,7 +8,7 @@ import pytest
 import aether_amd as A
 from tests import _kv8_serve as S
 from tests.test_gpu_kv8 import rand, some_layer, stream, within
-from tests.test_gpu_kv8_serve import axes_exact, axes_rope, ints, shared, some_layers, table, weigh
+from tests.test_gpu_kv8_serve import axes_exact, axes_rope, ints, shared, some_layers, table, weigh, weigh_batch
 
 pytestmark = pytest.mark.gpu
 
@@ -123,6 +123,45 @@ def test_weights_behind_blocks_of_many_columns(gpu, hd, n, seq, nkv, g, window):
     lit[head // g, max(0, end - window) if window else 0:end] = False
     assert w[~lit].isnan().all()
     within(torch, w[lit], ww[lit], wt[lit])
+
+
+# ── a batch's token weights, four keys a thread ───────────────────────────
+
+# (head_dim, sequences, KV heads, query heads of each, longest, window), with the attention's chunks: more than 2048 pieces of 256 keys
+PIECES = [(128, 33, 8, 4, 2100, 0),     # 3, joined with all in flight
+          (256, 33, 8, 4, 2100, 0),     # 3
+          (64, 20, 8, 10, 4096, 0),     # 4
+          (128, 5, 8, 4, 14000, 0),     # 19, a workgroup a column
+          (256, 5, 8, 4, 14000, 0),     # 19
+          (64, 5, 8, 4, 14000, 0),      # 19
+          (64, 12, 8, 4, 6000, 0),      # 8
+          (256, 70, 8, 1, 1000, 0),     # 1
+          (128, 5, 8, 4, 14000, 9000),  # 18
+          (128, 40, 8, 4, 2100, 2000)]  # 1
+
+
+@pytest.mark.parametrize("hd,seqs,nkv,g,longest,window", PIECES)
+def test_batch_weights_of_four_keys_a_thread(gpu, hd, seqs, nkv, g, longest, window):
+    """Lengths at the borders of pieces and chunks, some of whose newest tokens are NaN, weights added in place."""
+    torch = gpu
+    lens = ([longest, 0, 769, 1] + [l for l in (769, 1024, 1025, 1537, 256, 255) if l <= longest] + [(613 * b) % (longest + 1) for b in range(seqs)])[:seqs]
+    bad = [b for b in (2, 3, seqs - 1) if lens[b]]
+    layers, q, prior = some_layers(torch, 3, seqs, nkv, hd, longest + 3), rand(torch, 4, seqs, nkv * g * hd), rand(torch, 5, seqs, nkv, longest + 3).abs()
+    for b in range(seqs):
+        no_numbers(torch, layers[b], hd, range(lens[b] - (b in bad), -(-(longest + 3) // 64) * 64))
+    w = prior.clone()
+    out, _ = weigh_batch(torch, q, layers, ints(torch, lens), nkv, hd, longest + 3, longest, window, w, into=w)
+    for b, seq in enumerate(lens):
+        first = max(0, seq - window) if window else 0
+        assert torch.equal(w[b, :, seq:], prior[b, :, seq:]) and torch.equal(w[b, :, :first], prior[b, :, :first])
+        if b in bad:
+            assert out[b].isnan().all() and w[b, :, first:seq].isnan().all()
+        elif seq:
+            o, ot, ww, wt = S.weights(q[b:b + 1], layers[b], nkv, hd, longest + 3, seq, window, prior[b])
+            within(torch, out[b:b + 1], o, ot)
+            within(torch, w[b, :, :seq], ww, wt)
+        else:
+            assert (out[b] == 0).all()
 
 
 # ── four heads a thread by several axes ───────────────────────────────────
