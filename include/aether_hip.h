@@ -365,7 +365,8 @@ AETH_API int64_t aeth_attn_kv8_shared_ws_bytes(int64_t n_seqs, int64_t n_heads, 
  * sequence i's own slice, whose slot j stands at position prefix_len + j. Query i sees all of
  * them or, with a window, the last `window`, which may end in the prefix. The prefix is read
  * once for many sequences. A row that sees nothing is zeros. prefix_len is taken at the call (a captured call keeps it),
- * d_lens on the stream. Numerics as for aeth_attn_kv8; the slices may not overlap d_out. */
+ * d_lens on the stream. Numerics as for aeth_attn_kv8; the slices may not overlap d_out.
+ * Unsupported: n_seqs·kv_heads·ceil(n_heads/kv_heads/16) past 2^22. */
 AETH_API int aeth_attn_kv8_shared(const float* d_q, int64_t q_stride, const void* d_prefix, int64_t prefix_seq,
                                   int64_t prefix_len, const void* d_layers, int64_t layer_stride, const int32_t* d_lens,
                                   int64_t n_seqs, int64_t n_heads, int64_t kv_heads, int64_t head_dim, int64_t max_seq,
@@ -383,13 +384,13 @@ AETH_API int64_t aeth_attn_kv8_weights_ws_bytes(int64_t n_seqs, int64_t n, int64
  * has relative error of the probabilities' (about 2^-23 of a score's terms, as in the attention) and of f32
  * sums; a query whose row is NaN makes the weights of what it sees NaN. Sums have a fixed
  * order: the same call gives the same bits again. n = 0 leaves the prior (d_q and d_out
- * may then be NULL). */
+ * may then be NULL). Unsupported: kv_heads·ceil(seq/256) + n·n_heads past 2^23. */
 AETH_API int aeth_attn_kv8_weights(const float* d_q, int64_t q_stride, const void* d_layer, int64_t n, int64_t n_heads,
                                    int64_t kv_heads, int64_t head_dim, int64_t max_seq, int64_t seq, int64_t window,
                                    float* d_out, const float* d_prior, float* d_weights, void* d_ws, int64_t ws_bytes,
                                    void* stream);
 /* The same beside aeth_attn_kv8_batch: weights [n_seqs][kv_heads][max_seq], the slots
- * below d_lens[i] of sequence i. */
+ * below d_lens[i] of sequence i. Unsupported: kv_heads·ceil(max_len/256) + n_heads past 2^23. */
 AETH_API int aeth_attn_kv8_weights_batch(const float* d_q, int64_t q_stride, const void* d_layers, int64_t layer_stride,
                                          const int32_t* d_lens, int64_t n_seqs, int64_t n_heads, int64_t kv_heads,
                                          int64_t head_dim, int64_t max_seq, int64_t max_len, int64_t window, float* d_out,
@@ -408,7 +409,8 @@ AETH_API int64_t aeth_kv8_evict_ws_bytes(int64_t n_seqs, int64_t kv_heads, int64
  * d_weights where dst_seq = max_seq, and else overlaps none of it) receives
  * [kv_heads][dst_seq] the kept tokens' weights and behind them zeros; d_kept (may be NULL)
  * [kv_heads][keep] the slots they had, ascending, and nothing behind them. What follows an eviction counts slots, not
- * positions: a window of the attention, `first` and `recent` of the next one. */
+ * positions: a window of the attention, `first` and `recent` of the next one. Unsupported: ceil(min(keep, seq)/64) +
+ * ceil(dst_seq/2048) past 2^23. */
 AETH_API int aeth_kv8_evict(const void* d_layer, const float* d_weights, int64_t kv_heads, int64_t head_dim,
                             int64_t max_seq, int64_t seq, int64_t keep, int64_t first, int64_t recent, void* d_dst,
                             float* d_dst_weights, int64_t dst_seq, int32_t* d_kept, void* d_ws, int64_t ws_bytes,

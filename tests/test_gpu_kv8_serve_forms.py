@@ -1,6 +1,7 @@
 """The forms of the serving calls over the 8-bit cache that take many columns, at shapes that are reckoned to take them on
 256 CUs: a prefix in blocks of 128 columns, the weights of tokens behind the attention in blocks of 128 and 256,
-four keys a thread of a batch's weights, and four heads a thread of the rotation by several axes; against 64 bits (tests/_kv8.py, tests/_kv8_serve.py)."""
+four keys a thread of a batch's weights, and four heads a thread of the rotation by several axes; against 64 bits (tests/_kv8.py, tests/_kv8_serve.py).
+The attentions of tests/test_gpu_kv8_serve.py take blocks of 16 columns throughout."""
 import math
 
 import pytest
